@@ -707,6 +707,69 @@ int rumpy_row_axpy(float* dst, const float* src, const float* coef, int32_t N, i
 int rumpy_moco_enqueue(float* queue, const float* keys, void* slots, void* queue_ptr, void* queue_labels, const void* labels,
                        int32_t n, int32_t key_stride, int32_t C, int32_t K, void* stream);
 
+/* ---- the joint between two residual blocks (csrc/residual_norm.hip): norm behind a block, gate, residual scale, skip, norm in front of the
+ * next block, in one launch over rows of C channels (pixels of an NHWC tensor, or tokens).  What rumpy_ca_scale is to an RCAB (out = res + gate * t),
+ * with the norms of a normalised residual network around it:
+ *   z = N_post(t) ; y = x + scale * g * z ; h = N_pre(y) ; N: 0 none, 1 layer norm, 2 root-mean-square norm, weight / bias fp32 [C] or NULL.
+ * t NULL: h = N_pre(x) alone.  x / dx / y / dy in x_fmt, the others in t_fmt: both the same RUMPY_FMT_*, or x in fp32 beside a 16-bit t.
+ * gate_mode 0: none, gate NULL; 1: fp32 [rows / group_rows, C], row r uses gate row r / group_rows; 2: [rows, C] in t_fmt.
+ * Inputs have row strides (elements; channels are contiguous, any alignment of an element); outputs are contiguous.  1 <= C <= 8192.
+ * `stats` [4][rows] (mean and factor of N_post, of N_pre) is written by the forward pass for the backward pass (NULL: not kept). */
+typedef struct {
+  const void* x; const void* t; const void* gate;
+  const float* post_w; const float* post_b; const float* pre_w; const float* pre_b;
+  void* y; void* h; float* stats;
+  int64_t rows, group_rows, ldx, ldt, ldg;
+  int32_t C, x_fmt, t_fmt, gate_mode, post, pre;
+  float scale, eps;
+} rumpy_residual_norm_args;
+int rumpy_residual_norm_fwd(const rumpy_residual_norm_args* a, void* stream);
+/* dy / dh may be NULL (no gradient arrives there); every output may be NULL (not asked for).  dgate: fp32 [rows / group_rows, C] in gate mode 1,
+ * [rows, C] in t_fmt in mode 2; parameter gradients fp32 [C], overwritten.  partial: rumpy_residual_norm_partial_floats(...) floats.  Deterministic. */
+typedef struct {
+  const void* dy; const void* dh; const void* x; const void* t; const void* gate;
+  const float* post_w; const float* post_b; const float* pre_w; const float* stats;
+  void* dx; void* dt; void* dgate;
+  float* d_post_w; float* d_post_b; float* d_pre_w; float* d_pre_b; float* partial;
+  int64_t rows, group_rows, lddy, lddh, ldx, ldt, ldg;
+  int32_t C, x_fmt, t_fmt, gate_mode, post, pre;
+  float scale;
+  int32_t pad_;
+} rumpy_residual_norm_bwd_args;
+int rumpy_residual_norm_bwd(const rumpy_residual_norm_bwd_args* a, void* stream);
+int64_t rumpy_residual_norm_partial_floats(int64_t rows, int64_t group_rows, int32_t C, int32_t gate_mode);
+
+/* ---- distillation from a teacher's top logits (csrc/distill.hip), beside rumpy_ce_rows: rows of V logits in fp32 / bf16 / fp16 with a row stride
+ * (columns contiguous, any alignment of an element), all sums in fp32, fixed orders.
+ * rumpy_top_logits: per row the k <= 256 largest logits, descending, equal ones by index (NaN counts as largest), as they are in `values`
+ * [rows, k] (the logits' format) with int64 `indices`; tail[r] = log of the sum of exp(logit * inv_tau) over all others (-inf: none). */
+typedef struct {
+  const void* logits; void* values; void* indices; float* tail;
+  int64_t rows, ld;
+  int32_t V, k, fmt;
+  float inv_tau;
+} rumpy_top_logits_args;
+int rumpy_top_logits(const rumpy_top_logits_args* a, void* stream);
+/* Cross-entropy of softmax(logits / tau) against the teacher's distribution over its listed columns, minus that distribution's entropy, times tau^2:
+ *   l = tau^2 [ sum_i p_i (log p_i - log q_i) + p_t (log p_t - log q_t) ]
+ * p = softmax(top_values / tau) over the entries of a row with index >= 0; with `tail` (as rumpy_top_logits makes it, at the same temperature) the
+ * unlisted columns are one more outcome t.  A column that is listed twice takes both shares; an index >= V makes the row NaN; rows whose entries
+ * are all unused or -inf give 0.  row_weight [rows] or NULL: weights, 0 = the row is not looked at.
+ * row_loss [rows] = weight * l.  loss (or NULL): their sum (mean = 0) or sum / sum of weights (mean = 1; weights that sum to 0: 0).
+ * state [rows][8], factor [1]: kept for the backward pass; partial: rumpy_distill_partial_floats(rows, V) floats (0: NULL).
+ * backward: dlogits [rows, V] contiguous in the logits' format; gout = the gradient of `loss` [1], or of row_loss [rows] when loss is NULL. */
+typedef struct {
+  const void* logits; const void* top_values; const void* top_indices; const float* tail; const float* row_weight;
+  float* row_loss; float* state; float* loss; float* factor; float* partial;
+  const float* gout; void* dlogits;
+  int64_t rows, ld;
+  int32_t V, k, fmt, value_fmt, index64, mean;
+  float tau, inv_tau;
+} rumpy_distill_args;
+int rumpy_distill_fwd(const rumpy_distill_args* a, void* stream);
+int rumpy_distill_bwd(const rumpy_distill_args* a, void* stream);
+int64_t rumpy_distill_partial_floats(int64_t rows, int32_t V);
+
 /* ---- optimizer: torch.optim.Adam semantics (base_architecture.py:93-95,437), flat fp32 buffers ---- */
 typedef struct {
   float lr, beta1, beta2, eps;

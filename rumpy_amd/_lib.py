@@ -309,6 +309,34 @@ class SgemmArgs(_S):
                 ('alpha', c_float), ('leaky_slope', c_float), ('accumulate', c_int32), ('pad_', c_int32)]
 
 
+class ResidualNormArgs(_S):
+    _fields_ = [('x', c_void_p), ('t', c_void_p), ('gate', c_void_p), ('post_w', c_void_p), ('post_b', c_void_p), ('pre_w', c_void_p), ('pre_b', c_void_p), ('y', c_void_p), ('h', c_void_p), ('stats', c_void_p),
+                ('rows', c_int64), ('group_rows', c_int64), ('ldx', c_int64), ('ldt', c_int64), ('ldg', c_int64),
+                ('C', c_int32), ('x_fmt', c_int32), ('t_fmt', c_int32), ('gate_mode', c_int32), ('post', c_int32), ('pre', c_int32),
+                ('scale', c_float), ('eps', c_float)]
+
+
+class ResidualNormBwdArgs(_S):
+    _fields_ = [('dy', c_void_p), ('dh', c_void_p), ('x', c_void_p), ('t', c_void_p), ('gate', c_void_p), ('post_w', c_void_p), ('post_b', c_void_p), ('pre_w', c_void_p), ('stats', c_void_p),
+                ('dx', c_void_p), ('dt', c_void_p), ('dgate', c_void_p),
+                ('d_post_w', c_void_p), ('d_post_b', c_void_p), ('d_pre_w', c_void_p), ('d_pre_b', c_void_p), ('partial', c_void_p),
+                ('rows', c_int64), ('group_rows', c_int64), ('lddy', c_int64), ('lddh', c_int64), ('ldx', c_int64), ('ldt', c_int64), ('ldg', c_int64),
+                ('C', c_int32), ('x_fmt', c_int32), ('t_fmt', c_int32), ('gate_mode', c_int32), ('post', c_int32), ('pre', c_int32),
+                ('scale', c_float), ('pad_', c_int32)]
+
+
+class TopLogitsArgs(_S):
+    _fields_ = [('logits', c_void_p), ('values', c_void_p), ('indices', c_void_p), ('tail', c_void_p), ('rows', c_int64), ('ld', c_int64), ('V', c_int32), ('k', c_int32), ('fmt', c_int32),
+                ('inv_tau', c_float)]
+
+
+class DistillArgs(_S):
+    _fields_ = [('logits', c_void_p), ('top_values', c_void_p), ('top_indices', c_void_p), ('tail', c_void_p), ('row_weight', c_void_p),
+                ('row_loss', c_void_p), ('state', c_void_p), ('loss', c_void_p), ('factor', c_void_p), ('partial', c_void_p), ('gout', c_void_p), ('dlogits', c_void_p),
+                ('rows', c_int64), ('ld', c_int64),
+                ('V', c_int32), ('k', c_int32), ('fmt', c_int32), ('value_fmt', c_int32), ('index64', c_int32), ('mean', c_int32), ('tau', c_float), ('inv_tau', c_float)]
+
+
 # every symbol include/rumpy_amd.h declares: name -> (restype, argtypes)
 _P = C.POINTER
 SYMBOLS = {
@@ -342,6 +370,13 @@ SYMBOLS = {
     'rumpy_l2norm_rows': (C.c_int, [c_void_p, c_void_p, c_void_p, c_int32, c_int32, c_void_p]),
     'rumpy_l2norm_rows_bwd': (C.c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int32, c_int32, c_void_p]),
     'rumpy_rowdot': (C.c_int, [c_void_p, c_void_p, c_void_p, c_int32, c_int32, c_int32, c_float, c_void_p]),
+    'rumpy_residual_norm_fwd': (C.c_int, [_P(ResidualNormArgs), c_void_p]),
+    'rumpy_residual_norm_bwd': (C.c_int, [_P(ResidualNormBwdArgs), c_void_p]),
+    'rumpy_residual_norm_partial_floats': (c_int64, [c_int64, c_int64, c_int32, c_int32]),
+    'rumpy_top_logits': (C.c_int, [_P(TopLogitsArgs), c_void_p]),
+    'rumpy_distill_fwd': (C.c_int, [_P(DistillArgs), c_void_p]),
+    'rumpy_distill_bwd': (C.c_int, [_P(DistillArgs), c_void_p]),
+    'rumpy_distill_partial_floats': (c_int64, [c_int64, c_int32]),
     'rumpy_label_match': (C.c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int32, c_int32, c_void_p]),
     'rumpy_pos_vector': (C.c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int32, c_int32, c_int32, c_float, c_void_p]),
     'rumpy_ce_rows': (C.c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int32, c_int32, c_void_p]),

@@ -49,3 +49,17 @@ class SupConLoss(nn.Module):
         log_prob = sim - torch.log((torch.exp(sim) * not_self).sum(1, keepdim=True) + 1e-6)
         mean_log_prob_pos = (positives * log_prob).sum(1) / positives.sum(1)
         return (-(self.temperature / self.base_temperature) * mean_log_prob_pos).view(anchors, bsz).mean()
+
+
+class TopLogitsDistillLoss(nn.Module):
+    """Distillation from a teacher's top logits, forward and backward in HIP (``rumpy_amd.distill.distill_loss``; the reference has no such
+    loss): call with the student's logits [..., V] and what ``rumpy_amd.distill.top_logits`` made of the teacher's."""
+
+    def __init__(self, temperature=1.0, reduction='mean'):
+        super(TopLogitsDistillLoss, self).__init__()
+        self.temperature = temperature
+        self.reduction = reduction
+
+    def forward(self, logits, top_values, top_indices, tail=None, row_weight=None):
+        from rumpy_amd.distill import distill_loss
+        return distill_loss(logits, top_values, top_indices, tail=tail, temperature=self.temperature, row_weight=row_weight, reduction=self.reduction)

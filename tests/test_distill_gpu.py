@@ -1,0 +1,419 @@
+"""top_logits and distill_loss on the GPU against their definitions in 64 bits.
+
+Tolerances.  With u = z / T, the exponent of a column is off by a few roundings (2^-24) of |u - max u| (the product with log2(e) / T, both
+rounded, and the exponential's own last bits), and a row's sum by as many roundings as it has joining steps, at most V / 4096 pieces of 8 per thread and
+13 more: E = 2^-24 (8 max|u - max u| + 64 + V / 256) relative for a probability, absolute for a logarithm.  A stored gradient adds half a step of its
+type (bf16 2^-8, fp16 2^-11 and at least 2^-25, fp32 2^-24, relative).  The exponential gives 0 where its result lies under the smallest normal
+number: a column's q and p may each be off by 2^-126 for that, its gradient by 2 x 2^-126 times the row's factor (T, weight, upstream)."""
+import math
+
+import pytest
+import torch
+
+from rumpy_amd.distill import distill_loss, top_logits
+from rumpy_amd.sr_tools.loss_functions import TopLogitsDistillLoss
+
+pytestmark = pytest.mark.gpu
+DEV = 'cuda:0'
+U24 = 2.0 ** -24
+STEP = {torch.float32: 2.0 ** -24, torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}
+F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
+LOWEST = {t: torch.finfo(t).min for t in STEP}
+INF, NAN = math.inf, math.nan
+
+
+# ---------------------------------------------------------------------------------------------------------------- top_logits
+def _top_reference(z, k, tau):
+    values, order = torch.sort(z.double() + 0.0, dim=-1, descending=True, stable=True)         # NaN first, equal values by index
+    rest = values[..., k:] / tau
+    tail = torch.logsumexp(rest, -1) if rest.shape[-1] else torch.full(z.shape[:-1], -INF, dtype=torch.float64)
+    return order[..., :k], tail
+
+
+def _check_top(z, k, tau):
+    values, indices, tail = top_logits(z, k, temperature=tau)
+    zc = z.cpu()
+    order, want = _top_reference(zc, k, tau)
+    assert indices.dtype == torch.int64 and values.dtype == z.dtype and tail.dtype == F32
+    assert torch.equal(indices.cpu(), order)
+    got = torch.gather(zc, -1, order)
+    assert torch.equal(values.cpu().nan_to_num(7.0, 8.0, 9.0), got.nan_to_num(7.0, 8.0, 9.0))
+    tail = tail.double().cpu()
+    finite = torch.isfinite(want)
+    assert torch.equal(torch.isnan(tail), torch.isnan(want)) and torch.equal(tail[~finite].nan_to_num(1.0), want[~finite].nan_to_num(1.0))
+    if finite.any():
+        u = torch.where(torch.isfinite(zc.double()), zc.double() / tau, torch.zeros((), dtype=torch.float64))
+        mag = u.abs().amax(-1)
+        tol = U24 * (8 * mag + 64 + zc.shape[-1] / 256) + U24 * want.abs()
+        assert ((tail - want).abs() <= tol)[finite].all(), float(((tail - want).abs() / tol)[finite].max())
+
+
+@pytest.mark.parametrize('dtype', [F32, BF16, F16], ids=str)
+@pytest.mark.parametrize('rows,cols,ks', [(3, 1, (1,)), (2, 2, (1, 2)), (5, 63, (1, 63)), (4, 300, (5, 256)), (3, 512, (1, 256)), (3, 513, (1, 7, 256)), (5, 1000, (64, 256)),
+                                          (3, 4095, (100,)), (3, 4096, (100, 256)), (2, 8192, (64,)), (33, 8193, (64,)), (2, 50021, (1, 256)),
+                                          (1, 262144, (17, 256)), (700, 600, (8,))])
+def test_top_logits_over_sizes(rows, cols, ks, dtype):
+    g = torch.Generator().manual_seed(rows * cols)
+    z = torch.randn(rows, cols, generator=g).mul(3).to(dtype).to(DEV)
+    for k in ks:
+        for tau in (1.0, 0.07, 4.0):
+            _check_top(z, k, tau)
+
+
+@pytest.mark.parametrize('cols', [200, 900, 5000, 70001])
+def test_top_logits_with_equal_values(cols):
+    """rows that are constant, of few distinct values, ascending, descending; zeros of both signs"""
+    j = torch.arange(cols, dtype=F32)
+    g = torch.Generator().manual_seed(cols)
+    z = torch.stack([torch.full((cols,), 2.5), j % 3, j / cols, -j / cols, torch.where(j % 2 == 0, 0.0, -0.0),
+                     torch.randint(0, 40, (cols,), generator=g).float(), (j >= cols - 70).float(), (j < 70).float()])
+    for dtype in (F32, BF16):
+        for k in (1, 64, 200):
+            _check_top(z.to(dtype).to(DEV), k, 1.0)
+
+
+@pytest.mark.parametrize('cols', [300, 3000, 20000])
+@pytest.mark.parametrize('dtype', [F32, BF16, F16], ids=str)
+def test_top_logits_with_masks_and_odd_values(cols, dtype):
+    g = torch.Generator().manual_seed(cols)
+    base = torch.randn(12, cols, generator=g)
+    z = base.clone()
+    z[0, 50:] = -INF                        # fewer finite values than k
+    z[1, 100:] = LOWEST[dtype]
+    z[2] = -INF                             # nothing at all
+    z[3] = LOWEST[dtype]
+    z[4, 17] = NAN
+    z[5, [3, 250]] = INF
+    z[6, torch.randperm(cols, generator=g)[:280]] = INF       # more than k
+    z[7, ::2] = -INF
+    z[8, torch.randperm(cols, generator=g)[:290]] = NAN
+    z[9, 64:] = -INF                        # exactly k
+    z[10, 64:] -= 300.0                     # a gap that no 32-bit exponential spans
+    z[11, 100:] -= 300.0
+    z = z.to(dtype).to(DEV)
+    for tau in (1.0, 4.0):
+        _check_top(z, 64, tau)
+
+
+def test_top_logits_of_slices_and_leading_dimensions():
+    g = torch.Generator().manual_seed(8)
+    wide = torch.randn(6, 8200, generator=g).to(DEV)
+    _check_top(wide[:, 1:], 64, 0.07)
+    _check_top(wide[:, 3:8003].to(BF16)[:, 5:], 10, 1.0)
+    _check_top(torch.randn(2, 3, 4, 700, generator=g).to(DEV), 9, 1.0)
+    _check_top(torch.randn(900, 4, generator=g).to(DEV).t(), 9, 1.0)
+    _check_top(torch.randn(1, 700, generator=g).to(DEV).expand(5, 700), 9, 1.0)
+    _check_top(torch.randn(700, generator=g).to(DEV), 9, 1.0)
+    for shape in ((0, 700), (3, 0, 700)):
+        values, indices, tail = top_logits(torch.zeros(shape, device=DEV), 5)
+        assert values.shape == indices.shape == torch.Size(shape[:-1] + (5,)) and tail.shape == torch.Size(shape[:-1])
+
+
+def test_offsets_beyond_32_bits():
+    cols, stride = 3000, 2 ** 31 + 9
+    buf = torch.empty(2 * stride + cols, dtype=BF16, device=DEV)
+    z = buf.as_strided((3, cols), (stride, 1))
+    g = torch.Generator().manual_seed(4)
+    z.copy_(torch.randn(3, cols, generator=g).to(BF16))
+    _check_top(z, 20, 1.0)
+    values, indices, tail = top_logits(z, 20)
+    near = z.clone()
+    assert torch.equal(distill_loss(z, values, indices, tail=tail, reduction='none'), distill_loss(near, values, indices, tail=tail, reduction='none'))
+
+
+# ---------------------------------------------------------------------------------------------------------------- distill_loss
+def _loss_reference(z, values, indices, tail, tau, weight, upstream):
+    """64 bits: weighted row losses, d (upstream . row losses) / d z, and the relative error E of a probability of each row"""
+    rows, cols = z.shape
+    u = z.double() / tau
+    used = indices >= 0
+    idx = indices.clamp(min=0).long()
+    v = torch.where(used, values.double() / tau, torch.full((), -INF, dtype=torch.float64))
+    listed = torch.zeros(rows, cols, dtype=torch.bool)
+    for r in range(rows):
+        listed[r, idx[r][used[r]]] = True
+    lse = torch.logsumexp(u, 1, keepdim=True)
+    lq = u - lse
+    parts = v if tail is None else torch.cat([v, tail.double()[:, None]], 1)
+    total = torch.logsumexp(parts, 1, keepdim=True)
+    says = total[:, 0] > -INF
+    lp = parts - torch.where(says[:, None], total, torch.zeros((), dtype=torch.float64))
+    p = torch.exp(lp)
+    lqs = torch.gather(lq, 1, idx)
+    if tail is not None:
+        rest = torch.where(listed, torch.full((), -INF, dtype=torch.float64), u)
+        lrest = torch.logsumexp(rest, 1, keepdim=True)
+        lqs = torch.cat([lqs, lrest - lse], 1)
+    terms = torch.where(p > 0, p * (lp - lqs), torch.zeros((), dtype=torch.float64))
+    loss = tau ** 2 * terms.sum(1)
+    q = torch.exp(lq)
+    share = torch.zeros(rows, cols, dtype=torch.float64).scatter_add_(1, idx, torch.where(used, p[:, :idx.shape[1]], torch.zeros((), dtype=torch.float64)))
+    grad = q - share
+    mag = q + share
+    if tail is not None:
+        r = torch.exp(rest - lrest)
+        pt = p[:, -1:]
+        qt = torch.exp(lrest - lse)
+        r = torch.where(torch.isfinite(lrest), r, torch.zeros_like(r))
+        grad = torch.where(listed, grad, r * (qt - pt))
+        mag = torch.where(listed, mag, r * (qt + pt))
+    live = says & (weight != 0)
+    loss = torch.where(live, loss * weight, torch.zeros_like(loss))
+    scale = torch.where(live, tau * weight * upstream, torch.zeros_like(loss))[:, None]
+    grad = torch.where(live[:, None], grad * scale, torch.zeros_like(grad))
+    mag = torch.where(live[:, None], mag * scale.abs(), torch.zeros_like(mag))
+    fin = torch.isfinite(u)
+    span = torch.where(fin, u, torch.full((), -INF, dtype=torch.float64)).amax(1) - torch.where(fin, u, torch.full((), INF, dtype=torch.float64)).amin(1)
+    vfin = torch.where(torch.isfinite(v), v, torch.zeros_like(v))
+    span = torch.nan_to_num(span, 0.0, 0.0, 0.0).clamp(min=0) + (vfin.amax(1) - vfin.amin(1)) + (0 if tail is None else torch.nan_to_num(tail.double(), 0, 0, 0).abs() + vfin.abs().amax(1))
+    return loss, grad, mag, U24 * (8 * span + 64 + cols / 256), 2 * 2.0 ** -126 * scale.abs()
+
+
+def _teacher(z, k, tau, rest, g):
+    t = (z.double() + 0.5 * torch.randn(z.shape, generator=g)).float()
+    v, i = torch.sort(t, dim=1, descending=True, stable=True)
+    tail = torch.logsumexp(v[:, k:].double() / tau, 1).float() if rest else None
+    return v[:, :k].contiguous(), i[:, :k].contiguous(), tail
+
+
+def _check_loss(z, values, indices, tail, tau, weight=None, lay=lambda t: t):
+    """all three reductions, each with its gradient; z on the CPU"""
+    rows = z.shape[0]
+    w = torch.ones(rows, dtype=torch.float64) if weight is None else weight.double()
+    dev = lambda t: None if t is None else t.to(DEV)
+    for reduction in ('none', 'sum', 'mean'):
+        zd = lay(z.to(DEV)).detach().requires_grad_()
+        got = distill_loss(zd, dev(values), dev(indices), tail=dev(tail), temperature=tau, row_weight=dev(weight), reduction=reduction)
+        f = 1.0 if reduction != 'mean' else (1.0 / float(w.sum()) if float(w.sum()) else 0.0)
+        # a loss scale, as 16-bit floats of 5 exponent bits need it
+        up = torch.linspace(0.5, 2.0, rows).mul(32) if reduction == 'none' else torch.tensor(64.0 * rows)
+        grad, = torch.autograd.grad(got, zd, up.to(DEV))
+        loss, want, mag, err, tiny = _loss_reference(z, values, indices, tail, tau, w, up.float().double() * f)
+        tol_rows = tau ** 2 * w.abs() * 3 * err + 16 * U24 * loss.abs()
+        finite = torch.isfinite(loss)
+        if reduction == 'none':
+            assert got.shape == torch.Size([rows])
+            res = got.detach().double().cpu()
+            assert torch.equal(torch.isnan(res), torch.isnan(loss)) and torch.equal(res[~finite].nan_to_num(1.0), loss[~finite].nan_to_num(1.0))
+            assert ((res - loss).abs() <= tol_rows)[finite].all()
+        elif finite.all():
+            tol = f * float(tol_rows.sum() + rows * U24 * loss.abs().sum())
+            assert abs(float(got.detach()) - f * float(loss.sum())) <= tol, (float(got), f * float(loss.sum()), tol)
+        assert grad.dtype == z.dtype and grad.shape == z.shape
+        grad = grad.double().cpu()
+        step = STEP[z.dtype]
+        tol = (step * want.abs() + 3 * err[:, None] * mag) * (1 + step) + (2.0 ** -25 if z.dtype == F16 else 2.0 ** -126) + tiny
+        assert torch.equal(torch.isnan(grad), torch.isnan(want))
+        ok = torch.isnan(want) | ((grad - want).abs() <= tol)
+        assert bool(ok.all()), (reduction, int((~ok).sum()), float(((grad - want).abs() / tol)[~ok].max()))
+
+
+@pytest.mark.parametrize('dtype', [F32, BF16, F16], ids=str)
+@pytest.mark.parametrize('rest', [False, True])
+@pytest.mark.parametrize('rows,cols,k', [(1, 1, 1), (3, 2, 1), (4, 7, 7), (5, 100, 64), (3, 256, 256), (6, 4095, 17), (4, 4097, 1), (8, 8192, 64), (3, 8193, 256),
+                                         (2, 40001, 100), (1, 300000, 256), (70, 1000, 5)])
+def test_loss_and_gradient_over_sizes(rows, cols, k, rest, dtype):
+    g = torch.Generator().manual_seed(rows + cols + k)
+    z = torch.randn(rows, cols, generator=g).mul(3).to(dtype)
+    for tau in (1.0, 0.2, 4.0):
+        values, indices, tail = _teacher(z, k, tau, rest, g)
+        _check_loss(z, values.to(dtype), indices if tau == 1.0 else indices.int(), tail, tau)
+
+
+@pytest.mark.parametrize('rest', [False, True])
+def test_padded_rows_are_not_looked_at(rest):
+    g = torch.Generator().manual_seed(2)
+    for cols in (900, 20000):               # whole rows, and rows that are cut
+        z = torch.randn(6, cols, generator=g)
+        values, indices, tail = _teacher(z, 16, 1.0, rest, g)
+        z[1], z[4] = NAN, INF
+        values[4] = NAN
+        weight = torch.tensor([1.0, 0.0, 0.5, 2.0, 0.0, 1.0])
+        _check_loss(z.nan_to_num(0.0, 0.0, 0.0) * (weight[:, None] != 0), values.nan_to_num(0.0), indices, tail, 1.0, weight)
+        zd = z.to(DEV).requires_grad_()
+        out = distill_loss(zd, values.to(DEV), indices.to(DEV), tail=None if tail is None else tail.to(DEV), row_weight=weight.to(DEV))
+        grad, = torch.autograd.grad(out, zd)
+        assert torch.isfinite(out) and torch.isfinite(grad).all() and float(grad[[1, 4]].abs().sum()) == 0
+        zd = z.to(DEV).requires_grad_()
+        out = distill_loss(zd, values.to(DEV), indices.to(DEV), row_weight=torch.zeros(6, device=DEV))
+        assert float(out.detach()) == 0 and float(torch.autograd.grad(out, zd)[0].abs().sum()) == 0
+
+
+@pytest.mark.parametrize('rest', [False, True])
+@pytest.mark.parametrize('cols', [500, 20000])
+def test_unused_doubled_and_empty_entries(rest, cols):
+    g = torch.Generator().manual_seed(3)
+    z = torch.randn(7, cols, generator=g)
+    values, indices, tail = _teacher(z, 12, 1.0, rest, g)
+    indices[0, 4:] = -1                     # fewer entries than k
+    indices[1, 5] = indices[1, 2]           # the same column twice, and three times
+    indices[2, 1:3] = indices[2, 0]
+    values[3] = -INF                        # only the rest, or nothing
+    indices[4] = -1
+    values[5, 3:] = -INF
+    if tail is not None:
+        tail[4] = -INF                      # nothing at all
+        tail[6] = -INF                      # no rest
+    _check_loss(z, values, indices, tail, 1.0)
+
+
+@pytest.mark.parametrize('rest', [False, True])
+@pytest.mark.parametrize('dtype', [F32, BF16, F16], ids=str)
+def test_masked_columns_and_wide_gaps(rest, dtype):
+    g = torch.Generator().manual_seed(5)
+    cols = 1500
+    z = torch.randn(6, cols, generator=g)
+    for mask in (-INF, LOWEST[dtype]):
+        m = z.clone()
+        m[0, 300:] = mask                   # the student's mask; the teacher lists what is left
+        m[1, ::2] = mask
+        m[2, 40] += 400.0                   # one column holds everything
+        m[3] += 300.0                       # far from zero
+        m[4] -= 300.0
+        values, indices, tail = _teacher(torch.where(m.abs() > 1e4, torch.full((), -1e4), m), 8, 1.0, rest, g)
+        _check_loss(m.to(dtype), values, indices, tail, 1.0)
+
+
+def test_rows_that_cannot_be_answered_are_nan_alone():
+    g = torch.Generator().manual_seed(6)
+    z = torch.randn(6, 700, generator=g)
+    values, indices, tail = _teacher(z, 9, 1.0, True, g)
+    indices[1, 3] = 700                     # no such column
+    z[2, 11] = NAN
+    values[3, 2] = NAN
+    z[4] = -INF
+    for t in (None, tail):
+        zd = z.to(DEV).requires_grad_()
+        rows = distill_loss(zd, values.to(DEV), indices.to(DEV), tail=None if t is None else t.to(DEV), reduction='none')
+        grad, = torch.autograd.grad(rows.sum(), zd)
+        nan = torch.isnan(rows).cpu().tolist()
+        assert nan == [False, True, True, True, True, False]
+        assert torch.isfinite(grad[[0, 5]]).all() and torch.isnan(grad[[1, 3]]).all()
+
+
+def test_a_listed_column_that_the_student_excludes_costs_everything():
+    z = torch.zeros(1, 600)
+    z[0, 5] = -INF
+    v, i = torch.tensor([[1.0, 0.5]]), torch.tensor([[5, 6]])
+    assert float(distill_loss(z.to(DEV), v.to(DEV), i.to(DEV))) == INF
+    v[0, 0] = -INF                          # ... unless the teacher gives it nothing
+    assert math.isfinite(float(distill_loss(z.to(DEV), v.to(DEV), i.to(DEV))))
+
+
+def test_slices_and_leading_dimensions():
+    g = torch.Generator().manual_seed(7)
+    z = torch.randn(5, 3001, generator=g)
+    values, indices, tail = _teacher(z, 20, 1.0, True, g)
+
+    def odd(t):
+        wide = torch.zeros(t.shape[0], t.shape[1] + 3, dtype=t.dtype, device=t.device)
+        wide[:, 1:-2] = t
+        return wide[:, 1:-2]
+    for dtype in (F32, BF16):
+        _check_loss(z.to(dtype), values, indices, tail, 1.0, lay=odd)
+        _check_loss(z.to(dtype), values, indices, tail, 1.0, lay=lambda t: t.t().contiguous().t())
+    flat = distill_loss(z.to(DEV), values.to(DEV), indices.to(DEV), tail=tail.to(DEV), reduction='none')
+    deep = distill_loss(z.view(5, 1, 1, -1).to(DEV), values.view(5, 1, 1, -1).to(DEV), indices.view(5, 1, 1, -1).to(DEV), tail=tail.view(5, 1, 1).to(DEV), reduction='none')
+    assert deep.shape == (5, 1, 1) and torch.equal(deep.view(5), flat)
+    one = distill_loss(z[0].to(DEV), values[0].to(DEV), indices[0].to(DEV), tail=tail[0].to(DEV))
+    assert one.shape == () and float(one) == float(flat[0])
+    for shape in ((0, 700), (2, 0, 700)):
+        zd = torch.zeros(shape, device=DEV, requires_grad=True)
+        out = distill_loss(zd, torch.zeros(shape[:-1] + (4,), device=DEV), torch.zeros(shape[:-1] + (4,), dtype=torch.long, device=DEV))
+        assert float(out.detach()) == 0 and torch.autograd.grad(out, zd)[0].shape == torch.Size(shape)
+
+
+def test_formulas_are_the_derivatives():
+    """the reference's gradient against autograd through the definition and against differences, 64 bits, on the CPU"""
+    g = torch.Generator().manual_seed(11)
+    z = torch.randn(3, 12, generator=g)
+    values, indices, tail = _teacher(z, 4, 0.7, True, g)
+    indices[1, 2] = indices[1, 0]
+    for t in (None, tail):
+        for r in range(3):
+            def total(row):
+                u = row / 0.7
+                parts = values[r].double() / 0.7 if t is None else torch.cat([values[r].double() / 0.7, t[r:r + 1].double()])
+                lp = parts - torch.logsumexp(parts, 0)
+                lq = u - torch.logsumexp(u, 0)
+                res = (lp[:4].exp() * (lp[:4] - lq[indices[r]])).sum()
+                if t is not None:
+                    rest = [j for j in range(12) if j not in indices[r].tolist()]
+                    res = res + lp[4].exp() * (lp[4] - torch.logsumexp(lq[rest], 0))
+                return 0.49 * res
+            leaf = z[r].double().requires_grad_()
+            want, = torch.autograd.grad(total(leaf), leaf)
+            loss, grad, _, _, _ = _loss_reference(z, values, indices, t, 0.7, torch.ones(3).double(), torch.ones(3).double())
+            assert torch.allclose(grad[r], want, rtol=1e-9, atol=1e-12) and abs(float(loss[r] - total(z[r].double()))) < 1e-12
+            for j in range(12):
+                e = torch.zeros(12, dtype=torch.float64)
+                e[j] = 1e-6
+                assert abs(float(total(z[r].double() + e) - total(z[r].double() - e)) / 2e-6 - float(want[j])) < 1e-8
+
+
+# ---------------------------------------------------------------------------------------------------------------- how it is called
+def _pass(z, teacher, k, tau, weight=None):
+    values, indices, tail = top_logits(teacher, k, temperature=tau)
+    leaf = z.detach().requires_grad_()
+    loss = distill_loss(leaf, values, indices, tail=tail, temperature=tau, row_weight=weight)
+    return [values, indices, tail, loss.detach(), torch.autograd.grad(loss, leaf)[0]]
+
+
+@pytest.mark.parametrize('rows,cols', [(40, 9001), (2, 100000)])
+def test_same_bits_every_time_and_on_other_streams(rows, cols):
+    g = torch.Generator().manual_seed(12)
+    z, teacher = (torch.randn(rows, cols, generator=g).to(BF16).to(DEV) for _ in range(2))
+    first = _pass(z, teacher, 50, 2.0)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for _ in range(3):
+        res = []
+        for s in streams:
+            with torch.cuda.stream(s):
+                res.append(_pass(z, teacher, 50, 2.0))
+        torch.cuda.synchronize()
+        for r in res:
+            assert all(torch.equal(a, b) for a, b in zip(first, r))
+
+
+@pytest.mark.parametrize('rows,cols', [(20, 9001), (2, 100000)])
+def test_captured_and_replayed(rows, cols):
+    g = torch.Generator().manual_seed(13)
+    z, teacher = (torch.randn(rows, cols, generator=g).to(DEV) for _ in range(2))
+    weight = torch.ones(rows, device=DEV)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        _pass(z, teacher, 30, 0.5, weight)
+    torch.cuda.current_stream().wait_stream(s)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = _pass(z, teacher, 30, 0.5, weight)
+    for i in range(4):
+        z.copy_(torch.randn(rows, cols, generator=g))
+        teacher.copy_(torch.randn(rows, cols, generator=g))
+        weight[i % rows] = float(i)
+        graph.replay()
+        torch.cuda.synchronize()
+        want = _pass(z, teacher, 30, 0.5, weight)
+        assert all(torch.equal(a, b) for a, b in zip(out, want))
+
+
+def test_module_is_the_function():
+    g = torch.Generator().manual_seed(14)
+    z, teacher = (torch.randn(9, 500, generator=g).to(DEV) for _ in range(2))
+    values, indices, tail = top_logits(teacher, 10, temperature=3.0)
+    m = TopLogitsDistillLoss(temperature=3.0, reduction='sum')
+    assert torch.equal(m(z, values, indices, tail=tail), distill_loss(z, values, indices, tail=tail, temperature=3.0, reduction='sum'))
+
+
+def test_teacher_against_itself_costs_nothing():
+    """a student that is the teacher: the loss is 0 and so is the gradient, to the roundings of a row"""
+    g = torch.Generator().manual_seed(15)
+    z = torch.randn(8, 8192, generator=g).mul(4).to(DEV)
+    values, indices, tail = top_logits(z, 64, temperature=0.5)
+    leaf = z.clone().requires_grad_()
+    loss = distill_loss(leaf, values, indices, tail=tail, temperature=0.5)
+    grad, = torch.autograd.grad(loss, leaf)
+    err = U24 * (8 * 64 + 64 + 32)          # u spans less than 64 here
+    assert abs(float(loss.detach())) <= 0.25 * 3 * err and float(grad.abs().sum()) <= 2 * 0.5 * 3 * err
