@@ -714,7 +714,7 @@ int rumpy_moco_enqueue(float* queue, const float* keys, void* slots, void* queue
  * t NULL: h = N_pre(x) alone.  x / dx / y / dy in x_fmt, the others in t_fmt: both the same RUMPY_FMT_*, or x in fp32 beside a 16-bit t.
  * gate_mode 0: none, gate NULL; 1: fp32 [rows / group_rows, C], row r uses gate row r / group_rows; 2: [rows, C] in t_fmt.
  * Inputs have row strides (elements; channels are contiguous, any alignment of an element); outputs are contiguous.  1 <= C <= 8192.
- * `stats` [4][rows] (mean and factor of N_post, of N_pre) is written by the forward pass for the backward pass (NULL: not kept). */
+ * `stats` [rows][4] (mean and factor of N_post, of N_pre; 16-byte aligned) is written by the forward pass for the backward pass (NULL: not kept). */
 typedef struct {
   const void* x; const void* t; const void* gate;
   const float* post_w; const float* post_b; const float* pre_w; const float* pre_b;

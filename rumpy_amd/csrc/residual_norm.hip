@@ -14,9 +14,10 @@
 // Column sums (parameters, gates) run in a fixed order: registers over a workgroup's contiguous rows, one partial row per workgroup, then
 // residual_norm_reduce_kernel - bitwise reproducible, no atomics.
 #include "row_vec.hpp"
+#include <type_traits>
 
 constexpr int RN_GATE_NONE = 0, RN_GATE_GROUP = 1, RN_GATE_FULL = 2;
-constexpr int RN_NONE = 0, RN_LAYER = 1, RN_RMS = 2;
+constexpr int RN_NONE = 0, RN_LAYER = 1, RN_RMS = 2;   // (RUMPY_FMT_*, gate modes and kinds are the header's)
 constexpr int RN_MAXC = 8192;
 
 // sums over the TPR lanes of a row; rows of more than a wave meet in LDS.  `par` alternates between two buffers, so one barrier per call is enough:
@@ -43,70 +44,127 @@ template <int TPR> struct RowSum {
   __device__ __forceinline__ float one(float a) { float b = 0.f; two(a, b); return a; }
 };
 
-__device__ __forceinline__ void load_params(const float* p, int col, int n, float dflt, float (&o)[8]) {
+// Where a lane's 8 channels lie.  The last piece of a row is moved back to end with the row, and lanes behind it repeat it: every access is one
+// whole 16- or 32-byte access inside the row, with no branch around it.  What two lanes both hold they compute and store alike; in a row's sums
+// the repeated elements (the first `lo` of a lane) count zero times (`m`).  Rows of less than 8 channels have one lane (TPR 1) and partial accesses.
+template <int TPR> struct RnLane {
+  int at, n;             // first channel; channels of a partial access (TPR 1)
+  float m[8];
+  __device__ __forceinline__ explicit RnLane(int C) {
+    const int col = ((int)threadIdx.x % TPR) * 8;
+    at = TPR == 1 ? 0 : min(col, C - 8);
+    n = TPR == 1 ? C : 8;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) o[i] = (p && i < n) ? p[col + i] : dflt;
-}
+    for (int i = 0; i < 8; ++i) m[i] = (TPR == 1 ? i < C : i >= col - at) ? 1.f : 0.f;
+  }
+  template <int FMT> __device__ __forceinline__ RowRaw<FMT> load(const void* base, size_t row_off) const {
+    return load_piece<FMT>((const typename RowElem<FMT>::type*)base + row_off + at, TPR == 1 ? n : 8, 0.f);
+  }
+  template <int FMT> __device__ __forceinline__ void store(void* base, size_t row_off, const float (&v)[8]) const {
+    store8<FMT>(base, row_off + at, TPR == 1 ? n : 8, v);
+  }
+  // fp32 parameters; NULL: the default
+  __device__ __forceinline__ void params(const float* p, float dflt, float (&o)[8]) const {
+    if (p) unpack_piece<RUMPY_FMT_F32>(load<RUMPY_FMT_F32>(p, 0), o);
+    else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) o[i] = dflt;
+    }
+  }
+};
 
-// mean and 1 / sqrt(var + eps) of a row whose elements lie n per lane (zero beyond n)
-template <int TPR> __device__ __forceinline__ void row_stats(RowSum<TPR>& sum, const float (&v)[8], int n, int kind, float inv_c, float eps, float& mu, float& rs) {
+// mean and 1 / sqrt(var + eps) of a row.  The variance is taken around the mean in a second sum (the row is in registers): no cancellation
+// where the mean is large.  v_rsq_f32 is right to one unit in the last place for normal arguments (eps is one).
+template <int TPR> __device__ __forceinline__ void row_stats(RowSum<TPR>& sum, const float (&v)[8], const float (&m)[8], int kind, float inv_c, float eps,
+                                                             float& mu, float& rs) {
   mu = 0.f;
   if (kind == RN_LAYER) {
     float s = 0.f;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) s += v[i];
+    for (int i = 0; i < 8; ++i) s = fmaf(v[i], m[i], s);
     mu = sum.one(s) * inv_c;
   }
   float q = 0.f;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) { const float d = i < n ? v[i] - mu : 0.f; q = fmaf(d, d, q); }
-  rs = 1.f / sqrtf(sum.one(q) * inv_c + eps);
+  for (int i = 0; i < 8; ++i) { const float d = (v[i] - mu) * m[i]; q = fmaf(d, d, q); }
+  rs = __builtin_amdgcn_rsqf(sum.one(q) * inv_c + eps);
 }
 
-template <int XF, int TF, int TPR> __global__ void __launch_bounds__(TPR <= 64 ? 256 : TPR) residual_norm_fwd_kernel(rumpy_residual_norm_args a) {
+// The grid holds what the chip runs at once and every workgroup walks over rows; a row's tensors are asked for before the row in front of it
+// is computed, and unpacked behind that row's stores.  The counter that loads and stores share counts in order: where the number of stores in
+// between is known, the wait for the loads leaves the stores in flight, so the usual calls (t, y and h; with or without statistics) are kernels of
+// their own (MODE) and everything else is RN_ANY.  Rows behind the last one repeat it: they store the same values once more.
+constexpr int RN_ANY = 0, RN_EVAL = 1, RN_TRAIN = 2;
+template <int XF, int TF, int TPR, int MODE> __global__ void __launch_bounds__(TPR <= 64 ? 256 : TPR) residual_norm_fwd_kernel(rumpy_residual_norm_args a) {
   constexpr int WG = TPR <= 64 ? 256 : TPR, SUB = WG / TPR;
   __shared__ float red[2][2 * RowSum<TPR>::WAVES];
   RowSum<TPR> sum{red, 0};
-  const int tid = threadIdx.x, col = (tid % TPR) * 8, sub = tid / TPR;
-  const int nc = min(8, max(0, a.C - col));
+  const RnLane<TPR> lane(a.C);
+  const int sub = (int)threadIdx.x / TPR;
   const float inv_c = 1.f / (float)a.C;
+  const uint32_t rows = (uint32_t)a.rows, step = gridDim.x * SUB;
+  const bool has_t = MODE != RN_ANY || a.t, has_pre = MODE != RN_ANY || a.pre != RN_NONE, keep = MODE == RN_TRAIN || (MODE == RN_ANY && a.stats);
+  uint32_t rb = blockIdx.x * SUB;
+  // the gate row of the row that is asked for next, advanced without a division per row
+  uint32_t grp = 0, rem = 0, grp_step = 0, rem_step = 0;
+  const bool grouped = a.gate_mode == RN_GATE_GROUP, full = a.gate_mode == RN_GATE_FULL;
+  if (grouped) {
+    const uint32_t gr = (uint32_t)a.group_rows;
+    grp = (rb + sub) / gr; rem = (rb + sub) % gr;
+    grp_step = step / gr; rem_step = step % gr;
+  }
+  const uint32_t last_grp = grouped ? (rows - 1) / (uint32_t)a.group_rows : 0;
+  RowRaw<XF> rx;
+  RowRaw<TF> rt, rg;
+  RowRaw<RUMPY_FMT_F32> rgate;
+  auto ask = [&](uint32_t base) {
+    const size_t r = min(base + sub, rows - 1);
+    rx = lane.template load<XF>(a.x, r * a.ldx);
+    if (has_t) rt = lane.template load<TF>(a.t, r * a.ldt);
+    if (full) rg = lane.template load<TF>(a.gate, r * a.ldg);
+    if (grouped) {
+      rgate = lane.template load<RUMPY_FMT_F32>(a.gate, (size_t)min(grp, last_grp) * a.C);
+      grp += grp_step; rem += rem_step;
+      if (rem >= (uint32_t)a.group_rows) { rem -= (uint32_t)a.group_rows; ++grp; }
+    }
+  };
+  float x[8], t[8], g[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) { t[i] = 0.f; g[i] = 1.f; }
+  auto take = [&]() {
+    unpack_piece<XF>(rx, x);
+    if (has_t) unpack_piece<TF>(rt, t);
+    if (full) unpack_piece<TF>(rg, g);
+    if (grouped) unpack_piece<RUMPY_FMT_F32>(rgate, g);
+  };
+  ask(rb);
   float wp[8], bp[8], w[8], b[8];
-  load_params(a.post_w, col, nc, 1.f, wp);
-  load_params(a.post_b, col, nc, 0.f, bp);
-  load_params(a.pre_w, col, nc, 1.f, w);
-  load_params(a.pre_b, col, nc, 0.f, b);
-  for (int64_t rb = (int64_t)blockIdx.x * SUB; rb < a.rows; rb += (int64_t)gridDim.x * SUB) {
-    const int64_t r = rb + sub;
-    const bool live = r < a.rows;                   // (a row of more than a wave: always)
-    const int n = live ? nc : 0;
-    const size_t rr = live ? (size_t)r : 0;
-    float y[8];
-    load8<XF>(a.x, rr * a.ldx + col, n, y);
-    float mu = 0.f, rs = 1.f;
-    if (a.t) {
-      float t[8], g[8];
-      load8<TF>(a.t, rr * a.ldt + col, n, t);
+  lane.params(a.post_w, 1.f, wp);
+  lane.params(a.post_b, 0.f, bp);
+  lane.params(a.pre_w, 1.f, w);
+  lane.params(a.pre_b, 0.f, b);
+  take();
+  while (true) {
+    const size_t r = min(rb + sub, rows - 1);
+    const bool more = rows - rb > step;
+    ask(more ? rb + step : rb);
+    float4 st = make_float4(0.f, 1.f, 0.f, 1.f);
+    if (has_t) {
+      if (a.post != RN_NONE) row_stats<TPR>(sum, t, lane.m, a.post, inv_c, a.eps, st.x, st.y);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) g[i] = 1.f;
-      if (a.gate_mode == RN_GATE_GROUP) load_params((const float*)a.gate + (size_t)((uint32_t)rr / (uint32_t)a.group_rows) * a.C, col, n, 0.f, g);
-      else if (a.gate_mode == RN_GATE_FULL) load8<TF>(a.gate, rr * a.ldg + col, n, g);
-      if (a.post != RN_NONE) row_stats<TPR>(sum, t, n, a.post, inv_c, a.eps, mu, rs);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float z = fmaf((t[i] - mu) * rs, wp[i], bp[i]);
-        y[i] = i < n ? fmaf(a.scale * g[i], z, y[i]) : 0.f;
-      }
-      store8<XF>(a.y, rr * a.C + col, n, y);
-      if (a.stats && a.post != RN_NONE && live && col == 0) { a.stats[rr] = mu; a.stats[a.rows + rr] = rs; }
+      for (int i = 0; i < 8; ++i) x[i] = fmaf(a.scale * g[i], fmaf((t[i] - st.x) * st.y, wp[i], bp[i]), x[i]);
+      lane.template store<XF>(a.y, r * a.C, x);
     }
-    if (a.pre != RN_NONE) {
-      row_stats<TPR>(sum, y, n, a.pre, inv_c, a.eps, mu, rs);
-      float h[8];
+    if (has_pre) {
+      row_stats<TPR>(sum, x, lane.m, a.pre, inv_c, a.eps, st.z, st.w);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) h[i] = fmaf((y[i] - mu) * rs, w[i], b[i]);
-      store8<TF>(a.h, rr * a.C + col, n, h);
-      if (a.stats && live && col == 0) { a.stats[2 * a.rows + rr] = mu; a.stats[3 * a.rows + rr] = rs; }
+      for (int i = 0; i < 8; ++i) x[i] = fmaf((x[i] - st.z) * st.w, w[i], b[i]);
+      lane.template store<TF>(a.h, r * a.C, x);
     }
+    if (keep) reinterpret_cast<float4*>(a.stats)[r] = st;
+    if (!more) break;
+    take();
+    rb += step;
   }
 }
 
@@ -117,161 +175,199 @@ template <int XF, int TF, int TPR> __global__ void __launch_bounds__(TPR <= 64 ?
 struct RnPlan { int tpr, sub, wgs, rpw; bool direct; };
 static RnPlan rn_plan(int64_t rows, int64_t group_rows, int32_t C, int gate_mode) {
   RnPlan p;
-  p.tpr = 8;
+  p.tpr = C < 8 ? 1 : 8;
   while (p.tpr * 8 < C) p.tpr *= 2;
   p.sub = p.tpr <= 64 ? 256 / p.tpr : 1;
   const int64_t steps = (rows + p.sub - 1) / p.sub;
-  int64_t wgs = (steps + 3) / 4;
-  if (wgs > 512) wgs = 512;
-  if (wgs < 1) wgs = 1;
+  // two waves of these registers fit a SIMD: 512 threads a CU.  At least two steps each, so that the partial rows stay fewer than the rows
+  const int64_t most = p.tpr <= 64 ? 512 : p.tpr <= 512 ? 256 * (512 / p.tpr) : 256;
+  int64_t wgs = (steps + 1) / 2;
+  if (wgs > most) wgs = most;
   p.rpw = (int)((steps + wgs - 1) / wgs * p.sub);
   p.wgs = (int)((rows + p.rpw - 1) / p.rpw);
   p.direct = gate_mode == RN_GATE_GROUP && group_rows < p.sub;
   return p;
 }
 
+// sum over the lanes of a wave that hold the same channels of different rows (every TPR-th lane), in each of them, without the LDS crossbar
+template <int TPR> __device__ __forceinline__ float steps_sum(float v, int lane) {
+  if constexpr (TPR == 1) return wave64_sum(v, lane);
+  if constexpr (TPR <= 8) {
+    const int i = __float_as_int(v);
+    v += __int_as_float(__builtin_amdgcn_update_dpp(i, i, 0x128, 0xF, 0xF, false));      // row_ror 8: lane ^ 8
+  }
+  if constexpr (TPR <= 16) v += lane_xor16(v, lane >> 4);
+  if constexpr (TPR <= 32) v += lane_xor32(v, lane);
+  return v;
+}
 // column sums of a workgroup: the rows of a step lie side by side in its waves
-template <int TPR> __device__ __forceinline__ void flush_columns(float (&acc)[8], float* dst, int col, int nc, float* lds) {
-  if constexpr (TPR > 64) {
+template <int TPR> __device__ __forceinline__ void flush_columns(const RnLane<TPR>& lane, float (&acc)[8], float* dst, float* lds) {
+  if constexpr (TPR <= 64) {
+    const int tid = threadIdx.x, l = tid & 63, wave = tid >> 6;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) if (i < nc) dst[col + i] = acc[i];
-  } else {
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      float v = acc[i];
-#pragma unroll
-      for (int o = TPR; o < 64; o *= 2) v += __shfl_xor(v, o);
-      acc[i] = v;
-    }
+    for (int i = 0; i < 8; ++i) acc[i] = steps_sum<TPR>(acc[i], l);
     __syncthreads();
-    if (lane < TPR) {
+    if (l < TPR) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) lds[wave * TPR * 8 + lane * 8 + i] = acc[i];
+      for (int i = 0; i < 8; ++i) lds[(wave * 8 + i) * TPR + l] = acc[i];
     }
     __syncthreads();
     if (tid < TPR) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (i < nc) dst[col + i] = (lds[tid * 8 + i] + lds[TPR * 8 + tid * 8 + i]) + (lds[2 * TPR * 8 + tid * 8 + i] + lds[3 * TPR * 8 + tid * 8 + i]);
+      for (int i = 0; i < 8; ++i) acc[i] = (lds[i * TPR + l] + lds[(8 + i) * TPR + l]) + (lds[(16 + i) * TPR + l] + lds[(24 + i) * TPR + l]);
+      lane.template store<RUMPY_FMT_F32>(dst, 0, acc);
     }
+  } else {
+    lane.template store<RUMPY_FMT_F32>(dst, 0, acc);
   }
 #pragma unroll
   for (int i = 0; i < 8; ++i) acc[i] = 0.f;
 }
 
-template <int XF, int TF, int TPR> __global__ void __launch_bounds__(TPR <= 64 ? 256 : TPR) residual_norm_bwd_kernel(rumpy_residual_norm_bwd_args a, RnPlan plan) {
+// MODE as in the forward kernel: RN_ALL = dy, dh, t, dx, dt (and no gate of t's shape), RN_ALL_FULL = those and a gate of t's shape with its gradient.
+constexpr int RN_ALL = 1, RN_ALL_FULL = 2;
+template <int XF, int TF, int TPR, int MODE> __global__ void __launch_bounds__(TPR <= 64 ? 256 : TPR) residual_norm_bwd_kernel(rumpy_residual_norm_bwd_args a, RnPlan plan) {
   constexpr int WG = TPR <= 64 ? 256 : TPR, SUB = WG / TPR;
+  // 1024 threads leave 128 registers each: the sums alone stay there, parameters come from the caches per row and nothing is asked for ahead
+  constexpr bool HOLD = TPR <= 512;
   __shared__ float red[2][2 * RowSum<TPR>::WAVES];
   __shared__ float cols[TPR <= 64 ? 4 * TPR * 8 : 1];
   RowSum<TPR> sum{red, 0};
-  const int tid = threadIdx.x, col = (tid % TPR) * 8, sub = tid / TPR;
-  const int nc = min(8, max(0, a.C - col));
+  const RnLane<TPR> lane(a.C);
+  const int sub = (int)threadIdx.x / TPR;
   const float inv_c = 1.f / (float)a.C;
-  float wp[8], bp[8], w[8], g[8];
-  load_params(a.post_w, col, nc, 1.f, wp);
-  load_params(a.post_b, col, nc, 0.f, bp);
-  load_params(a.pre_w, col, nc, 1.f, w);
+  const uint32_t rows = (uint32_t)a.rows, r0 = min(rows, blockIdx.x * (uint32_t)plan.rpw), r1 = min(rows, r0 + (uint32_t)plan.rpw);
+  float* gpart = a.partial + (size_t)4 * plan.wgs * a.C;               // partial: [4][wgs][C], then the gate's partial rows
+  const bool has_t = MODE != RN_ANY || a.t, has_dy = MODE != RN_ANY || a.dy, has_dh = MODE != RN_ANY || a.dh;
+  const bool full = MODE == RN_ALL_FULL || (MODE == RN_ANY && a.gate_mode == RN_GATE_FULL);
+  const bool direct = MODE != RN_ALL_FULL && plan.direct, group_sums = MODE != RN_ALL_FULL && a.gate_mode == RN_GATE_GROUP && !plan.direct;
+
+  RowRaw<XF> rx, rdy;
+  RowRaw<TF> rt, rdh, rg;
+  float4 rst = make_float4(0.f, 1.f, 0.f, 1.f), st;
+  float x[8], t[8], d[8], e[8], g[8];
+  auto ask = [&](size_t r) {
+    rx = lane.template load<XF>(a.x, r * a.ldx);
+    if (has_t) rt = lane.template load<TF>(a.t, r * a.ldt);
+    if (has_dy) rdy = lane.template load<XF>(a.dy, r * a.lddy);
+    if (has_dh) rdh = lane.template load<TF>(a.dh, r * a.lddh);
+    if (full) rg = lane.template load<TF>(a.gate, r * a.ldg);
+    if (MODE != RN_ANY || a.stats) rst = reinterpret_cast<const float4*>(a.stats)[r];
+  };
+  auto take = [&]() {
+    unpack_piece<XF>(rx, x);
+    if (has_t) unpack_piece<TF>(rt, t);
+    if (has_dy) unpack_piece<XF>(rdy, d);
+    if (has_dh) unpack_piece<TF>(rdh, e);
+    if (full) unpack_piece<TF>(rg, g);
+    st = rst;
+  };
+  float wp[8], bp[8], w[8];
   float aw[8], ab[8], awp[8], abp[8], ag[8];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) { aw[i] = ab[i] = awp[i] = abp[i] = ag[i] = 0.f; g[i] = 1.f; }
-  const int64_t r0 = (int64_t)blockIdx.x * plan.rpw, r1 = min(a.rows, r0 + plan.rpw);
-  float* part = a.partial;                                            // [4][wgs][C], then the gate's partial rows
-  float* gpart = a.partial + (size_t)4 * plan.wgs * a.C;
-  const bool group_sums = a.gate_mode == RN_GATE_GROUP && !plan.direct;
-  for (int64_t seg = r0; seg < r1;) {
-    int64_t seg_end = r1;
-    size_t group = 0;
-    if (group_sums) {
-      group = (uint32_t)seg / (uint32_t)a.group_rows;
-      seg_end = min(r1, (int64_t)(group + 1) * a.group_rows);
-      load_params((const float*)a.gate + group * a.C, col, nc, 0.f, g);
+  for (int i = 0; i < 8; ++i) { aw[i] = ab[i] = awp[i] = abp[i] = ag[i] = t[i] = d[i] = e[i] = 0.f; g[i] = 1.f; }
+  if (HOLD) { lane.params(a.post_w, 1.f, wp); lane.params(a.post_b, 0.f, bp); lane.params(a.pre_w, 1.f, w); }
+  // one step: SUB rows; those behind the segment repeat its last row, `live` takes them out of the column sums (TAIL steps alone have any)
+  auto step = [&](size_t r, bool live, auto tail) {
+    constexpr bool TAIL = decltype(tail)::value;
+    if (!HOLD) { lane.params(a.post_w, 1.f, wp); lane.params(a.post_b, 0.f, bp); }
+    if (direct) unpack_piece<RUMPY_FMT_F32>(lane.template load<RUMPY_FMT_F32>(a.gate, (size_t)((uint32_t)r / (uint32_t)a.group_rows) * a.C), g);
+    if (has_t) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        t[i] = (t[i] - st.x) * st.y;                                              // that
+        x[i] = fmaf(a.scale * g[i], fmaf(t[i], wp[i], bp[i]), x[i]);               // y, unrounded
+      }
     }
-    for (int64_t rb = seg; rb < seg_end; rb += SUB) {
-      const int64_t r = rb + sub;
-      const bool live = r < seg_end;
-      const int n = live ? nc : 0;
-      const size_t rr = live ? (size_t)r : (size_t)seg;
-      float x[8], t[8], d[8], e[8];
-      load8<XF>(a.x, rr * a.ldx + col, n, x);
-      if (a.t) load8<TF>(a.t, rr * a.ldt + col, n, t);
-      if (a.dy) load8<XF>(a.dy, rr * a.lddy + col, n, d);
-      else {
+    if (!has_dy) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) d[i] = 0.f;
+      for (int i = 0; i < 8; ++i) d[i] = 0.f;
+    }
+    if (has_dh) {
+      if (!HOLD) lane.params(a.pre_w, 1.f, w);
+      float s1 = 0.f, s2 = 0.f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        x[i] = (x[i] - st.z) * st.w;                                              // yhat
+        const float ea = TAIL && !live ? 0.f : e[i];
+        ab[i] += ea;
+        aw[i] = fmaf(ea, x[i], aw[i]);
+        e[i] *= w[i];
+        const float em = e[i] * lane.m[i];
+        s1 += em;
+        s2 = fmaf(em, x[i], s2);
       }
-      if (a.dh) load8<TF>(a.dh, rr * a.lddh + col, n, e);
-      if (a.gate_mode == RN_GATE_FULL) load8<TF>(a.gate, rr * a.ldg + col, n, g);
-      else if (plan.direct) load_params((const float*)a.gate + (size_t)((uint32_t)rr / (uint32_t)a.group_rows) * a.C, col, n, 0.f, g);
-      float mu_t = 0.f, rs_t = 1.f;
-      if (a.t) {
-        if (a.post != RN_NONE) { mu_t = a.stats[rr]; rs_t = a.stats[a.rows + rr]; }
+      sum.two(s1, s2);
+      s1 = a.pre == RN_LAYER ? s1 * inv_c : 0.f;
+      s2 *= inv_c;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          t[i] = i < n ? (t[i] - mu_t) * rs_t : 0.f;                                // that
-          x[i] = i < n ? fmaf(a.scale * g[i], fmaf(t[i], wp[i], bp[i]), x[i]) : 0.f;     // y, unrounded
-        }
-      }
-      if (a.dh) {
-        const float mu = a.stats[2 * a.rows + rr], rs = a.stats[3 * a.rows + rr];
-        float s1 = 0.f, s2 = 0.f;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const float yh = i < n ? (x[i] - mu) * rs : 0.f;
-          x[i] = yh;
-          ab[i] += e[i];
-          aw[i] = fmaf(e[i], yh, aw[i]);
-          e[i] *= w[i];
-          s1 += e[i];
-          s2 = fmaf(e[i], yh, s2);
-        }
-        sum.two(s1, s2);
-        s1 = a.pre == RN_LAYER ? s1 * inv_c : 0.f;
-        s2 *= inv_c;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) d[i] = fmaf(rs, (e[i] - s1) - x[i] * s2, d[i]);
-      }
-      if (a.dx) store8<XF>(a.dx, rr * a.C + col, n, d);
-      if (!a.t) continue;
+      for (int i = 0; i < 8; ++i) d[i] = fmaf(st.w, (e[i] - s1) - x[i] * s2, d[i]);
+    }
+    if (MODE != RN_ANY || a.dx) lane.template store<XF>(a.dx, r * a.C, d);
+    if (has_t) {
+      if (!HOLD) { lane.params(a.post_w, 1.f, wp); lane.params(a.post_b, 0.f, bp); }
       float s1 = 0.f, s2 = 0.f;
       float gr[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const float dd = i < n ? a.scale * d[i] : 0.f;
+        const float dd = a.scale * d[i];
         gr[i] = dd * fmaf(t[i], wp[i], bp[i]);
-        ag[i] += gr[i];
         const float dz = g[i] * dd;
-        abp[i] += dz;
-        awp[i] = fmaf(dz, t[i], awp[i]);
+        if (!TAIL || live) { ag[i] += gr[i]; abp[i] += dz; awp[i] = fmaf(dz, t[i], awp[i]); }
         d[i] = dz * wp[i];
-        s1 += d[i];
-        s2 = fmaf(d[i], t[i], s2);
+        const float dm = d[i] * lane.m[i];
+        s1 += dm;
+        s2 = fmaf(dm, t[i], s2);
       }
-      if (a.gate_mode == RN_GATE_FULL) { if (a.dgate) store8<TF>(a.dgate, rr * a.C + col, n, gr); }
-      else if (plan.direct && a.dgate) store8<RUMPY_FMT_F32>(gpart, rr * a.C + col, n, gr);
+      if (MODE == RN_ALL_FULL || (full && a.dgate)) lane.template store<TF>(a.dgate, r * a.C, gr);
+      else if (direct && a.dgate) lane.template store<RUMPY_FMT_F32>(gpart, r * a.C, gr);
       if (a.post != RN_NONE) {
         sum.two(s1, s2);
         s1 = a.post == RN_LAYER ? s1 * inv_c : 0.f;
         s2 *= inv_c;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) d[i] = rs_t * ((d[i] - s1) - t[i] * s2);
+        for (int i = 0; i < 8; ++i) d[i] = st.y * ((d[i] - s1) - t[i] * s2);
       }
-      if (a.dt) store8<TF>(a.dt, rr * a.C + col, n, d);
+      if (MODE != RN_ANY || a.dt) lane.template store<TF>(a.dt, r * a.C, d);
     }
-    if (group_sums && a.dgate) flush_columns<TPR>(ag, gpart + (blockIdx.x + group) * a.C, col, nc, cols);
-    seg = seg_end;
+  };
+  for (uint32_t seg = r0; seg < r1;) {
+    uint32_t end = r1;
+    size_t group = 0;
+    if (group_sums) {
+      group = seg / (uint32_t)a.group_rows;
+      end = (uint32_t)min((int64_t)r1, (int64_t)(group + 1) * a.group_rows);
+      unpack_piece<RUMPY_FMT_F32>(lane.template load<RUMPY_FMT_F32>(a.gate, group * a.C), g);
+    }
+    const uint32_t last = end - 1;
+    uint32_t rb = seg;
+    if (HOLD) { ask(min(rb + sub, last)); take(); }
+    for (; end - rb >= SUB && rb < end; rb += SUB) {
+      if (HOLD) ask(min(rb + SUB + sub, last));
+      else { ask(rb + sub); take(); }
+      step(rb + sub, true, std::false_type());
+      if (HOLD) take();
+    }
+    if (SUB > 1 && rb < end) {
+      if (!HOLD) { ask(min(rb + sub, last)); take(); }
+      step(min(rb + sub, last), rb + sub < end, std::true_type());
+    }
+    if (group_sums && a.dgate) flush_columns<TPR>(lane, ag, gpart + (blockIdx.x + group) * a.C, cols);
+    seg = end;
   }
   const size_t wc = (size_t)plan.wgs * a.C;
-  float* mine = part + (size_t)blockIdx.x * a.C;
-  if (a.d_post_w) flush_columns<TPR>(awp, mine, col, nc, cols);
-  if (a.d_post_b) flush_columns<TPR>(abp, mine + wc, col, nc, cols);
-  if (a.d_pre_w) flush_columns<TPR>(aw, mine + 2 * wc, col, nc, cols);
-  if (a.d_pre_b) flush_columns<TPR>(ab, mine + 3 * wc, col, nc, cols);
+  float* mine = a.partial + (size_t)blockIdx.x * a.C;
+  if (a.d_post_w) flush_columns<TPR>(lane, awp, mine, cols);
+  if (a.d_post_b) flush_columns<TPR>(lane, abp, mine + wc, cols);
+  if (a.d_pre_w) flush_columns<TPR>(lane, aw, mine + 2 * wc, cols);
+  if (a.d_pre_b) flush_columns<TPR>(lane, ab, mine + 3 * wc, cols);
 }
 
-// out[c] = sum over consecutive partial rows: items 0..3 = the parameters (all workgroups), 4.. = the gate rows
-__global__ void __launch_bounds__(256) residual_norm_reduce_kernel(rumpy_residual_norm_bwd_args a, RnPlan plan, int tiles) {
-  __shared__ float red[4][64];
+// out[c] = sum over consecutive partial rows: items 0..3 = the parameters (all workgroups), 4.. = the gate rows.  16 waves share a column's rows:
+// with four a sum of 461 rows took 7 us of dependent loads.
+constexpr int RN_SLICES = 16;
+__global__ void __launch_bounds__(64 * RN_SLICES) residual_norm_reduce_kernel(rumpy_residual_norm_bwd_args a, RnPlan plan, int tiles) {
+  __shared__ float red[RN_SLICES][64];
   const size_t item = blockIdx.x / tiles;
   const int lane = threadIdx.x & 63, slice = threadIdx.x >> 6, c = (blockIdx.x % tiles) * 64 + lane;
   const size_t wc = (size_t)plan.wgs * a.C;
@@ -279,8 +375,7 @@ __global__ void __launch_bounds__(256) residual_norm_reduce_kernel(rumpy_residua
   float* dst;
   int64_t count;
   if (item < 4) {
-    float* const outs[4] = {a.d_post_w, a.d_post_b, a.d_pre_w, a.d_pre_b};
-    dst = outs[item];
+    dst = item == 0 ? a.d_post_w : item == 1 ? a.d_post_b : item == 2 ? a.d_pre_w : a.d_pre_b;
     src = a.partial + item * wc;
     count = plan.wgs;
   } else {
@@ -294,11 +389,15 @@ __global__ void __launch_bounds__(256) residual_norm_reduce_kernel(rumpy_residua
   float s = 0.f;
   if (c < a.C) {
 #pragma unroll 8
-    for (int64_t i = slice; i < count; i += 4) s += src[(size_t)i * a.C + c];
+    for (int64_t i = slice; i < count; i += RN_SLICES) s += src[(size_t)i * a.C + c];
   }
   red[slice][lane] = s;
   __syncthreads();
-  if (slice == 0 && c < a.C) dst[c] = (red[0][lane] + red[1][lane]) + (red[2][lane] + red[3][lane]);
+  if (slice == 0 && c < a.C) {
+#pragma unroll
+    for (int i = 1; i < RN_SLICES; ++i) s += red[i][lane];
+    dst[c] = s;
+  }
 }
 
 // ---- entry points ----
@@ -318,31 +417,51 @@ static const char* rn_check(int64_t rows, int64_t group_rows, int32_t C, int x_f
   return nullptr;
 }
 
+// the usual calls have kernels of their own, from 8 channels on
+template <int XF, int TF, int TPR> static void rn_launch_fwd_tpr(const rumpy_residual_norm_args& a, const dim3& grid, hipStream_t s) {
+  const dim3 wg(TPR <= 64 ? 256 : TPR);
+  if (TPR > 1 && a.t && a.pre != RN_NONE) {
+    if (a.stats) hipLaunchKernelGGL((residual_norm_fwd_kernel<XF, TF, TPR, TPR == 1 ? RN_ANY : RN_TRAIN>), grid, wg, 0, s, a);
+    else hipLaunchKernelGGL((residual_norm_fwd_kernel<XF, TF, TPR, TPR == 1 ? RN_ANY : RN_EVAL>), grid, wg, 0, s, a);
+  } else {
+    hipLaunchKernelGGL((residual_norm_fwd_kernel<XF, TF, TPR, RN_ANY>), grid, wg, 0, s, a);
+  }
+}
+template <int XF, int TF, int TPR> static void rn_launch_bwd_tpr(const rumpy_residual_norm_bwd_args& a, const RnPlan& p, hipStream_t s) {
+  const dim3 grid((unsigned)p.wgs), wg(TPR <= 64 ? 256 : TPR);
+  const bool all = TPR > 1 && a.dy && a.dh && a.t && a.dx && a.dt && a.stats;
+  if (all && a.gate_mode != RN_GATE_FULL) hipLaunchKernelGGL((residual_norm_bwd_kernel<XF, TF, TPR, TPR == 1 ? RN_ANY : RN_ALL>), grid, wg, 0, s, a, p);
+  else if (all && a.dgate) hipLaunchKernelGGL((residual_norm_bwd_kernel<XF, TF, TPR, TPR == 1 ? RN_ANY : RN_ALL_FULL>), grid, wg, 0, s, a, p);
+  else hipLaunchKernelGGL((residual_norm_bwd_kernel<XF, TF, TPR, RN_ANY>), grid, wg, 0, s, a, p);
+}
 template <int XF, int TF> static void rn_launch_fwd(const rumpy_residual_norm_args& a, const RnPlan& p, hipStream_t s) {
   const int64_t steps = (a.rows + p.sub - 1) / p.sub;
-  const dim3 grid((unsigned)(steps < 4096 ? steps : 4096));
+  // four waves of these registers fit a SIMD: 1024 threads a CU
+  const int64_t most = p.tpr <= 64 ? 1024 : 256 * 1024 / p.tpr;
+  const dim3 grid((unsigned)(steps < most ? steps : most));
   switch (p.tpr) {
-    case 8: hipLaunchKernelGGL((residual_norm_fwd_kernel<XF, TF, 8>), grid, dim3(256), 0, s, a); break;
-    case 16: hipLaunchKernelGGL((residual_norm_fwd_kernel<XF, TF, 16>), grid, dim3(256), 0, s, a); break;
-    case 32: hipLaunchKernelGGL((residual_norm_fwd_kernel<XF, TF, 32>), grid, dim3(256), 0, s, a); break;
-    case 64: hipLaunchKernelGGL((residual_norm_fwd_kernel<XF, TF, 64>), grid, dim3(256), 0, s, a); break;
-    case 128: hipLaunchKernelGGL((residual_norm_fwd_kernel<XF, TF, 128>), grid, dim3(128), 0, s, a); break;
-    case 256: hipLaunchKernelGGL((residual_norm_fwd_kernel<XF, TF, 256>), grid, dim3(256), 0, s, a); break;
-    case 512: hipLaunchKernelGGL((residual_norm_fwd_kernel<XF, TF, 512>), grid, dim3(512), 0, s, a); break;
-    default: hipLaunchKernelGGL((residual_norm_fwd_kernel<XF, TF, 1024>), grid, dim3(1024), 0, s, a); break;
+    case 1: return rn_launch_fwd_tpr<XF, TF, 1>(a, grid, s);
+    case 8: return rn_launch_fwd_tpr<XF, TF, 8>(a, grid, s);
+    case 16: return rn_launch_fwd_tpr<XF, TF, 16>(a, grid, s);
+    case 32: return rn_launch_fwd_tpr<XF, TF, 32>(a, grid, s);
+    case 64: return rn_launch_fwd_tpr<XF, TF, 64>(a, grid, s);
+    case 128: return rn_launch_fwd_tpr<XF, TF, 128>(a, grid, s);
+    case 256: return rn_launch_fwd_tpr<XF, TF, 256>(a, grid, s);
+    case 512: return rn_launch_fwd_tpr<XF, TF, 512>(a, grid, s);
+    default: return rn_launch_fwd_tpr<XF, TF, 1024>(a, grid, s);
   }
 }
 template <int XF, int TF> static void rn_launch_bwd(const rumpy_residual_norm_bwd_args& a, const RnPlan& p, hipStream_t s) {
-  const dim3 grid((unsigned)p.wgs);
   switch (p.tpr) {
-    case 8: hipLaunchKernelGGL((residual_norm_bwd_kernel<XF, TF, 8>), grid, dim3(256), 0, s, a, p); break;
-    case 16: hipLaunchKernelGGL((residual_norm_bwd_kernel<XF, TF, 16>), grid, dim3(256), 0, s, a, p); break;
-    case 32: hipLaunchKernelGGL((residual_norm_bwd_kernel<XF, TF, 32>), grid, dim3(256), 0, s, a, p); break;
-    case 64: hipLaunchKernelGGL((residual_norm_bwd_kernel<XF, TF, 64>), grid, dim3(256), 0, s, a, p); break;
-    case 128: hipLaunchKernelGGL((residual_norm_bwd_kernel<XF, TF, 128>), grid, dim3(128), 0, s, a, p); break;
-    case 256: hipLaunchKernelGGL((residual_norm_bwd_kernel<XF, TF, 256>), grid, dim3(256), 0, s, a, p); break;
-    case 512: hipLaunchKernelGGL((residual_norm_bwd_kernel<XF, TF, 512>), grid, dim3(512), 0, s, a, p); break;
-    default: hipLaunchKernelGGL((residual_norm_bwd_kernel<XF, TF, 1024>), grid, dim3(1024), 0, s, a, p); break;
+    case 1: return rn_launch_bwd_tpr<XF, TF, 1>(a, p, s);
+    case 8: return rn_launch_bwd_tpr<XF, TF, 8>(a, p, s);
+    case 16: return rn_launch_bwd_tpr<XF, TF, 16>(a, p, s);
+    case 32: return rn_launch_bwd_tpr<XF, TF, 32>(a, p, s);
+    case 64: return rn_launch_bwd_tpr<XF, TF, 64>(a, p, s);
+    case 128: return rn_launch_bwd_tpr<XF, TF, 128>(a, p, s);
+    case 256: return rn_launch_bwd_tpr<XF, TF, 256>(a, p, s);
+    case 512: return rn_launch_bwd_tpr<XF, TF, 512>(a, p, s);
+    default: return rn_launch_bwd_tpr<XF, TF, 1024>(a, p, s);
   }
 }
 #define RN_BY_FORMAT(fn, ...)                                                                                          \
@@ -357,6 +476,7 @@ template <int XF, int TF> static void rn_launch_bwd(const rumpy_residual_norm_bw
 extern "C" int rumpy_residual_norm_fwd(const rumpy_residual_norm_args* p, void* stream) {
   const char* bad = !p ? "no arguments" : rn_check(p->rows, p->group_rows, p->C, p->x_fmt, p->t_fmt, p->t, p->gate, p->gate_mode, p->post, p->pre);
   if (!bad && p->rows && (!p->x || (p->t && !p->y) || (p->pre != RN_NONE && !p->h))) bad = "a tensor is missing";
+  if (!bad && ((uintptr_t)p->stats & 15)) bad = "stats lies at a multiple of 16 bytes";
   if (!bad && (p->ldx < 0 || p->ldt < 0 || p->ldg < 0)) bad = "row strides are not negative";
   if (bad) { rumpy_set_error("rumpy_residual_norm_fwd: %s", bad); return RUMPY_E_ARG; }
   if (p->rows == 0) return RUMPY_OK;
@@ -379,6 +499,7 @@ extern "C" int rumpy_residual_norm_bwd(const rumpy_residual_norm_bwd_args* p, vo
   if (!bad && (!p->x || !p->partial || (!p->dy && !p->dh))) bad = "a tensor is missing";
   if (!bad && (p->dh && p->pre == RN_NONE)) bad = "dh without a norm in front";
   if (!bad && ((p->post != RN_NONE || p->dh) && !p->stats)) bad = "the statistics of the forward pass are missing";
+  if (!bad && ((uintptr_t)p->stats & 15)) bad = "stats lies at a multiple of 16 bytes";
   if (!bad && (p->ldx < 0 || p->ldt < 0 || p->ldg < 0 || p->lddy < 0 || p->lddh < 0)) bad = "row strides are not negative";
   if (!bad && (!p->t && (p->dt || p->dgate || p->d_post_w || p->d_post_b))) bad = "a gradient of a branch that is not there";
   if (!bad && (p->gate_mode == RN_GATE_NONE && p->dgate)) bad = "a gradient of a gate that is not there";
@@ -392,6 +513,6 @@ extern "C" int rumpy_residual_norm_bwd(const rumpy_residual_norm_bwd_args* p, vo
   hipStream_t s = (hipStream_t)stream;
   RN_BY_FORMAT(rn_launch_bwd, *p, plan, s);
   if (gate_rows || p->d_post_w || p->d_post_b || p->d_pre_w || p->d_pre_b)
-    hipLaunchKernelGGL(residual_norm_reduce_kernel, dim3((unsigned)(items * tiles)), dim3(256), 0, s, *p, plan, tiles);
+    hipLaunchKernelGGL(residual_norm_reduce_kernel, dim3((unsigned)(items * tiles)), dim3(64 * RN_SLICES), 0, s, *p, plan, tiles);
   return rumpy_check_launch("rumpy_residual_norm_bwd");
 }

@@ -57,7 +57,7 @@ def _forward(x, branch, gate, post_w, post_b, pre_w, pre_b, cfg, keep):
     tb = x if branch is None else branch
     y = torch.empty(x.shape, dtype=x.dtype, device=x.device) if branch is not None else None
     h = torch.empty(x.shape, dtype=tb.dtype, device=x.device) if pre else None
-    stats = torch.empty((4, rows), dtype=torch.float32, device=x.device) if keep else None
+    stats = torch.empty((rows, 4), dtype=torch.float32, device=x.device) if keep else None
     if rows == 0:
         return y, h, stats
     x, ldx = _rows(x)
