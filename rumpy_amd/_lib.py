@@ -326,7 +326,7 @@ class ResidualNormBwdArgs(_S):
 
 
 class TopLogitsArgs(_S):
-    _fields_ = [('logits', c_void_p), ('values', c_void_p), ('indices', c_void_p), ('tail', c_void_p), ('rows', c_int64), ('ld', c_int64), ('V', c_int32), ('k', c_int32), ('fmt', c_int32),
+    _fields_ = [('logits', c_void_p), ('values', c_void_p), ('indices', c_void_p), ('tail', c_void_p), ('work', c_void_p), ('rows', c_int64), ('ld', c_int64), ('V', c_int32), ('k', c_int32), ('fmt', c_int32),
                 ('inv_tau', c_float)]
 
 
@@ -374,6 +374,7 @@ SYMBOLS = {
     'rumpy_residual_norm_bwd': (C.c_int, [_P(ResidualNormBwdArgs), c_void_p]),
     'rumpy_residual_norm_partial_floats': (c_int64, [c_int64, c_int64, c_int32, c_int32]),
     'rumpy_top_logits': (C.c_int, [_P(TopLogitsArgs), c_void_p]),
+    'rumpy_top_logits_work_bytes': (c_int64, [c_int64, c_int32, c_int32]),
     'rumpy_distill_fwd': (C.c_int, [_P(DistillArgs), c_void_p]),
     'rumpy_distill_bwd': (C.c_int, [_P(DistillArgs), c_void_p]),
     'rumpy_distill_partial_floats': (c_int64, [c_int64, c_int32]),

@@ -49,198 +49,382 @@ __device__ __forceinline__ uint32_t order_key(float v) {
 
 __device__ __forceinline__ float key_value(uint32_t key) { return __uint_as_float(key & 0x80000000u ? key ^ 0x80000000u : ~key); }
 
-constexpr int TL_WG = 512, TL_WAVES = TL_WG / 64, TL_CAP = 2048;
+// (value, column) as one number: larger value first, then the lower column.  Never 0.
+__device__ __forceinline__ uint64_t pair_of(float v, int col) { return ((uint64_t)order_key(v) << 32) | (uint32_t)~(uint32_t)col; }
+__device__ __forceinline__ float pair_value(uint64_t p) { return key_value((uint32_t)(p >> 32)); }
 
-// fn(values, first column, count) over the row's pieces of CH elements, piece by piece over the threads; elements outside hold -inf
-template <int FMT, int CH, typename Fn> __device__ __forceinline__ void for_pieces(const typename RowElem<FMT>::type* z, int V, Fn fn) {
-  for (int64_t j = (int64_t)threadIdx.x * CH; j < V; j += TL_WG * CH) {
-    float v[8];
-    if constexpr (CH == 8) unpack_piece<FMT>(load_piece<FMT>(z + j, (int)min((int64_t)8, V - j), -INFINITY), v);
-    else v[0] = elem_to_f32<FMT>(z[j]);
-    fn(v, (int)j);
+constexpr int TL_WG = 512, TL_WAVES = TL_WG / 64, TL_CAP = 2048, TL_WAVE_CAP = 512;      // candidates of a row, of a wave
+constexpr float NOT_A_NUMBER = __builtin_nanf("");
+
+// Rows that are few and long are cut: every piece of a row gives its own k largest pairs and its tail to a workspace, and one more workgroup per
+// row joins them.
+struct TlPlan { int splits, seg; };
+static TlPlan tl_plan(int64_t rows, int32_t V) {
+  TlPlan p;
+  int64_t s = 1;
+  if (V >= 32768 && rows > 0) {
+    s = (256 + rows - 1) / rows;
+    const int64_t most = V / 8192;
+    if (s > most) s = most;
+    if (s > 32) s = 32;
   }
+  p.seg = (int)((((int64_t)V + s - 1) / s + 63) / 64 * 64);
+  p.splits = (int)(((int64_t)V + p.seg - 1) / p.seg);
+  return p;
 }
 
-// a bound that at least k of the row's elements reach: per wave the value that ceil(k / waves) of its lanes' maxima reach (a bitwise search on
-// ballots), the smallest of them over the waves
-template <int FMT, int CH> __device__ __forceinline__ float top_bound(const typename RowElem<FMT>::type* z, int V, int k, float* red) {
-  float mx = -INFINITY;
-  for_pieces<FMT, CH>(z, V, [&](const float (&v)[8], int) {
-#pragma unroll
-    for (int i = 0; i < CH; ++i) mx = fmaxf(mx, v[i]);            // (NaN is passed over here; the second look meets it)
-  });
-  const uint32_t key = order_key(mx);
-  const int want = (k + TL_WAVES - 1) / TL_WAVES;
+struct TlShared {
+  float red[TL_WAVES];
+  uint64_t cand[TL_WAVES][TL_WAVE_CAP + 16];
+  uint32_t count[TL_WAVES];
+  float after[TL_CAP];              // the candidates that are not chosen, by place
+  uint32_t hist[256];
+  uint32_t need;
+  uint64_t prefix, kth, next;
+};
+
+// the value that `want` lanes of every wave reach with their `mine` (a bitwise search on ballots), the smallest of them over the waves: a bound that
+// at least waves * want of the workgroup's values reach
+__device__ __forceinline__ uint32_t bound_of(uint32_t mine, int want, TlShared& sh) {
   uint32_t t = 0;
   for (int bit = 31; bit >= 0; --bit) {
     const uint32_t trial = t | (1u << bit);
-    if (__popcll(__ballot(key >= trial)) >= want) t = trial;
+    if (__popcll(__ballot(mine >= trial)) >= want) t = trial;
   }
   __syncthreads();
-  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = key_value(t);
+  if ((threadIdx.x & 63) == 0) sh.red[threadIdx.x >> 6] = __uint_as_float(t);
   __syncthreads();
-  float T = red[0];
+  uint32_t b = __float_as_uint(sh.red[0]);
 #pragma unroll
-  for (int i = 1; i < TL_WAVES; ++i) T = fminf(T, red[i]);
-  return T;
+  for (int i = 1; i < TL_WAVES; ++i) b = min(b, __float_as_uint(sh.red[i]));
+  return b;
 }
-// the second look: collects what reaches T; returns this thread's sum of exp2((z - T) c) over the rest
-template <int FMT, int CH> __device__ __forceinline__ float collect(const typename RowElem<FMT>::type* z, int V, float T, float c, uint64_t* cand, uint32_t* found) {
-  float sum = 0.f;
-  const float m = T * c;
-  for_pieces<FMT, CH>(z, V, [&](const float (&v)[8], int j) {
-    float s = 0.f, top = -INFINITY;
-#pragma unroll
-    for (int i = 0; i < CH; ++i) { s += __builtin_amdgcn_exp2f(fmaf(v[i], c, -m)); top = fmaxf(top, v[i]); }
-    if (top >= T) {
-      s = 0.f;
-#pragma unroll
-      for (int i = 0; i < CH; ++i) {
-        if (v[i] >= T) {
-          const uint32_t at = atomicAdd(found, 1u);
-          if (at < TL_CAP) cand[at] = ((uint64_t)order_key(v[i]) << 32) | (uint32_t)~(uint32_t)(j + i);
-        } else {
-          s += __builtin_amdgcn_exp2f(fmaf(v[i], c, -m));
-        }
+// the k-th largest of `count` different pairs, 8 bits at a time from the top: needs no assumption about them
+template <typename At> __device__ __forceinline__ uint64_t radix_kth(At at, int64_t count, int k, TlShared& sh) {
+  const int tid = threadIdx.x;
+  __syncthreads();
+  if (tid == 0) { sh.prefix = 0; sh.need = (uint32_t)k; }
+  for (int shift = 56; shift >= 0; shift -= 8) {
+    for (int i = tid; i < 256; i += TL_WG) sh.hist[i] = 0;
+    __syncthreads();
+    const uint64_t prefix = sh.prefix, mask = shift == 56 ? 0ull : ~0ull << (shift + 8);
+    const int64_t rounds = (count + TL_WG - 1) / TL_WG;
+    for (int64_t i = 0; i < rounds; ++i) {                   // (whole waves: the ballots need every lane)
+      const int64_t j = i * TL_WG + tid;
+      const uint64_t kk = j < count ? at(j) : 0;
+      const bool in = j < count && (kk & mask) == prefix;
+      const uint32_t bin = (uint32_t)(kk >> shift) & 255u;
+      uint64_t left = __ballot(in);
+      while (left) {                                       // one LDS add per distinct digit of the wave
+        const int first = __ffsll((unsigned long long)left) - 1;
+        const uint32_t b = __shfl(bin, first);
+        const uint64_t same = __ballot(in && bin == b) & left;
+        if ((tid & 63) == first) atomicAdd(&sh.hist[b], (uint32_t)__popcll(same));
+        left &= ~same;
       }
     }
-    sum += s;
-  });
-  return sum;
-}
-// log sum exp(z / tau) over the elements whose (key, ~index) pair lies below `kth`, by their maximum; every thread gets it
-template <int FMT> __device__ __forceinline__ float rest_below(const typename RowElem<FMT>::type* z, int V, uint64_t kth, float c, float inv_tau, float* red) {
-  float rmx = -INFINITY, bad = 0.f;
-  for (int64_t j = threadIdx.x; j < V; j += TL_WG) {
-    const float v = elem_to_f32<FMT>(z[j]);
-    if ((((uint64_t)order_key(v) << 32) | (uint32_t)~(uint32_t)j) < kth) { rmx = fmaxf(rmx, v); if (v != v) bad = 1.f; }
+    __syncthreads();
+    if (tid == 0) {
+      uint32_t need = sh.need, b = 255;
+      while (b > 0 && sh.hist[b] < need) { need -= sh.hist[b]; --b; }
+      sh.need = need;
+      sh.prefix = prefix | ((uint64_t)b << shift);
+    }
+    __syncthreads();
   }
+  return sh.prefix;
+}
+// Every wave keeps a list of its own in LDS, in the order of its walk: a place is the wave's count so far plus the hits in front in the wave, no atomics
+// and nothing to wait for.  Called by whole waves.
+__device__ __forceinline__ void push(bool hit, uint64_t p, uint32_t& count, TlShared& sh) {
+  const uint64_t hits = __ballot(hit);
+  if (hits) {
+    const uint32_t at = count + __builtin_amdgcn_mbcnt_hi((uint32_t)(hits >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)hits, 0));
+    if (hit && at < TL_WAVE_CAP) sh.cand[threadIdx.x >> 6][at] = p;
+    count += (uint32_t)__popcll(hits);
+  }
+}
+// closes the lists; returns the number of candidates (more than TL_CAP where a list is too long)
+__device__ __forceinline__ uint32_t lists_done(uint32_t count, TlShared& sh) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  if (lane < 16 && count <= TL_WAVE_CAP) sh.cand[wave][count + lane] = 0;             // (place looks at 16 at a time; no pair is 0)
+  if (lane == 0) sh.count[wave] = count;
+  __syncthreads();
+  uint32_t n = 0;
+#pragma unroll
+  for (int w = 0; w < TL_WAVES; ++w) n += sh.count[w] > TL_WAVE_CAP ? TL_CAP + 1 : sh.count[w];
+  return n;
+}
+// the candidates by their place, the number of candidates in front of them: emit(place, pair) for the first k; kth and next (0: there is none)
+// for what comes after
+template <typename Emit> __device__ __forceinline__ void place(int k, TlShared& sh, Emit emit) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  if (threadIdx.x == 0) sh.next = 0;
+  __syncthreads();
+  for (uint32_t i = lane; i < sh.count[wave]; i += 64) {
+    const uint64_t mine = sh.cand[wave][i];
+    uint32_t rank = 0;
+    for (int w = 0; w < TL_WAVES; ++w) {
+      for (uint32_t o = 0; o < sh.count[w]; o += 16) {
+        uint64_t other[16];
+#pragma unroll
+        for (int u = 0; u < 16; ++u) other[u] = sh.cand[w][o + u];
+#pragma unroll
+        for (int u = 0; u < 16; ++u) rank += other[u] > mine;
+      }
+    }
+    if (rank < (uint32_t)k) {
+      emit((int)rank, mine);
+      if (rank == (uint32_t)k - 1) sh.kth = mine;
+    } else {
+      sh.after[rank] = pair_value(mine);
+      if (rank == (uint32_t)k) sh.next = mine;
+    }
+  }
+  __syncthreads();
+}
+
+// A row (or a piece of one) as whole 16-byte pieces of 8 elements at aligned addresses, and up to 7 elements in front and behind (a row of odd
+// length starts anywhere: pieces at odd addresses run at two thirds of the rate).  NP > 0: a thread's NP pieces stay in registers, so that
+// the row is read once.
+template <int FMT, int NP> struct RowPieces {
+  typedef typename RowElem<FMT>::type E;
+  const E* z;
+  int len, head, count, tailn;
+  RowRaw<FMT> raw[NP > 0 ? NP : 1];
+  __device__ __forceinline__ RowPieces(const E* z_, int len_) : z(z_), len(len_) {
+    head = min(len, (int)((16u - (uint32_t)(uintptr_t)z % 16u) % 16u / (uint32_t)sizeof(E)));
+    count = (len - head) / 8;
+    tailn = len - head - 8 * count;
+  }
+  __device__ __forceinline__ void load() {
+    if constexpr (NP > 0) {
+#pragma unroll
+      for (int u = 0; u < NP; ++u) {
+        if (u * TL_WG >= count) break;
+        raw[u] = load_piece<FMT>(z + head + 8 * min(u * TL_WG + (int)threadIdx.x, count - 1), 8, 0.f);
+      }
+    }
+  }
+  // fn(8 values, column of the first): the thread's pieces; what lies outside the row is -inf
+  template <typename Fn> __device__ __forceinline__ void each(Fn fn) const {
+    float v[8];
+    if constexpr (NP > 0) {
+#pragma unroll
+      for (int u = 0; u < NP; ++u) {
+        if (u * TL_WG >= count) break;
+        unpack_piece<FMT>(raw[u], v);
+        const int p = u * TL_WG + (int)threadIdx.x;
+        if ((u + 1) * TL_WG > count) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) v[i] = p < count ? v[i] : -INFINITY;
+        }
+        fn(v, head + 8 * p);
+      }
+    } else {
+      for (int p0 = 0; p0 < count; p0 += TL_WG) {          // (whole waves)
+        const int p = p0 + (int)threadIdx.x;
+        unpack_piece<FMT>(load_piece<FMT>(z + head + (size_t)8 * min(p, count - 1), 8, 0.f), v);
+        if (p0 + TL_WG > count) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) v[i] = p < count ? v[i] : -INFINITY;
+        }
+        fn(v, head + 8 * p);
+      }
+    }
+    if (threadIdx.x < 64 && head + tailn) {          // the ends: lanes 0 and 1
+      const int first = threadIdx.x == 0 ? 0 : len - tailn, n = threadIdx.x == 0 ? head : threadIdx.x == 1 ? tailn : 0;
+      unpack_piece<FMT>(load_piece<FMT>(z + first, n, -INFINITY), v);
+      fn(v, first);
+    }
+  }
+  // fn(inside, value, column): single elements, threads in turn, by whole waves
+  template <typename Fn> __device__ __forceinline__ void each_element(Fn fn) const {
+    for (int64_t j0 = 0; j0 < len; j0 += TL_WG) {
+      const int64_t j = j0 + threadIdx.x;
+      fn(j < len, elem_to_f32<FMT>(z[min(j, (int64_t)len - 1)]), (int)j);
+    }
+  }
+};
+
+// log sum exp(z / tau) over the elements whose pair lies under `kth`, by their maximum; every thread gets it
+template <int FMT, int NP> __device__ __forceinline__ float rest_below(const RowPieces<FMT, NP>& row, uint64_t kth, float c, float inv_tau, float* red) {
+  float rmx = -INFINITY, bad = 0.f;
+  row.each_element([&](bool in, float v, int j) { if (in && pair_of(v, j) < kth) { rmx = fmaxf(rmx, v); if (v != v) bad = 1.f; } });
   rmx = block_max<TL_WAVES>(rmx, red);
-  if (block_max<TL_WAVES>(bad, red) > 0.f) return __uint_as_float(0x7fc00000u);
+  if (block_max<TL_WAVES>(bad, red) > 0.f) return NOT_A_NUMBER;
   if (!(fabsf(rmx) < INFINITY)) return rmx;
   float s = 0.f;
-  for (int64_t j = threadIdx.x; j < V; j += TL_WG) {
-    const float v = elem_to_f32<FMT>(z[j]);
-    if ((((uint64_t)order_key(v) << 32) | (uint32_t)~(uint32_t)j) < kth) s += __builtin_amdgcn_exp2f((v - rmx) * c);
-  }
-  s = block_sum<TL_WAVES>(s, red);
-  return fmaf(rmx, inv_tau, __builtin_amdgcn_logf(s) * LN2);
+  row.each_element([&](bool in, float v, int j) { if (in && pair_of(v, j) < kth) s += __builtin_amdgcn_exp2f((v - rmx) * c); });
+  return fmaf(rmx, inv_tau, __builtin_amdgcn_logf(block_sum<TL_WAVES>(s, red)) * LN2);
 }
 
-// One workgroup per row, two looks at it: the bound, then the few elements that reach it (a few times k) and the sum of exp over all others.
-// A candidate's place is the number of candidates in front of it (larger value, or equal and lower index).  Rows whose bound collects too
-// much or is not finite (fewer than about k finite elements), or that hold NaN, take the exact way: the k-th largest (value, index) pair by an
-// 8-bit radix search over the row, which needs no assumption about the values.
-template <int FMT> __global__ void __launch_bounds__(TL_WG) top_logits_kernel(rumpy_top_logits_args a) {
+// One workgroup per row or piece, two looks at it: a bound that at least k elements reach, from every thread's maximum; then the few elements
+// that reach the bound (a few times k) and the sum of exp over all others.  Rows whose bound collects too much or is not finite (fewer than about k
+// finite elements), or that hold NaN, take the exact way: the k-th pair by radix search.
+template <int FMT, int NP> __global__ void __launch_bounds__(TL_WG) top_logits_kernel(rumpy_top_logits_args a, TlPlan plan) {
   typedef typename RowElem<FMT>::type E;
-  __shared__ float red[TL_WAVES];
-  __shared__ uint64_t cand[TL_CAP];
-  __shared__ float after[TL_CAP];              // the candidates that are not chosen, by place: cand's own order is the atomics'
-  __shared__ uint32_t hist[256];
-  __shared__ uint32_t found, need_s;
-  __shared__ uint64_t prefix_s, kth_s, next_s;
-  const int tid = threadIdx.x, V = a.V, k = a.k;
+  __shared__ TlShared sh;
+  const int tid = threadIdx.x;
   const float c = a.inv_tau * LOG2E;
-  for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
-    const E* z = reinterpret_cast<const E*>(a.logits) + (size_t)row * a.ld;
-    uint32_t n = 0;
-    float T = 0.f, sum = 0.f;
-    bool exact_way = false;
-    if (tid == 0) { found = 0; next_s = 0; }
-    if (V <= TL_WG) {                                       // a row of one element per thread: all of them are candidates
-      if (tid < V) cand[tid] = ((uint64_t)order_key(elem_to_f32<FMT>(z[tid])) << 32) | (uint32_t)~(uint32_t)tid;
-      n = (uint32_t)V;
-      __syncthreads();
-    } else {
-      // single elements instead of pieces where pieces would leave threads (whole waves, then) without any
-      const bool pieces = V >= TL_WG * 8;
-      T = pieces ? top_bound<FMT, 8>(z, V, k, red) : top_bound<FMT, 1>(z, V, k, red);
-      exact_way = !(fabsf(T * c) < INFINITY) || !(fabsf(T) < INFINITY);
-      if (!exact_way) {
-        sum = pieces ? collect<FMT, 8>(z, V, T, c, cand, &found) : collect<FMT, 1>(z, V, T, c, cand, &found);
-        sum = block_sum<TL_WAVES>(sum, red);
-        n = found;
-        exact_way = n > TL_CAP || sum != sum;
-      }
-    }
-    if (exact_way) {
-      // (key << 32 | ~index), 8 bits at a time from the top
-      if (tid == 0) { prefix_s = 0; need_s = (uint32_t)k; }
-      for (int shift = 56; shift >= 0; shift -= 8) {
-        for (int i = tid; i < 256; i += TL_WG) hist[i] = 0;
-        __syncthreads();
-        const uint64_t prefix = prefix_s, mask = shift == 56 ? 0ull : ~0ull << (shift + 8);
-        const int64_t rounds = ((int64_t)V + TL_WG - 1) / TL_WG;
-        for (int64_t i = 0; i < rounds; ++i) {                   // (whole waves: the ballots below need every lane)
-          const int64_t j = i * TL_WG + tid;
-          bool in = j < V;
-          uint64_t kk = 0;
-          if (in) { kk = ((uint64_t)order_key(elem_to_f32<FMT>(z[j])) << 32) | (uint32_t)~(uint32_t)j; in = (kk & mask) == prefix; }
-          const uint32_t bin = (uint32_t)(kk >> shift) & 255u;
-          uint64_t left = __ballot(in);
-          while (left) {                                       // one LDS add per distinct digit of the wave
-            const int first = __ffsll((unsigned long long)left) - 1;
-            const uint32_t b = __shfl(bin, first);
-            const uint64_t same = __ballot(in && bin == b) & left;
-            if ((tid & 63) == first) atomicAdd(&hist[b], (uint32_t)__popcll(same));
-            left &= ~same;
-          }
+  const int64_t row = blockIdx.x / plan.splits;
+  const int piece = blockIdx.x % plan.splits, c0 = piece * plan.seg;
+  RowPieces<FMT, NP> r(reinterpret_cast<const E*>(a.logits) + (size_t)row * a.ld + c0, min(plan.seg, a.V - c0));
+  r.load();
+  const int len = r.len, k = min(a.k, len);
+  uint32_t n, mine = 0;                                   // candidates of the row, of the wave
+  float T = 0.f, sum = 0.f;
+  bool exact_way = false;
+  if (len <= TL_WG) {                                     // one element per thread: all of them are candidates
+    push(tid < len, pair_of(elem_to_f32<FMT>(r.z[min(tid, len - 1)]), tid), mine, sh);
+    n = lists_done(mine, sh);
+  } else {
+    // single elements instead of pieces where pieces would leave threads without any
+    const bool pieces = r.count >= TL_WG;
+    float mx = -INFINITY;                                 // (NaN is passed over here; the second look meets it)
+    if (pieces) r.each([&](const float (&v)[8], int) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) mx = fmaxf(mx, v[i]);
+    });
+    else r.each_element([&](bool in, float v, int) { mx = fmaxf(mx, in ? v : -INFINITY); });
+    T = key_value(bound_of(order_key(mx), (k + TL_WAVES - 1) / TL_WAVES, sh));
+    const float m = T * c;
+    exact_way = !(fabsf(m) < INFINITY && fabsf(T) < INFINITY);
+    if (!exact_way) {
+      if (pieces) r.each([&](const float (&v)[8], int j) {
+        bool any = false;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const bool hit = v[i] >= T;
+          any |= hit;
+          sum += __builtin_amdgcn_exp2f(fmaf(hit ? -INFINITY : v[i], c, -m));
         }
-        __syncthreads();
-        if (tid == 0) {
-          uint32_t need = need_s, b = 255;
-          while (b > 0 && hist[b] < need) { need -= hist[b]; --b; }
-          need_s = need;
-          prefix_s = prefix | ((uint64_t)b << shift);
+        if (__ballot(any)) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) push(v[i] >= T, pair_of(v[i], j + i), mine, sh);
         }
-        __syncthreads();
-      }
-      const uint64_t kth = prefix_s;                            // exactly k pairs are >= kth
-      if (tid == 0) found = 0;
-      __syncthreads();
-      for (int64_t j = tid; j < V; j += TL_WG) {
-        const uint64_t kk = ((uint64_t)order_key(elem_to_f32<FMT>(z[j])) << 32) | (uint32_t)~(uint32_t)j;
-        if (kk >= kth) { const uint32_t at = atomicAdd(&found, 1u); if (at < TL_CAP) cand[at] = kk; }
-      }
-      n = (uint32_t)k;
-      __syncthreads();
+      });
+      else r.each_element([&](bool in, float v, int j) {
+        const bool hit = in && v >= T;
+        push(hit, pair_of(v, j), mine, sh);
+        sum += __builtin_amdgcn_exp2f(fmaf(hit || !in ? -INFINITY : v, c, -m));
+      });
+      sum = block_sum<TL_WAVES>(sum, sh.red);
+      n = lists_done(mine, sh);
+      exact_way = n > TL_CAP || sum != sum;
     }
-    for (uint32_t i = tid; i < n; i += TL_WG) {
-      const uint64_t mine = cand[i];
-      uint32_t rank = 0;
-      for (uint32_t o = 0; o < n; ++o) rank += cand[o] > mine;
-      if (rank < (uint32_t)k) {
-        const uint32_t idx = ~(uint32_t)mine;
-        reinterpret_cast<E*>(a.values)[(size_t)row * k + rank] = z[idx];
-        reinterpret_cast<int64_t*>(a.indices)[(size_t)row * k + rank] = idx;
-        if (rank == (uint32_t)k - 1) kth_s = mine;
-      } else {
-        after[rank] = key_value((uint32_t)(mine >> 32));
-        if (rank == (uint32_t)k) next_s = mine;
-      }
+  }
+  if (exact_way) {
+    const uint64_t kth = radix_kth([&](int64_t j) { return pair_of(elem_to_f32<FMT>(r.z[j]), (int)j); }, len, k, sh);      // exactly k pairs reach it
+    mine = 0;
+    r.each_element([&](bool in, float v, int j) { const uint64_t p = pair_of(v, j); push(in && p >= kth, p, mine, sh); });
+    n = lists_done(mine, sh);
+  }
+  uint64_t* pairs = plan.splits > 1 ? (uint64_t*)a.work + (size_t)blockIdx.x * a.k : nullptr;
+  place(k, sh, [&](int at, uint64_t p) {
+    const uint32_t col = ~(uint32_t)p;
+    if (pairs) pairs[at] = p - (uint32_t)c0;               // ~(col + c0) = ~col - c0
+    else {
+      reinterpret_cast<E*>(a.values)[(size_t)row * a.k + at] = r.z[col];
+      reinterpret_cast<int64_t*>(a.indices)[(size_t)row * a.k + at] = col;
     }
-    __syncthreads();
-    float tail;
-    if (next_s == 0 && n < (uint32_t)V && (exact_way || sum < 1e-20f)) {
-      // nothing collected beyond the top, and the others lie so far under the bound that their sum has no digits left (or was not made)
-      tail = rest_below<FMT>(z, V, kth_s, c, a.inv_tau, red);
-    } else {
-      const float next = next_s ? key_value((uint32_t)(next_s >> 32)) : T;
-      if (n == (uint32_t)V && next_s == 0) tail = -INFINITY;      // k = V: nothing is left
-      else if (!(fabsf(next) < INFINITY)) tail = next;
-      else {
-        // relative to the largest that was not chosen: the other candidates, and the sum under the bound with T's distance from it
-        float s = 0.f;
-        for (uint32_t i = k + tid; i < n; i += TL_WG) s += __builtin_amdgcn_exp2f((after[i] - next) * c);
-        s = block_sum<TL_WAVES>(s, red) + (sum > 0.f ? sum * __builtin_amdgcn_exp2f((T - next) * c) : 0.f);
-        tail = fmaf(next, a.inv_tau, __builtin_amdgcn_logf(s) * LN2);
-      }
+  });
+  if (pairs && tid >= k && tid < a.k) pairs[tid] = 0;       // a piece shorter than k
+  float tail;
+  if (n == (uint32_t)len && sh.next == 0) tail = -INFINITY;      // everything is chosen
+  else if (sh.next == 0 && (exact_way || sum < 1e-20f)) {
+    // nothing collected beyond the top, and the others lie so far under the bound that their sum has no digits left (or was not made)
+    tail = rest_below<FMT, NP>(r, sh.kth, c, a.inv_tau, sh.red);
+  } else {
+    const float next = sh.next ? pair_value(sh.next) : T;
+    if (!(fabsf(next) < INFINITY)) tail = next;
+    else {
+      // relative to the largest that was not chosen: the other candidates, and the sum under the bound with T's distance from it
+      float s = 0.f;
+      for (uint32_t i = k + tid; i < n; i += TL_WG) s += __builtin_amdgcn_exp2f((sh.after[i] - next) * c);
+      s = block_sum<TL_WAVES>(s, sh.red) + (sum > 0.f ? sum * __builtin_amdgcn_exp2f((T - next) * c) : 0.f);
+      tail = fmaf(next, a.inv_tau, __builtin_amdgcn_logf(s) * LN2);
     }
-    if (tid == 0) a.tail[row] = tail;
-    __syncthreads();
+  }
+  if (tid == 0) {
+    if (pairs) reinterpret_cast<float*>((uint64_t*)a.work + (size_t)gridDim.x * a.k)[blockIdx.x] = tail;
+    else a.tail[row] = tail;
   }
 }
 
+// the pieces' pairs (each list in order) to the row's k, by the same two steps; what is left of them joins the pieces' tails
+template <int FMT> __global__ void __launch_bounds__(TL_WG) top_join_kernel(rumpy_top_logits_args a, TlPlan plan) {
+  typedef typename RowElem<FMT>::type E;
+  __shared__ TlShared sh;
+  const int tid = threadIdx.x, k = a.k, S = plan.splits, count = S * k;
+  const int64_t row = blockIdx.x;
+  const E* z = reinterpret_cast<const E*>(a.logits) + (size_t)row * a.ld;
+  const uint64_t* pairs = (const uint64_t*)a.work + (size_t)row * count;
+  const float* tails = reinterpret_cast<const float*>((const uint64_t*)a.work + (size_t)gridDim.x * count) + (size_t)row * S;
+  // the bound: of every list the pair that ceil(k / lists) of its pairs reach, the smallest of them
+  if (tid == 0) sh.prefix = ~0ull;
+  __syncthreads();
+  if (tid < S) atomicMin((unsigned long long*)&sh.prefix, (unsigned long long)pairs[tid * k + (k + S - 1) / S - 1]);
+  __syncthreads();
+  const uint64_t bound = sh.prefix;
+  auto gather = [&](uint64_t from) {
+    uint32_t mine = 0;
+    for (int j0 = 0; j0 < count; j0 += TL_WG) {
+      const int j = j0 + tid;
+      const uint64_t p = j < count ? pairs[j] : 0;
+      push(p && p >= from, p, mine, sh);
+    }
+    return lists_done(mine, sh);
+  };
+  uint32_t n = gather(bound);
+  if (n > TL_CAP || n < (uint32_t)k) {                   // (fewer than k: the last list is short)
+    const uint64_t kth = radix_kth([&](int64_t j) { return pairs[j]; }, count, k, sh);
+    n = gather(kth);
+  }
+  place(k, sh, [&](int at, uint64_t p) {
+    const uint32_t col = ~(uint32_t)p;
+    reinterpret_cast<E*>(a.values)[(size_t)row * k + at] = z[col];
+    reinterpret_cast<int64_t*>(a.indices)[(size_t)row * k + at] = col;
+  });
+  const uint64_t kth = sh.kth;
+  float m = -INFINITY, bad = 0.f;
+  for (int j = tid; j < count + S; j += TL_WG) {
+    const uint64_t p = j < count ? pairs[j] : 0;
+    if (j < count && (p >= kth || !p)) continue;
+    const float u = j < count ? pair_value(p) * a.inv_tau : tails[j - count];
+    m = fmaxf(m, u);
+    if (u != u) bad = 1.f;
+  }
+  m = block_max<TL_WAVES>(m, sh.red);
+  bad = block_max<TL_WAVES>(bad, sh.red);
+  float s = 0.f;
+  for (int j = tid; j < count + S; j += TL_WG) {
+    const uint64_t p = j < count ? pairs[j] : 0;
+    if (j < count && (p >= kth || !p)) continue;
+    const float u = j < count ? pair_value(p) * a.inv_tau : tails[j - count];
+    s += __builtin_amdgcn_exp2f((u - m) * LOG2E);
+  }
+  s = block_sum<TL_WAVES>(s, sh.red);
+  if (tid == 0) a.tail[row] = bad > 0.f ? NOT_A_NUMBER : fabsf(m) < INFINITY ? m + __builtin_amdgcn_logf(s) * LN2 : m;
+}
+
+extern "C" int64_t rumpy_top_logits_work_bytes(int64_t rows, int32_t V, int32_t k) {
+  if (rows <= 0 || V < 1 || V > DS_MAXV || k < 1 || k > DS_MAXK) return 0;
+  const TlPlan plan = tl_plan(rows, V);
+  return plan.splits > 1 ? rows * plan.splits * (k * 8 + 4) : 0;
+}
+template <int FMT> static void tl_launch(const rumpy_top_logits_args& a, const TlPlan& plan, hipStream_t s) {
+  // pieces a thread holds: 64 registers' worth at most
+  const dim3 grid((unsigned)(a.rows * plan.splits)), wg(TL_WG);
+  const int np = (plan.seg / 8 + TL_WG - 1) / TL_WG, len = a.V < plan.seg ? a.V : plan.seg;
+  constexpr int MOST = FMT == RUMPY_FMT_F32 ? 8 : 16;
+  if (len < TL_WG * 8 || np > MOST) hipLaunchKernelGGL((top_logits_kernel<FMT, 0>), grid, wg, 0, s, a, plan);
+  else if (np <= 2) hipLaunchKernelGGL((top_logits_kernel<FMT, 2>), grid, wg, 0, s, a, plan);
+  else if (np <= 4) hipLaunchKernelGGL((top_logits_kernel<FMT, 4>), grid, wg, 0, s, a, plan);
+  else if (np <= 8) hipLaunchKernelGGL((top_logits_kernel<FMT, 8>), grid, wg, 0, s, a, plan);
+  else hipLaunchKernelGGL((top_logits_kernel<FMT, MOST>), grid, wg, 0, s, a, plan);
+  if (plan.splits > 1) hipLaunchKernelGGL((top_join_kernel<FMT>), dim3((unsigned)a.rows), wg, 0, s, a, plan);
+}
 extern "C" int rumpy_top_logits(const rumpy_top_logits_args* p, void* stream) {
   const char* bad = !p ? "no arguments" : nullptr;
   if (!bad && (p->fmt != RUMPY_FMT_F32 && p->fmt != RUMPY_FMT_BF16 && p->fmt != RUMPY_FMT_F16)) bad = "fp32, bf16 or fp16 logits";
@@ -248,13 +432,16 @@ extern "C" int rumpy_top_logits(const rumpy_top_logits_args* p, void* stream) {
   if (!bad && (p->k < 1 || p->k > DS_MAXK || p->k > p->V)) bad = "1 .. 256 top logits, no more than the row has";
   if (!bad && !(p->inv_tau > 0.f && p->inv_tau < INFINITY)) bad = "a temperature above zero";
   if (!bad && p->rows && (!p->logits || !p->values || !p->indices || !p->tail)) bad = "a tensor is missing";
+  if (!bad && rumpy_top_logits_work_bytes(p->rows, p->V, p->k) && (!p->work || ((uintptr_t)p->work & 7)))
+    bad = "rows of this length and number are cut and need `work` (rumpy_top_logits_work_bytes, at a multiple of 8)";
+  if (!bad && p->rows > 0x7fffffff) bad = "too many rows";
   if (bad) { rumpy_set_error("rumpy_top_logits: %s", bad); return RUMPY_E_ARG; }
   if (p->rows == 0) return RUMPY_OK;
-  const dim3 grid((unsigned)(p->rows < 65536 ? p->rows : 65536));
+  const TlPlan plan = tl_plan(p->rows, p->V);
   hipStream_t s = (hipStream_t)stream;
-  if (p->fmt == RUMPY_FMT_F32) hipLaunchKernelGGL((top_logits_kernel<RUMPY_FMT_F32>), grid, dim3(TL_WG), 0, s, *p);
-  else if (p->fmt == RUMPY_FMT_BF16) hipLaunchKernelGGL((top_logits_kernel<RUMPY_FMT_BF16>), grid, dim3(TL_WG), 0, s, *p);
-  else hipLaunchKernelGGL((top_logits_kernel<RUMPY_FMT_F16>), grid, dim3(TL_WG), 0, s, *p);
+  if (p->fmt == RUMPY_FMT_F32) tl_launch<RUMPY_FMT_F32>(*p, plan, s);
+  else if (p->fmt == RUMPY_FMT_BF16) tl_launch<RUMPY_FMT_BF16>(*p, plan, s);
+  else tl_launch<RUMPY_FMT_F16>(*p, plan, s);
   return rumpy_check_launch("rumpy_top_logits");
 }
 
@@ -301,23 +488,32 @@ __device__ __forceinline__ float ds_value(const rumpy_distill_args& a, int64_t r
 
 // what the teacher lists of a row, in LDS.  idx -1 = an entry that is not used (negative index); -2 = outside the row (the row becomes NaN).
 // first[i]: no earlier entry names the same column
-struct DsListed { int idx[DS_MAXK]; float v[DS_MAXK]; float z[DS_MAXK]; uint8_t first[DS_MAXK]; };
-template <int FMT> __device__ __forceinline__ void ds_load_listed(const rumpy_distill_args& a, int64_t row, const typename RowElem<FMT>::type* z, DsListed& l) {
+struct DsListed { int idx[DS_MAXK]; float v[DS_MAXK]; float z[DS_MAXK]; bool first[DS_MAXK]; };
+template <int FMT> __device__ __forceinline__ int ds_load_listed(const rumpy_distill_args& a, int64_t row, const typename RowElem<FMT>::type* z, DsListed& l) {
   const int tid = threadIdx.x;
+  int mine = -1;
   if (tid < a.k) {
     const int64_t i = ds_index(a, row, tid);
     const bool inside = i >= 0 && i < a.V;
-    l.idx[tid] = i < 0 ? -1 : inside ? (int)i : -2;
+    mine = i < 0 ? -1 : inside ? (int)i : -2;
+    l.idx[tid] = mine;
     l.v[tid] = ds_value(a, row, tid);
     l.z[tid] = inside ? elem_to_f32<FMT>(z[i]) : 0.f;
   }
   __syncthreads();
-  if (tid < a.k) {
+  // (16 at a time, from LDS whole: one by one every look waits for the one before it - 20 us for 256 entries)
+  if (a.tail && tid < a.k) {
     bool f = true;
-    const int mine = l.idx[tid];
-    for (int o = 0; o < a.k; ++o) f &= !(o < tid && l.idx[o] == mine);
+    for (int o = 0; o < a.k; o += 16) {
+      int other[16];
+#pragma unroll
+      for (int i = 0; i < 16; ++i) other[i] = l.idx[o + i];
+#pragma unroll
+      for (int i = 0; i < 16; ++i) f &= !(o + i < tid && other[i] == mine);
+    }
     l.first[tid] = f;
   }
+  return mine;
 }
 
 // one wave: the row's loss and what its gradient needs, from the sum over the streamed columns (all of them, or the unlisted ones when the
@@ -402,32 +598,40 @@ template <int FMT, bool REST> __global__ void __launch_bounds__(DS_WG) distill_f
     return;
   }
   const int64_t j0 = (int64_t)piece * plan.seg, j1 = min((int64_t)a.V, j0 + plan.seg);
-  if (plan.splits == 1) ds_load_listed<FMT>(a, row, z, l);
+  // whole pieces lie at 16-byte addresses (RowPieces); their bits at whole bytes: column j of the piece of the row has bit j - j0 + shift
+  const RowPieces<FMT, 0> r(z + j0, (int)(j1 - j0));
+  const int shift = (8 - r.head) & 7, body = r.head ? 1 : 0;
+  const uint8_t* bytes = reinterpret_cast<const uint8_t*>(bits);
+  // U pieces are asked for before the U before them are summed (the first before anything else); their maximum is joined once
+  constexpr int U = FMT == RUMPY_FMT_F32 ? 2 : 4;
+  RowRaw<FMT> raw[U];
+  const int whole = r.count / (DS_WG * U);             // rounds in which every thread has U whole pieces
+  const E* zp = r.z + r.head + tid * 8;
+  if (whole) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) raw[u] = load_piece<FMT>(zp + u * DS_WG * 8, 8, 0.f);
+  }
   if constexpr (REST) {
-    const int words = (int)((j1 - j0 + 31) / 32);
+    const int words = (r.len + 7 + 31) / 32;
     for (int i = tid; i < words; i += DS_WG) bits[i] = 0;
-    __syncthreads();
-    if (tid < a.k) {
-      const int64_t i = ds_index(a, row, tid);
-      if (i >= j0 && i < j1) atomicOr(&bits[(i - j0) >> 5], 1u << ((i - j0) & 31));
-    }
+    if (plan.splits > 1) __syncthreads();
+  }
+  int64_t mine = -1;
+  if (plan.splits == 1) mine = ds_load_listed<FMT>(a, row, z, l);      // (holds a barrier)
+  else if (REST && tid < a.k) mine = ds_index(a, row, tid);
+  if constexpr (REST) {
+    if (mine >= j0 && mine < j1) { const int bit = (int)(mine - j0) + shift; atomicOr(&bits[bit >> 5], 1u << (bit & 31)); }
     __syncthreads();
   }
   const float c = a.inv_tau * LOG2E;
   float m = -INFINITY, s = 0.f, mc = 0.f;
-  for (int64_t j = j0 + tid * 8; j < j1; j += DS_WG * 8) {
-    float v[8];
-    unpack_piece<FMT>(load_piece<FMT>(z + j, (int)min((int64_t)8, j1 - j), -INFINITY), v);
-    if constexpr (REST) {
-      const uint32_t here = reinterpret_cast<const uint8_t*>(bits)[(j - j0) >> 3];
-      if (here) {
+  auto sum_up = [&](auto& v) {
+    constexpr int N = sizeof(v) / sizeof(v[0]);
+    float top = v[0][0];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) if (here >> i & 1u) v[i] = -INFINITY;
-      }
-    }
-    float top = v[0];
+    for (int u = 0; u < N; ++u)
 #pragma unroll
-    for (int i = 1; i < 8; ++i) top = fmaxf(top, v[i]);
+      for (int i = 0; i < 8; ++i) top = fmaxf(top, v[u][i]);
     if (top > m) {
       s *= ds_rescale(m, top, c);
       m = top;
@@ -435,11 +639,56 @@ template <int FMT, bool REST> __global__ void __launch_bounds__(DS_WG) distill_f
     }
     if (fabsf(mc) < INFINITY) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) s += __builtin_amdgcn_exp2f(fmaf(v[i], c, -mc));
+      for (int u = 0; u < N; ++u)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) s += __builtin_amdgcn_exp2f(fmaf(v[u][i], c, -mc));
     } else {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) s += __builtin_amdgcn_exp2f((v[i] - m) * c);
+      for (int u = 0; u < N; ++u)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) s += __builtin_amdgcn_exp2f((v[u][i] - m) * c);
     }
+  };
+  auto leave_out = [&](float (&v)[8], uint32_t here) {
+    if (here) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) if (here >> i & 1u) v[i] = -INFINITY;
+    }
+  };
+  for (int b = 0; b < whole; ++b) {
+    float v[U][8];
+    uint32_t here[U];
+    if constexpr (REST) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) here[u] = bytes[(b * U + u) * DS_WG + tid + body];
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) unpack_piece<FMT>(raw[u], v[u]);
+    const E* next = zp + (size_t)min(b + 1, whole - 1) * (DS_WG * 8 * U);
+#pragma unroll
+    for (int u = 0; u < U; ++u) raw[u] = load_piece<FMT>(next + u * DS_WG * 8, 8, 0.f);
+    if constexpr (REST) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) leave_out(v[u], here[u]);
+    }
+    sum_up(v);
+  }
+  for (int p0 = whole * DS_WG * U; p0 < r.count; p0 += DS_WG) {
+    const int p = p0 + tid;
+    float v[1][8];
+    unpack_piece<FMT>(load_piece<FMT>(r.z + r.head + (size_t)8 * min(p, r.count - 1), 8, 0.f), v[0]);
+    leave_out(v[0], p >= r.count ? 0xffu : REST ? bytes[p + body] : 0u);
+    sum_up(v);
+  }
+  if (tid < 64 && r.head + r.tailn) {                  // the ends: lanes 0 and 1
+    const int first = tid == 0 ? 0 : r.len - r.tailn, n = tid == 0 ? r.head : tid == 1 ? r.tailn : 0;
+    float v[1][8];
+    unpack_piece<FMT>(load_piece<FMT>(r.z + first, n, -INFINITY), v[0]);
+    if constexpr (REST) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) { const int bit = first + i + shift; if (i < n && (bytes[bit >> 3] >> (bit & 7) & 1u)) v[0][i] = -INFINITY; }
+    }
+    sum_up(v);
   }
   const float M = block_max<DS_WAVES>(m, red);
   s = block_sum<DS_WAVES>(m == -INFINITY ? s : s * ds_rescale(m, M, c), red);
@@ -527,7 +776,15 @@ template <int FMT> __global__ void __launch_bounds__(DS_WG) distill_bwd_kernel(r
   __syncthreads();          // the listed columns are written over (same workgroup, behind the barrier); a column listed twice takes both shares
   if (tid < a.k && idx[tid] >= 0) {
     float share = 0.f;
-    for (int o = 0; o < a.k; ++o) share += idx[o] == idx[tid] ? p[o] : 0.f;
+    const int mine = idx[tid];
+    for (int o = 0; o < a.k; o += 16) {
+      int other[16];
+      float po[16];
+#pragma unroll
+      for (int i = 0; i < 16; ++i) { other[i] = idx[o + i]; po[i] = p[o + i]; }
+#pragma unroll
+      for (int i = 0; i < 16; ++i) share += o + i < a.k && other[i] == mine ? po[i] : 0.f;
+    }
     const float q = __builtin_amdgcn_exp2f(((elem_to_f32<FMT>(z[idx[tid]]) - st[2]) * a.inv_tau - st[3]) * LOG2E);
     reinterpret_cast<E*>(a.dlogits)[out + idx[tid]] = f32_to_elem<FMT>(g * (q - share));
   }
@@ -555,7 +812,7 @@ extern "C" int64_t rumpy_distill_partial_floats(int64_t rows, int32_t V) {
 
 template <int FMT> static void ds_launch_fwd(const rumpy_distill_args& a, const DsPlan& plan, hipStream_t s) {
   const dim3 grid((unsigned)(a.rows * plan.splits));
-  const size_t lds = a.tail ? ((size_t)(plan.splits == 1 ? a.V : plan.seg) + 31) / 32 * 4 : 0;
+  const size_t lds = a.tail ? ((size_t)(plan.splits == 1 ? a.V : plan.seg) + 7 + 31) / 32 * 4 : 0;
   if (a.tail) hipLaunchKernelGGL((distill_fwd_kernel<FMT, true>), grid, dim3(DS_WG), lds, s, a, plan);
   else hipLaunchKernelGGL((distill_fwd_kernel<FMT, false>), grid, dim3(DS_WG), 0, s, a, plan);
   if (plan.splits > 1) hipLaunchKernelGGL((distill_join_kernel<FMT>), dim3((unsigned)a.rows), dim3(DS_WG), 0, s, a, plan);

@@ -52,8 +52,11 @@ def top_logits(logits, k, temperature=1.0):
     if logits.numel() == 0:
         return values, indices, tail
     z, ld = _rows(logits)
-    _launch('rumpy_top_logits', L.TopLogitsArgs(logits=z.data_ptr(), values=values.data_ptr(), indices=indices.data_ptr(), tail=tail.data_ptr(),
-                                                rows=logits.numel() // v, ld=ld, V=v, k=k, fmt=_FMT[logits.dtype], inv_tau=1.0 / t), logits.device)
+    rows = logits.numel() // v
+    wb = int(L.lib().rumpy_top_logits_work_bytes(rows, v, k))
+    work = torch.empty(wb, dtype=torch.uint8, device=logits.device) if wb else None
+    _launch('rumpy_top_logits', L.TopLogitsArgs(logits=z.data_ptr(), values=values.data_ptr(), indices=indices.data_ptr(), tail=tail.data_ptr(), work=_p(work),
+                                                rows=rows, ld=ld, V=v, k=k, fmt=_FMT[logits.dtype], inv_tau=1.0 / t), logits.device)
     return values, indices, tail
 
 

@@ -95,6 +95,26 @@ def test_top_logits_with_masks_and_odd_values(cols, dtype):
         _check_top(z, 64, tau)
 
 
+@pytest.mark.parametrize('dtype', [F32, BF16, F16], ids=str)
+@pytest.mark.parametrize('rows,cols,offset', [(1, 32768, 0), (3, 32769, 1), (2, 65537, 3), (5, 100000, 5), (1, 270001, 7), (1, 73729, 0), (130, 33001, 1)])
+def test_top_logits_of_rows_that_are_cut(rows, cols, offset, dtype):
+    """few long rows: the pieces' own selections and their join, with pieces that hold everything, nothing, equal values or a short end"""
+    g = torch.Generator().manual_seed(cols)
+    z = torch.zeros(rows, cols + 8)
+    z[:, offset:offset + cols] = torch.randn(rows, cols, generator=g).mul(3)
+    z[0, offset:offset + 9000] += 20.0               # the first piece has all of the top
+    if rows > 1:
+        z[1] = (torch.arange(cols + 8) % 5).float()
+    if rows > 2:
+        z[2, 100:] = -INF
+        z[2, offset + cols - 30:] = 1.0
+    for i in range(3, min(rows, 6)):
+        z[i, offset + 17 * i] = (NAN, INF, -INF)[i - 3]
+    z = z.to(dtype).to(DEV)[:, offset:offset + cols]
+    for k in (1, 100, 256):
+        _check_top(z, k, 0.5)
+
+
 def test_top_logits_of_slices_and_leading_dimensions():
     g = torch.Generator().manual_seed(8)
     wide = torch.randn(6, 8200, generator=g).to(DEV)

@@ -79,7 +79,8 @@ def test_norm_backward_entry_point_refuses(bad):
 
 
 @pytest.mark.parametrize('bad', [dict(k=0), dict(k=257), dict(V=9, k=10), dict(V=0), dict(V=2 ** 30 + 1), dict(rows=-1), dict(ld=-1), dict(fmt=2), dict(inv_tau=0.0),
-                                 dict(inv_tau=float('inf')), dict(inv_tau=float('nan')), dict(logits=None), dict(values=None), dict(indices=None), dict(tail=None)], ids=str)
+                                 dict(inv_tau=float('inf')), dict(inv_tau=float('nan')), dict(logits=None), dict(values=None), dict(indices=None), dict(tail=None),
+                                 dict(V=200000, rows=1), dict(V=200000, rows=1, work=P + 4), dict(rows=2 ** 31)], ids=str)
 def test_top_logits_entry_point_refuses(bad):
     lib = _lib_or_skip()
     d = dict(logits=P, values=P, indices=P, tail=P, rows=3, ld=500, V=500, k=10, fmt=L.FMT_F32, inv_tau=1.0)
@@ -111,6 +112,8 @@ def test_workspace_sizes():
         assert n // c >= 4 + (rows // group if mode == 1 else 0)
     assert lib.rumpy_distill_partial_floats(0, 100000) == 0 and lib.rumpy_distill_partial_floats(4096, 50000) == 0
     assert lib.rumpy_distill_partial_floats(1, 262144) > 0
+    assert lib.rumpy_top_logits_work_bytes(1000, 50000, 64) == 0 and lib.rumpy_top_logits_work_bytes(32, 8192, 64) == 0
+    assert lib.rumpy_top_logits_work_bytes(1, 262144, 64) > 0 and lib.rumpy_top_logits_work_bytes(1, 262144, 257) == 0
 
 
 # ---------------------------------------------------------------------------------------------------------------- Python refusals
