@@ -53,12 +53,13 @@ __device__ __forceinline__ float key_value(uint32_t key) { return __uint_as_floa
 __device__ __forceinline__ uint64_t pair_of(float v, int col) { return ((uint64_t)order_key(v) << 32) | (uint32_t)~(uint32_t)col; }
 __device__ __forceinline__ float pair_value(uint64_t p) { return key_value((uint32_t)(p >> 32)); }
 
-constexpr int TL_WG = 512, TL_WAVES = TL_WG / 64, TL_CAP = 2048, TL_WAVE_CAP = 512;      // candidates of a row, of a wave
+constexpr int TL_WAVE_CAP = 256;      // candidates of a wave
 constexpr float NOT_A_NUMBER = __builtin_nanf("");
 
 // Rows that are few and long are cut: every piece of a row gives its own k largest pairs and its tail to a workspace, and one more workgroup per
 // row joins them.
 struct TlPlan { int splits, seg; };
+constexpr int TL_MOST_SPLITS = 32;
 static TlPlan tl_plan(int64_t rows, int32_t V) {
   TlPlan p;
   int64_t s = 1;
@@ -66,51 +67,53 @@ static TlPlan tl_plan(int64_t rows, int32_t V) {
     s = (256 + rows - 1) / rows;
     const int64_t most = V / 8192;
     if (s > most) s = most;
-    if (s > 32) s = 32;
+    if (s > TL_MOST_SPLITS) s = TL_MOST_SPLITS;
   }
   p.seg = (int)((((int64_t)V + s - 1) / s + 63) / 64 * 64);
   p.splits = (int)(((int64_t)V + p.seg - 1) / p.seg);
   return p;
 }
 
-struct TlShared {
-  float red[TL_WAVES];
-  uint64_t cand[TL_WAVES][TL_WAVE_CAP + 16];
-  uint32_t count[TL_WAVES];
-  float after[TL_CAP];              // the candidates that are not chosen, by place
+template <int WG> struct TlShared {
+  static constexpr int WAVES = WG / 64;
+  float red[WAVES];
+  uint64_t cand[WAVES][TL_WAVE_CAP + 16];
+  uint32_t count[WAVES];
+  float after[WAVES * TL_WAVE_CAP];              // the candidates that are not chosen, by place
   uint32_t hist[256];
   uint32_t need;
   uint64_t prefix, kth, next;
 };
 
 // the value that `want` lanes of every wave reach with their `mine` (a bitwise search on ballots), the smallest of them over the waves: a bound that
-// at least waves * want of the workgroup's values reach
-__device__ __forceinline__ uint32_t bound_of(uint32_t mine, int want, TlShared& sh) {
+// at least waves * want of the workgroup's values reach.  LOW: bits that only repeat the sign in this format's keys
+template <int WG, int LOW> __device__ __forceinline__ uint32_t bound_of(uint32_t mine, int want, TlShared<WG>& sh) {
   uint32_t t = 0;
-  for (int bit = 31; bit >= 0; --bit) {
+  for (int bit = 31; bit >= LOW; --bit) {
     const uint32_t trial = t | (1u << bit);
     if (__popcll(__ballot(mine >= trial)) >= want) t = trial;
   }
+  if (!(t & 0x80000000u)) t |= (1u << LOW) - 1u;
   __syncthreads();
   if ((threadIdx.x & 63) == 0) sh.red[threadIdx.x >> 6] = __uint_as_float(t);
   __syncthreads();
   uint32_t b = __float_as_uint(sh.red[0]);
 #pragma unroll
-  for (int i = 1; i < TL_WAVES; ++i) b = min(b, __float_as_uint(sh.red[i]));
+  for (int i = 1; i < WG / 64; ++i) b = min(b, __float_as_uint(sh.red[i]));
   return b;
 }
 // the k-th largest of `count` different pairs, 8 bits at a time from the top: needs no assumption about them
-template <typename At> __device__ __forceinline__ uint64_t radix_kth(At at, int64_t count, int k, TlShared& sh) {
+template <int WG, typename At> __device__ __forceinline__ uint64_t radix_kth(At at, int64_t count, int k, TlShared<WG>& sh) {
   const int tid = threadIdx.x;
   __syncthreads();
   if (tid == 0) { sh.prefix = 0; sh.need = (uint32_t)k; }
   for (int shift = 56; shift >= 0; shift -= 8) {
-    for (int i = tid; i < 256; i += TL_WG) sh.hist[i] = 0;
+    for (int i = tid; i < 256; i += WG) sh.hist[i] = 0;
     __syncthreads();
     const uint64_t prefix = sh.prefix, mask = shift == 56 ? 0ull : ~0ull << (shift + 8);
-    const int64_t rounds = (count + TL_WG - 1) / TL_WG;
+    const int64_t rounds = (count + WG - 1) / WG;
     for (int64_t i = 0; i < rounds; ++i) {                   // (whole waves: the ballots need every lane)
-      const int64_t j = i * TL_WG + tid;
+      const int64_t j = i * WG + tid;
       const uint64_t kk = j < count ? at(j) : 0;
       const bool in = j < count && (kk & mask) == prefix;
       const uint32_t bin = (uint32_t)(kk >> shift) & 255u;
@@ -136,7 +139,7 @@ template <typename At> __device__ __forceinline__ uint64_t radix_kth(At at, int6
 }
 // Every wave keeps a list of its own in LDS, in the order of its walk: a place is the wave's count so far plus the hits in front in the wave, no atomics
 // and nothing to wait for.  Called by whole waves.
-__device__ __forceinline__ void push(bool hit, uint64_t p, uint32_t& count, TlShared& sh) {
+template <int WG> __device__ __forceinline__ void push(bool hit, uint64_t p, uint32_t& count, TlShared<WG>& sh) {
   const uint64_t hits = __ballot(hit);
   if (hits) {
     const uint32_t at = count + __builtin_amdgcn_mbcnt_hi((uint32_t)(hits >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)hits, 0));
@@ -144,35 +147,68 @@ __device__ __forceinline__ void push(bool hit, uint64_t p, uint32_t& count, TlSh
     count += (uint32_t)__popcll(hits);
   }
 }
-// closes the lists; returns the number of candidates (more than TL_CAP where a list is too long)
-__device__ __forceinline__ uint32_t lists_done(uint32_t count, TlShared& sh) {
+// closes the lists and puts each in order (by counting the larger pairs of the list, 16 at a time from LDS); returns the number of candidates, or
+// ~0 where a list is too long
+template <int WG> __device__ __forceinline__ uint32_t lists_done(uint32_t count, TlShared<WG>& sh) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  if (lane < 16 && count <= TL_WAVE_CAP) sh.cand[wave][count + lane] = 0;             // (place looks at 16 at a time; no pair is 0)
+  uint64_t* list = sh.cand[wave];
+  if (count <= TL_WAVE_CAP) {
+    if (lane < 16) list[count + lane] = 0;             // (no pair is 0)
+    uint64_t mine[TL_WAVE_CAP / 64];
+    uint32_t rank[TL_WAVE_CAP / 64];
+#pragma unroll
+    for (int i = 0; i < TL_WAVE_CAP / 64; ++i) {
+      if (i * 64 >= count) break;
+      mine[i] = i * 64 + lane < count ? list[i * 64 + lane] : 0;
+      rank[i] = 0;
+      for (uint32_t o = 0; o < count; o += 16) {
+        uint64_t other[16];
+#pragma unroll
+        for (int u = 0; u < 16; ++u) other[u] = list[o + u];
+#pragma unroll
+        for (int u = 0; u < 16; ++u) rank[i] += other[u] > mine[i];
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < TL_WAVE_CAP / 64; ++i) {       // (a wave's LDS accesses stay in order: every pair is in a register by now)
+      if (i * 64 >= count) break;
+      if (i * 64 + lane < count) list[rank[i]] = mine[i];
+    }
+  }
   if (lane == 0) sh.count[wave] = count;
   __syncthreads();
   uint32_t n = 0;
+  bool over = false;
 #pragma unroll
-  for (int w = 0; w < TL_WAVES; ++w) n += sh.count[w] > TL_WAVE_CAP ? TL_CAP + 1 : sh.count[w];
-  return n;
+  for (int w = 0; w < WG / 64; ++w) { n += sh.count[w]; over |= sh.count[w] > TL_WAVE_CAP; }
+  return over ? ~0u : n;
 }
-// the candidates by their place, the number of candidates in front of them: emit(place, pair) for the first k; kth and next (0: there is none)
-// for what comes after
-template <typename Emit> __device__ __forceinline__ void place(int k, TlShared& sh, Emit emit) {
+// the candidates by their place among all: the place in the wave's own list and the larger pairs of the others, searched in all of them at once:
+// emit(place, pair) for the first k; kth and next (0: there is none) for what comes after
+template <int WG, typename Emit> __device__ __forceinline__ void place(int k, TlShared<WG>& sh, Emit emit) {
+  constexpr int WAVES = WG / 64;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   if (threadIdx.x == 0) sh.next = 0;
+  uint32_t most = 1;
+#pragma unroll
+  for (int w = 0; w < WAVES; ++w) most = max(most, sh.count[w]);
+  const uint32_t top = 1u << (31 - __clz((int)most));
   __syncthreads();
   for (uint32_t i = lane; i < sh.count[wave]; i += 64) {
     const uint64_t mine = sh.cand[wave][i];
-    uint32_t rank = 0;
-    for (int w = 0; w < TL_WAVES; ++w) {
-      for (uint32_t o = 0; o < sh.count[w]; o += 16) {
-        uint64_t other[16];
+    uint32_t in_front[WAVES];
 #pragma unroll
-        for (int u = 0; u < 16; ++u) other[u] = sh.cand[w][o + u];
+    for (int w = 0; w < WAVES; ++w) in_front[w] = 0;
+    for (uint32_t b = top; b; b >>= 1) {
+      uint64_t other[WAVES];
 #pragma unroll
-        for (int u = 0; u < 16; ++u) rank += other[u] > mine;
-      }
+      for (int w = 0; w < WAVES; ++w) other[w] = sh.cand[w][min(in_front[w] + b, (uint32_t)TL_WAVE_CAP) - 1];
+#pragma unroll
+      for (int w = 0; w < WAVES; ++w) if (in_front[w] + b <= sh.count[w] && other[w] > mine) in_front[w] += b;
     }
+    uint32_t rank = 0;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) rank += in_front[w];
     if (rank < (uint32_t)k) {
       emit((int)rank, mine);
       if (rank == (uint32_t)k - 1) sh.kth = mine;
@@ -185,62 +221,72 @@ template <typename Emit> __device__ __forceinline__ void place(int k, TlShared& 
 }
 
 // A row (or a piece of one) as whole 16-byte pieces of 8 elements at aligned addresses, and up to 7 elements in front and behind (a row of odd
-// length starts anywhere: pieces at odd addresses run at two thirds of the rate).  NP > 0: a thread's NP pieces stay in registers, so that
-// the row is read once.
-template <int FMT, int NP> struct RowPieces {
+// length starts anywhere: pieces at odd addresses run at two thirds of the rate).  NP > 1: a thread's NP pieces stay in registers, so that
+// the row is read once.  NP 1: rows of at most 8 WG elements, element by element over the threads (pieces would leave waves without any).
+template <int FMT, int WG, int NP> struct RowPieces {
   typedef typename RowElem<FMT>::type E;
   const E* z;
   int len, head, count, tailn;
-  RowRaw<FMT> raw[NP > 0 ? NP : 1];
+  RowRaw<FMT> raw[NP > 1 ? NP : 1];
+  E one[NP == 1 ? 8 : 1];
   __device__ __forceinline__ RowPieces(const E* z_, int len_) : z(z_), len(len_) {
     head = min(len, (int)((16u - (uint32_t)(uintptr_t)z % 16u) % 16u / (uint32_t)sizeof(E)));
     count = (len - head) / 8;
     tailn = len - head - 8 * count;
   }
   __device__ __forceinline__ void load() {
-    if constexpr (NP > 0) {
+    if constexpr (NP > 1) {
 #pragma unroll
       for (int u = 0; u < NP; ++u) {
-        if (u * TL_WG >= count) break;
-        raw[u] = load_piece<FMT>(z + head + 8 * min(u * TL_WG + (int)threadIdx.x, count - 1), 8, 0.f);
+        if (u * WG >= count) break;
+        raw[u] = load_piece<FMT>(z + head + 8 * min(u * WG + (int)threadIdx.x, count - 1), 8, 0.f);
       }
+    } else if constexpr (NP == 1) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) one[i] = z[min(i * WG + (int)threadIdx.x, len - 1)];
     }
   }
-  // fn(8 values, column of the first): the thread's pieces; what lies outside the row is -inf
+  // fn(8 values, column of the first, columns from one to the next), by whole waves; what lies outside the row is -inf
   template <typename Fn> __device__ __forceinline__ void each(Fn fn) const {
     float v[8];
-    if constexpr (NP > 0) {
+    if constexpr (NP == 1) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = i * WG + (int)threadIdx.x < len ? elem_to_f32<FMT>(one[i]) : -INFINITY;
+      fn(v, (int)threadIdx.x, WG);
+      return;
+    }
+    if constexpr (NP > 1) {
 #pragma unroll
       for (int u = 0; u < NP; ++u) {
-        if (u * TL_WG >= count) break;
+        if (u * WG >= count) break;
         unpack_piece<FMT>(raw[u], v);
-        const int p = u * TL_WG + (int)threadIdx.x;
-        if ((u + 1) * TL_WG > count) {
+        const int p = u * WG + (int)threadIdx.x;
+        if ((u + 1) * WG > count) {
 #pragma unroll
           for (int i = 0; i < 8; ++i) v[i] = p < count ? v[i] : -INFINITY;
         }
-        fn(v, head + 8 * p);
+        fn(v, head + 8 * p, 1);
       }
     } else {
-      for (int p0 = 0; p0 < count; p0 += TL_WG) {          // (whole waves)
+      for (int p0 = 0; p0 < count; p0 += WG) {
         const int p = p0 + (int)threadIdx.x;
         unpack_piece<FMT>(load_piece<FMT>(z + head + (size_t)8 * min(p, count - 1), 8, 0.f), v);
-        if (p0 + TL_WG > count) {
+        if (p0 + WG > count) {
 #pragma unroll
           for (int i = 0; i < 8; ++i) v[i] = p < count ? v[i] : -INFINITY;
         }
-        fn(v, head + 8 * p);
+        fn(v, head + 8 * p, 1);
       }
     }
     if (threadIdx.x < 64 && head + tailn) {          // the ends: lanes 0 and 1
       const int first = threadIdx.x == 0 ? 0 : len - tailn, n = threadIdx.x == 0 ? head : threadIdx.x == 1 ? tailn : 0;
       unpack_piece<FMT>(load_piece<FMT>(z + first, n, -INFINITY), v);
-      fn(v, first);
+      fn(v, first, 1);
     }
   }
   // fn(inside, value, column): single elements, threads in turn, by whole waves
   template <typename Fn> __device__ __forceinline__ void each_element(Fn fn) const {
-    for (int64_t j0 = 0; j0 < len; j0 += TL_WG) {
+    for (int64_t j0 = 0; j0 < len; j0 += WG) {
       const int64_t j = j0 + threadIdx.x;
       fn(j < len, elem_to_f32<FMT>(z[min(j, (int64_t)len - 1)]), (int)j);
     }
@@ -248,50 +294,48 @@ template <int FMT, int NP> struct RowPieces {
 };
 
 // log sum exp(z / tau) over the elements whose pair lies under `kth`, by their maximum; every thread gets it
-template <int FMT, int NP> __device__ __forceinline__ float rest_below(const RowPieces<FMT, NP>& row, uint64_t kth, float c, float inv_tau, float* red) {
+template <int FMT, int WG, int NP> __device__ __forceinline__ float rest_below(const RowPieces<FMT, WG, NP>& row, uint64_t kth, float c, float inv_tau, float* red) {
   float rmx = -INFINITY, bad = 0.f;
   row.each_element([&](bool in, float v, int j) { if (in && pair_of(v, j) < kth) { rmx = fmaxf(rmx, v); if (v != v) bad = 1.f; } });
-  rmx = block_max<TL_WAVES>(rmx, red);
-  if (block_max<TL_WAVES>(bad, red) > 0.f) return NOT_A_NUMBER;
+  rmx = block_max<WG / 64>(rmx, red);
+  if (block_max<WG / 64>(bad, red) > 0.f) return NOT_A_NUMBER;
   if (!(fabsf(rmx) < INFINITY)) return rmx;
   float s = 0.f;
   row.each_element([&](bool in, float v, int j) { if (in && pair_of(v, j) < kth) s += __builtin_amdgcn_exp2f((v - rmx) * c); });
-  return fmaf(rmx, inv_tau, __builtin_amdgcn_logf(block_sum<TL_WAVES>(s, red)) * LN2);
+  return fmaf(rmx, inv_tau, __builtin_amdgcn_logf(block_sum<WG / 64>(s, red)) * LN2);
 }
 
 // One workgroup per row or piece, two looks at it: a bound that at least k elements reach, from every thread's maximum; then the few elements
 // that reach the bound (a few times k) and the sum of exp over all others.  Rows whose bound collects too much or is not finite (fewer than about k
 // finite elements), or that hold NaN, take the exact way: the k-th pair by radix search.
-template <int FMT, int NP> __global__ void __launch_bounds__(TL_WG) top_logits_kernel(rumpy_top_logits_args a, TlPlan plan) {
+template <int FMT, int WG, int NP> __global__ void __launch_bounds__(WG) top_logits_kernel(rumpy_top_logits_args a, TlPlan plan) {
   typedef typename RowElem<FMT>::type E;
-  __shared__ TlShared sh;
+  __shared__ TlShared<WG> sh;
   const int tid = threadIdx.x;
   const float c = a.inv_tau * LOG2E;
   const int64_t row = blockIdx.x / plan.splits;
   const int piece = blockIdx.x % plan.splits, c0 = piece * plan.seg;
-  RowPieces<FMT, NP> r(reinterpret_cast<const E*>(a.logits) + (size_t)row * a.ld + c0, min(plan.seg, a.V - c0));
+  RowPieces<FMT, WG, NP> r(reinterpret_cast<const E*>(a.logits) + (size_t)row * a.ld + c0, min(plan.seg, a.V - c0));
   r.load();
   const int len = r.len, k = min(a.k, len);
   uint32_t n, mine = 0;                                   // candidates of the row, of the wave
   float T = 0.f, sum = 0.f;
   bool exact_way = false;
-  if (len <= TL_WG) {                                     // one element per thread: all of them are candidates
-    push(tid < len, pair_of(elem_to_f32<FMT>(r.z[min(tid, len - 1)]), tid), mine, sh);
+  if (NP == 1 && len <= WG) {                             // one element per thread: all of them are candidates
+    push(tid < len, pair_of(elem_to_f32<FMT>(r.one[0]), tid), mine, sh);
     n = lists_done(mine, sh);
   } else {
-    // single elements instead of pieces where pieces would leave threads without any
-    const bool pieces = r.count >= TL_WG;
     float mx = -INFINITY;                                 // (NaN is passed over here; the second look meets it)
-    if (pieces) r.each([&](const float (&v)[8], int) {
+    r.each([&](const float (&v)[8], int, int) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) mx = fmaxf(mx, v[i]);
     });
-    else r.each_element([&](bool in, float v, int) { mx = fmaxf(mx, in ? v : -INFINITY); });
-    T = key_value(bound_of(order_key(mx), (k + TL_WAVES - 1) / TL_WAVES, sh));
+    constexpr int LOW = FMT == RUMPY_FMT_BF16 ? 16 : 0;
+    T = key_value(bound_of<WG, LOW>(order_key(mx), (k + WG / 64 - 1) / (WG / 64), sh));
     const float m = T * c;
     exact_way = !(fabsf(m) < INFINITY && fabsf(T) < INFINITY);
     if (!exact_way) {
-      if (pieces) r.each([&](const float (&v)[8], int j) {
+      r.each([&](const float (&v)[8], int j, int stride) {
         bool any = false;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
@@ -301,17 +345,12 @@ template <int FMT, int NP> __global__ void __launch_bounds__(TL_WG) top_logits_k
         }
         if (__ballot(any)) {
 #pragma unroll
-          for (int i = 0; i < 8; ++i) push(v[i] >= T, pair_of(v[i], j + i), mine, sh);
+          for (int i = 0; i < 8; ++i) push(v[i] >= T, pair_of(v[i], j + i * stride), mine, sh);
         }
       });
-      else r.each_element([&](bool in, float v, int j) {
-        const bool hit = in && v >= T;
-        push(hit, pair_of(v, j), mine, sh);
-        sum += __builtin_amdgcn_exp2f(fmaf(hit || !in ? -INFINITY : v, c, -m));
-      });
-      sum = block_sum<TL_WAVES>(sum, sh.red);
+      sum = block_sum<WG / 64>(sum, sh.red);
       n = lists_done(mine, sh);
-      exact_way = n > TL_CAP || sum != sum;
+      exact_way = n == ~0u || sum != sum;
     }
   }
   if (exact_way) {
@@ -329,22 +368,19 @@ template <int FMT, int NP> __global__ void __launch_bounds__(TL_WG) top_logits_k
       reinterpret_cast<int64_t*>(a.indices)[(size_t)row * a.k + at] = col;
     }
   });
-  if (pairs && tid >= k && tid < a.k) pairs[tid] = 0;       // a piece shorter than k
+  if (pairs) for (int i = k + tid; i < a.k; i += WG) pairs[i] = 0;       // a piece shorter than k
   float tail;
   if (n == (uint32_t)len && sh.next == 0) tail = -INFINITY;      // everything is chosen
   else if (sh.next == 0 && (exact_way || sum < 1e-20f)) {
     // nothing collected beyond the top, and the others lie so far under the bound that their sum has no digits left (or was not made)
-    tail = rest_below<FMT, NP>(r, sh.kth, c, a.inv_tau, sh.red);
+    tail = rest_below(r, sh.kth, c, a.inv_tau, sh.red);
   } else {
     const float next = sh.next ? pair_value(sh.next) : T;
-    if (!(fabsf(next) < INFINITY)) tail = next;
-    else {
-      // relative to the largest that was not chosen: the other candidates, and the sum under the bound with T's distance from it
-      float s = 0.f;
-      for (uint32_t i = k + tid; i < n; i += TL_WG) s += __builtin_amdgcn_exp2f((sh.after[i] - next) * c);
-      s = block_sum<TL_WAVES>(s, sh.red) + (sum > 0.f ? sum * __builtin_amdgcn_exp2f((T - next) * c) : 0.f);
-      tail = fmaf(next, a.inv_tau, __builtin_amdgcn_logf(s) * LN2);
-    }
+    // relative to the largest that was not chosen: the other candidates, and the sum under the bound with T's distance from it
+    float s = 0.f;
+    for (uint32_t i = k + tid; i < n; i += WG) s += __builtin_amdgcn_exp2f((sh.after[i] - next) * c);
+    s = block_sum<WG / 64>(s, sh.red) + (sum > 0.f ? sum * __builtin_amdgcn_exp2f((T - next) * c) : 0.f);
+    tail = fabsf(next) < INFINITY ? fmaf(next, a.inv_tau, __builtin_amdgcn_logf(s) * LN2) : next;
   }
   if (tid == 0) {
     if (pairs) reinterpret_cast<float*>((uint64_t*)a.work + (size_t)gridDim.x * a.k)[blockIdx.x] = tail;
@@ -352,15 +388,24 @@ template <int FMT, int NP> __global__ void __launch_bounds__(TL_WG) top_logits_k
   }
 }
 
-// the pieces' pairs (each list in order) to the row's k, by the same two steps; what is left of them joins the pieces' tails
-template <int FMT> __global__ void __launch_bounds__(TL_WG) top_join_kernel(rumpy_top_logits_args a, TlPlan plan) {
+// the pieces' pairs (each list in order) to the row's k, by the same two steps; what is left of them joins the pieces' tails.  All pairs are in
+// registers; consecutive threads take the same place of consecutive lists, so that what is collected spreads over the waves.
+template <int FMT> __global__ void __launch_bounds__(512) top_join_kernel(rumpy_top_logits_args a, TlPlan plan) {
   typedef typename RowElem<FMT>::type E;
-  __shared__ TlShared sh;
+  constexpr int WG = 512, NP = TL_MOST_SPLITS * DS_MAXK / WG;
+  __shared__ TlShared<WG> sh;
   const int tid = threadIdx.x, k = a.k, S = plan.splits, count = S * k;
   const int64_t row = blockIdx.x;
   const E* z = reinterpret_cast<const E*>(a.logits) + (size_t)row * a.ld;
   const uint64_t* pairs = (const uint64_t*)a.work + (size_t)row * count;
   const float* tails = reinterpret_cast<const float*>((const uint64_t*)a.work + (size_t)gridDim.x * count) + (size_t)row * S;
+  uint64_t mine[NP];
+#pragma unroll
+  for (int u = 0; u < NP; ++u) {
+    const int j = u * WG + tid;
+    mine[u] = j < count ? pairs[(j % S) * k + j / S] : 0;
+  }
+  const float tail_in = tid < S ? tails[tid] : -INFINITY;
   // the bound: of every list the pair that ceil(k / lists) of its pairs reach, the smallest of them
   if (tid == 0) sh.prefix = ~0ull;
   __syncthreads();
@@ -368,16 +413,13 @@ template <int FMT> __global__ void __launch_bounds__(TL_WG) top_join_kernel(rump
   __syncthreads();
   const uint64_t bound = sh.prefix;
   auto gather = [&](uint64_t from) {
-    uint32_t mine = 0;
-    for (int j0 = 0; j0 < count; j0 += TL_WG) {
-      const int j = j0 + tid;
-      const uint64_t p = j < count ? pairs[j] : 0;
-      push(p && p >= from, p, mine, sh);
-    }
-    return lists_done(mine, sh);
+    uint32_t listed = 0;
+#pragma unroll
+    for (int u = 0; u < NP; ++u) push(mine[u] && mine[u] >= from, mine[u], listed, sh);
+    return lists_done(listed, sh);
   };
   uint32_t n = gather(bound);
-  if (n > TL_CAP || n < (uint32_t)k) {                   // (fewer than k: the last list is short)
+  if (n == ~0u || n < (uint32_t)k) {                   // (fewer than k: the last list is short)
     const uint64_t kth = radix_kth([&](int64_t j) { return pairs[j]; }, count, k, sh);
     n = gather(kth);
   }
@@ -387,24 +429,23 @@ template <int FMT> __global__ void __launch_bounds__(TL_WG) top_join_kernel(rump
     reinterpret_cast<int64_t*>(a.indices)[(size_t)row * k + at] = col;
   });
   const uint64_t kth = sh.kth;
-  float m = -INFINITY, bad = 0.f;
-  for (int j = tid; j < count + S; j += TL_WG) {
-    const uint64_t p = j < count ? pairs[j] : 0;
-    if (j < count && (p >= kth || !p)) continue;
-    const float u = j < count ? pair_value(p) * a.inv_tau : tails[j - count];
-    m = fmaxf(m, u);
-    if (u != u) bad = 1.f;
+  float m = tail_in, bad = tail_in != tail_in ? 1.f : 0.f;
+#pragma unroll
+  for (int u = 0; u < NP; ++u) {
+    if (mine[u] && mine[u] < kth) {
+      const float v = pair_value(mine[u]) * a.inv_tau;
+      m = fmaxf(m, v);
+      if (v != v) bad = 1.f;
+    }
   }
-  m = block_max<TL_WAVES>(m, sh.red);
-  bad = block_max<TL_WAVES>(bad, sh.red);
-  float s = 0.f;
-  for (int j = tid; j < count + S; j += TL_WG) {
-    const uint64_t p = j < count ? pairs[j] : 0;
-    if (j < count && (p >= kth || !p)) continue;
-    const float u = j < count ? pair_value(p) * a.inv_tau : tails[j - count];
-    s += __builtin_amdgcn_exp2f((u - m) * LOG2E);
+  m = block_max<WG / 64>(m, sh.red);
+  bad = block_max<WG / 64>(bad, sh.red);
+  float s = __builtin_amdgcn_exp2f((tail_in - m) * LOG2E);
+#pragma unroll
+  for (int u = 0; u < NP; ++u) {
+    if (mine[u] && mine[u] < kth) s += __builtin_amdgcn_exp2f((pair_value(mine[u]) * a.inv_tau - m) * LOG2E);
   }
-  s = block_sum<TL_WAVES>(s, sh.red);
+  s = block_sum<WG / 64>(s, sh.red);
   if (tid == 0) a.tail[row] = bad > 0.f ? NOT_A_NUMBER : fabsf(m) < INFINITY ? m + __builtin_amdgcn_logf(s) * LN2 : m;
 }
 
@@ -413,17 +454,25 @@ extern "C" int64_t rumpy_top_logits_work_bytes(int64_t rows, int32_t V, int32_t 
   const TlPlan plan = tl_plan(rows, V);
   return plan.splits > 1 ? rows * plan.splits * (k * 8 + 4) : 0;
 }
+template <int FMT, int WG> static void tl_launch_wg(const rumpy_top_logits_args& a, const TlPlan& plan, hipStream_t s) {
+  const dim3 grid((unsigned)(a.rows * plan.splits)), wg(WG);
+  const int len = a.V < plan.seg ? a.V : plan.seg, np = (len / 8 + WG - 1) / WG;
+  constexpr int MOST = WG == 128 ? 4 : WG == 256 || FMT == RUMPY_FMT_F32 ? 8 : 16;          // pieces in registers (the callers' limits; 64 registers)
+  if (len <= 8 * WG) hipLaunchKernelGGL((top_logits_kernel<FMT, WG, 1>), grid, wg, 0, s, a, plan);
+  else if (np <= 2) hipLaunchKernelGGL((top_logits_kernel<FMT, WG, 2>), grid, wg, 0, s, a, plan);
+  else if (np <= 4) hipLaunchKernelGGL((top_logits_kernel<FMT, WG, 4>), grid, wg, 0, s, a, plan);
+  else if (np <= 8 && MOST >= 8) hipLaunchKernelGGL((top_logits_kernel<FMT, WG, MOST >= 8 ? 8 : 1>), grid, wg, 0, s, a, plan);
+  else if (np <= MOST) hipLaunchKernelGGL((top_logits_kernel<FMT, WG, MOST>), grid, wg, 0, s, a, plan);
+  else if constexpr (WG == 512) hipLaunchKernelGGL((top_logits_kernel<FMT, WG, 0>), grid, wg, 0, s, a, plan);
+}
 template <int FMT> static void tl_launch(const rumpy_top_logits_args& a, const TlPlan& plan, hipStream_t s) {
-  // pieces a thread holds: 64 registers' worth at most
-  const dim3 grid((unsigned)(a.rows * plan.splits)), wg(TL_WG);
-  const int np = (plan.seg / 8 + TL_WG - 1) / TL_WG, len = a.V < plan.seg ? a.V : plan.seg;
-  constexpr int MOST = FMT == RUMPY_FMT_F32 ? 8 : 16;
-  if (len < TL_WG * 8 || np > MOST) hipLaunchKernelGGL((top_logits_kernel<FMT, 0>), grid, wg, 0, s, a, plan);
-  else if (np <= 2) hipLaunchKernelGGL((top_logits_kernel<FMT, 2>), grid, wg, 0, s, a, plan);
-  else if (np <= 4) hipLaunchKernelGGL((top_logits_kernel<FMT, 4>), grid, wg, 0, s, a, plan);
-  else if (np <= 8) hipLaunchKernelGGL((top_logits_kernel<FMT, 8>), grid, wg, 0, s, a, plan);
-  else hipLaunchKernelGGL((top_logits_kernel<FMT, MOST>), grid, wg, 0, s, a, plan);
-  if (plan.splits > 1) hipLaunchKernelGGL((top_join_kernel<FMT>), dim3((unsigned)a.rows), wg, 0, s, a, plan);
+  // Many short rows: small workgroups, more rows at once (a row is a chain of latencies: bound, lists, places).  At least 2 k threads, so that
+  // the bound comes from the better half of the threads' maxima.
+  const bool many = a.rows * plan.splits >= 1024;
+  if (many && a.V <= 4096 && a.k <= 64) tl_launch_wg<FMT, 128>(a, plan, s);
+  else if (many && a.V <= 16384 && a.k <= 128) tl_launch_wg<FMT, 256>(a, plan, s);
+  else tl_launch_wg<FMT, 512>(a, plan, s);
+  if (plan.splits > 1) hipLaunchKernelGGL((top_join_kernel<FMT>), dim3((unsigned)a.rows), dim3(512), 0, s, a, plan);
 }
 extern "C" int rumpy_top_logits(const rumpy_top_logits_args* p, void* stream) {
   const char* bad = !p ? "no arguments" : nullptr;
@@ -599,7 +648,7 @@ template <int FMT, bool REST> __global__ void __launch_bounds__(DS_WG) distill_f
   }
   const int64_t j0 = (int64_t)piece * plan.seg, j1 = min((int64_t)a.V, j0 + plan.seg);
   // whole pieces lie at 16-byte addresses (RowPieces); their bits at whole bytes: column j of the piece of the row has bit j - j0 + shift
-  const RowPieces<FMT, 0> r(z + j0, (int)(j1 - j0));
+  const RowPieces<FMT, DS_WG, 0> r(z + j0, (int)(j1 - j0));
   const int shift = (8 - r.head) & 7, body = r.head ? 1 : 0;
   const uint8_t* bytes = reinterpret_cast<const uint8_t*>(bits);
   // U pieces are asked for before the U before them are summed (the first before anything else); their maximum is joined once
