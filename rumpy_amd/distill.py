@@ -8,11 +8,12 @@ vocabulary of any size.  With u = z / T, q = softmax(u) and p the teacher's dist
     l = T^2 [ sum_i p_i (log p_i - log q_i)  +  p_t (log p_t - log q_t) ]
 
 over the listed columns i and, when the teacher's ``tail`` is given, the unlisted columns together as one more outcome t.  No CPU path."""
+import functools
+
 import torch
-from torch.autograd.function import once_differentiable
 
 from rumpy_amd import _lib as L
-from .residual_norm import _FMT, _launch, _p, _rows
+from .residual_norm import _FMT, _launch, _new_like, _once_differentiable, _p, _rows
 
 MAX_TOP = 256
 MAX_COLUMNS = 1 << 30
@@ -53,11 +54,21 @@ def top_logits(logits, k, temperature=1.0):
         return values, indices, tail
     z, ld = _rows(logits)
     rows = logits.numel() // v
-    wb = int(L.lib().rumpy_top_logits_work_bytes(rows, v, k))
+    wb = _work_bytes(rows, v, k)
     work = torch.empty(wb, dtype=torch.uint8, device=logits.device) if wb else None
     _launch('rumpy_top_logits', L.TopLogitsArgs(logits=z.data_ptr(), values=values.data_ptr(), indices=indices.data_ptr(), tail=tail.data_ptr(), work=_p(work),
                                                 rows=rows, ld=ld, V=v, k=k, fmt=_FMT[logits.dtype], inv_tau=1.0 / t), logits.device)
     return values, indices, tail
+
+
+@functools.lru_cache(maxsize=512)
+def _work_bytes(rows, v, k):
+    return int(L.lib().rumpy_top_logits_work_bytes(rows, v, k))
+
+
+@functools.lru_cache(maxsize=512)
+def _partial_floats(rows, v):
+    return int(L.lib().rumpy_distill_partial_floats(rows, v))
 
 
 class _DistillFn(torch.autograd.Function):
@@ -66,37 +77,36 @@ class _DistillFn(torch.autograd.Function):
         dev, v = logits.device, logits.shape[-1]
         rows, k = logits.numel() // v, values.shape[-1]
         z, ld = _rows(logits)
-        row_loss = torch.empty(logits.shape[:-1], dtype=torch.float32, device=dev)
-        state = torch.empty(rows * 8 + 1, dtype=torch.float32, device=dev)
-        loss = torch.empty((), dtype=torch.float32, device=dev) if reduction != 'none' else None
-        pf = int(L.lib().rumpy_distill_partial_floats(rows, v))
-        partial = torch.empty(pf, dtype=torch.float32, device=dev) if pf else None
-        args = L.DistillArgs(logits=z.data_ptr(), top_values=values.data_ptr(), top_indices=indices.data_ptr(), tail=_p(tail), row_weight=_p(row_weight),
-                             row_loss=row_loss.data_ptr(), state=state.data_ptr(), loss=_p(loss), factor=state.data_ptr() + 32 * rows, partial=_p(partial),
-                             rows=rows, ld=ld, V=v, k=k, fmt=_FMT[z.dtype], value_fmt=_FMT[values.dtype], index64=1 if indices.dtype == torch.int64 else 0,
-                             mean=1 if reduction == 'mean' else 0, tau=temperature, inv_tau=1.0 / temperature)
-        _launch('rumpy_distill_fwd', args, dev)
+        # state [rows, 8], the reduction's factor, the workspace of rows that are cut, the rows' losses
+        pf = _partial_floats(rows, v)
+        none = reduction == 'none'
+        state = torch.empty(rows * 9 + 1 + pf, dtype=torch.float32, device=dev)
+        loss = torch.empty(logits.shape[:-1] if none else (), dtype=torch.float32, device=dev)
+        at = state.data_ptr()
+        _launch('rumpy_distill_fwd', L.DistillArgs(
+            logits=z.data_ptr(), top_values=values.data_ptr(), top_indices=indices.data_ptr(), tail=_p(tail), row_weight=_p(row_weight),
+            row_loss=loss.data_ptr() if none else at + 4 * (8 * rows + 1 + pf), state=at, loss=None if none else loss.data_ptr(), factor=at + 32 * rows,
+            partial=at + 32 * rows + 4 if pf else None, rows=rows, ld=ld, V=v, k=k, fmt=_FMT[z.dtype], value_fmt=_FMT[values.dtype],
+            index64=1 if indices.dtype == torch.int64 else 0, mean=1 if reduction == 'mean' else 0, tau=temperature, inv_tau=1.0 / temperature), dev)
         ctx.reduction, ctx.temperature = reduction, temperature
         ctx.save_for_backward(logits, values, indices, tail, row_weight, state)
-        return row_loss if loss is None else loss
+        return loss
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, g):
+        _once_differentiable('distill_loss')
         logits, values, indices, tail, row_weight, state = ctx.saved_tensors
         dev, v = logits.device, logits.shape[-1]
         rows, k = logits.numel() // v, values.shape[-1]
         z, ld = _rows(logits)
         g = g.contiguous()
-        dl = torch.empty(logits.shape, dtype=logits.dtype, device=dev)
+        dl = _new_like(logits)
         if rows:
-            pf = int(L.lib().rumpy_distill_partial_floats(rows, v))
-            partial = torch.empty(pf, dtype=torch.float32, device=dev) if pf else None
-            # `loss` only says that g is the gradient of one number; nothing is written there
+            # (`loss` only says that g is the gradient of one number; nothing but dlogits is written)
             _launch('rumpy_distill_bwd', L.DistillArgs(
                 logits=z.data_ptr(), top_values=values.data_ptr(), top_indices=indices.data_ptr(), tail=_p(tail), row_weight=_p(row_weight),
                 row_loss=g.data_ptr(), state=state.data_ptr(), loss=None if ctx.reduction == 'none' else g.data_ptr(), factor=state.data_ptr() + 32 * rows,
-                partial=_p(partial), gout=g.data_ptr(), dlogits=dl.data_ptr(), rows=rows, ld=ld, V=v, k=k, fmt=_FMT[z.dtype], value_fmt=_FMT[values.dtype],
+                partial=state.data_ptr(), gout=g.data_ptr(), dlogits=dl.data_ptr(), rows=rows, ld=ld, V=v, k=k, fmt=_FMT[z.dtype], value_fmt=_FMT[values.dtype],
                 index64=1 if indices.dtype == torch.int64 else 0, mean=1 if ctx.reduction == 'mean' else 0, tau=ctx.temperature,
                 inv_tau=1.0 / ctx.temperature), dev)
         return dl, None, None, None, None, None, None
@@ -133,4 +143,5 @@ def distill_loss(logits, top_values, top_indices, tail=None, temperature=1.0, ro
             raise ValueError('rumpy_amd: distill_loss takes its tensors on one device, %s, not %s' % (dev, s.device))
     _need_gpu('distill_loss', logits)
     as_f32 = lambda s: None if s is None else s.detach().to(torch.float32).contiguous()
-    return _DistillFn.apply(logits, top_values.detach().contiguous(), top_indices.contiguous(), as_f32(tail), as_f32(row_weight), t, reduction)
+    values = top_values.detach() if top_values.requires_grad else top_values
+    return _DistillFn.apply(logits, values.contiguous(), top_indices.contiguous(), as_f32(tail), as_f32(row_weight), t, reduction)

@@ -9,9 +9,10 @@ pixel or token, before the block, after it, or both - need, between two blocks,
 
 with y the residual stream and h the next block's input.  ``residual_norm`` is that as a function, ``ResidualNorm`` as a module.
 No CPU path: tensors must be on the GPU."""
+import functools
+
 import torch
 from torch import nn
-from torch.autograd.function import once_differentiable
 
 from rumpy_amd import _lib as L
 
@@ -40,13 +41,26 @@ def _rows(t):
     return t.contiguous(), c
 
 
+_raw_stream = torch._C._cuda_getCurrentRawStream          # torch.cuda.current_stream builds a Stream object first: 2 us a call
+
+
 def _launch(name, args, dev):
     """on the current stream of the tensors' own device, whichever device is current"""
     if dev.index == torch.cuda.current_device():
-        L.call(name, args, torch.cuda.current_stream(dev).cuda_stream)
+        L.call(name, args, _raw_stream(dev.index))
     else:
         with torch.cuda.device(dev):
-            L.call(name, args, torch.cuda.current_stream(dev).cuda_stream)
+            L.call(name, args, _raw_stream(dev.index))
+
+
+def _new_like(t):
+    """an uninitialised contiguous tensor of t's shape and type (empty_like is half the price of empty, and keeps strides)"""
+    return torch.empty_like(t) if t.is_contiguous() else torch.empty(t.shape, dtype=t.dtype, device=t.device)
+
+
+@functools.lru_cache(maxsize=512)
+def _partial_floats(rows, group_rows, c, gate_mode):
+    return int(L.lib().rumpy_residual_norm_partial_floats(rows, group_rows, c, gate_mode))
 
 
 def _forward(x, branch, gate, post_w, post_b, pre_w, pre_b, cfg, keep):
@@ -55,8 +69,8 @@ def _forward(x, branch, gate, post_w, post_b, pre_w, pre_b, cfg, keep):
     c = x.shape[-1]
     rows = x.numel() // c
     tb = x if branch is None else branch
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device) if branch is not None else None
-    h = torch.empty(x.shape, dtype=tb.dtype, device=x.device) if pre else None
+    y = _new_like(x) if branch is not None else None
+    h = _new_like(tb) if pre else None
     stats = torch.empty((rows, 4), dtype=torch.float32, device=x.device) if keep else None
     if rows == 0:
         return y, h, stats
@@ -75,6 +89,11 @@ def _forward(x, branch, gate, post_w, post_b, pre_w, pre_b, cfg, keep):
     return y, h, stats
 
 
+def _once_differentiable(name):
+    if torch.is_grad_enabled():             # (only under create_graph=True)
+        raise RuntimeError('rumpy_amd: %s has no second derivative' % name)
+
+
 class _ResidualNormFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, branch, gate, post_w, post_b, pre_w, pre_b, cfg):
@@ -85,8 +104,8 @@ class _ResidualNormFn(torch.autograd.Function):
         return y, h
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dy, dh):
+        _once_differentiable('residual_norm')
         x, branch, gate, post_w, post_b, pre_w, stats = ctx.saved_tensors
         post, pre, gate_mode, group_rows, scale, _ = ctx.cfg
         need = ctx.needs_input_grad
@@ -95,15 +114,17 @@ class _ResidualNormFn(torch.autograd.Function):
         c, dev = x.shape[-1], x.device
         rows = x.numel() // c
         tb = x if branch is None else branch
-        new = torch.zeros if rows == 0 else torch.empty
-        f32 = lambda shape, wanted: new(shape, dtype=torch.float32, device=dev) if wanted else None
-        dx = new(x.shape, dtype=x.dtype, device=dev) if need[0] else None
-        dt = new(branch.shape, dtype=branch.dtype, device=dev) if need[1] else None
-        dgate = new(gate.shape, dtype=gate.dtype, device=dev) if need[2] else None
-        d_post_w, d_post_b = f32(c, need[3]), f32(c, need[4])
-        d_pre_w, d_pre_b = f32(c, need[5]), f32(c, need[6])
-        if dh is None:              # nothing arrived through the norm in front: its parameters have no gradient
-            d_pre_w = d_pre_b = None
+        dx = _new_like(x) if need[0] else None
+        dt = _new_like(branch) if need[1] else None
+        dgate = torch.empty(gate.shape, dtype=gate.dtype, device=dev) if need[2] else None
+        # (where nothing arrives through the norm in front, its parameters have no gradient)
+        wanted = (need[3], need[4], need[5] and dh is not None, need[6] and dh is not None)
+        params = torch.empty((4, c), dtype=torch.float32, device=dev).unbind(0) if any(wanted) else (None,) * 4
+        d_post_w, d_post_b, d_pre_w, d_pre_b = (p if w else None for p, w in zip(params, wanted))
+        if rows == 0:
+            for t in (dgate, d_post_w, d_post_b, d_pre_w, d_pre_b):
+                if t is not None:
+                    t.zero_()
         if rows:
             x, ldx = _rows(x)
             ldt = ldg = lddy = lddh = 0
@@ -117,7 +138,7 @@ class _ResidualNormFn(torch.autograd.Function):
                 dy, lddy = _rows(dy)
             if dh is not None:
                 dh, lddh = _rows(dh)
-            partial = torch.empty(int(L.lib().rumpy_residual_norm_partial_floats(rows, group_rows, c, gate_mode)), dtype=torch.float32, device=dev)
+            partial = torch.empty(_partial_floats(rows, group_rows, c, gate_mode), dtype=torch.float32, device=dev)
             _launch('rumpy_residual_norm_bwd', L.ResidualNormBwdArgs(
                 dy=_p(dy), dh=_p(dh), x=x.data_ptr(), t=_p(branch), gate=_p(gate), post_w=_p(post_w), post_b=_p(post_b), pre_w=_p(pre_w),
                 stats=stats.data_ptr(), dx=_p(dx), dt=_p(dt), dgate=_p(dgate), d_post_w=_p(d_post_w), d_post_b=_p(d_post_b), d_pre_w=_p(d_pre_w),
@@ -131,7 +152,7 @@ def _param(p, name, norm, c, dev):
         return None
     if norm is None:
         raise ValueError('rumpy_amd: residual_norm has %s but no norm it belongs to' % name)
-    if tuple(p.shape) != (c,) or p.dtype != torch.float32 or p.device != dev:
+    if p.shape != (c,) or p.dtype != torch.float32 or p.device != dev:
         raise ValueError('rumpy_amd: residual_norm takes %s as float32 [%d] beside its input, not %s %s' % (name, c, p.dtype, tuple(p.shape)))
     return p if p.is_contiguous() else p.contiguous()
 

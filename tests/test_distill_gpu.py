@@ -437,3 +437,10 @@ def test_teacher_against_itself_costs_nothing():
     grad, = torch.autograd.grad(loss, leaf)
     err = U24 * (8 * 64 + 64 + 32)          # u spans less than 64 here
     assert abs(float(loss.detach())) <= 0.25 * 3 * err and float(grad.abs().sum()) <= 2 * 0.5 * 3 * err
+
+
+def test_no_second_derivative():
+    z = torch.randn(3, 64, device=DEV, requires_grad=True)
+    loss = distill_loss(z, *top_logits(z.detach(), 4)[:2])
+    with pytest.raises(RuntimeError, match='second derivative'):
+        torch.autograd.grad(loss, z, create_graph=True)

@@ -422,3 +422,10 @@ def test_backward_twice_of_one_forward():
                          pre_norm='rms', pre_weight=leaf['pre_weight'], pre_bias=leaf['pre_bias'])
     grads = [torch.autograd.grad([y, h], list(leaf.values()), [dy.to(DEV), dh.to(DEV)], retain_graph=True) for _ in range(2)]
     assert all(torch.equal(a, b) for a, b in zip(*grads))
+
+
+def test_no_second_derivative():
+    x, t = (torch.randn(3, 64, device=DEV, requires_grad=True) for _ in range(2))
+    y, h = residual_norm(x, t, post_norm='rms', pre_norm='rms')
+    with pytest.raises(RuntimeError, match='second derivative'):
+        torch.autograd.grad(y.sum() + h.sum(), [x, t], create_graph=True)
