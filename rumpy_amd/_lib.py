@@ -479,3 +479,24 @@ def check(rc, what=''):
 def call(name, args, stream):
     """Invoke ``int name(const args*, stream)``."""
     check(getattr(lib(), name)(C.byref(args), stream), name)
+
+
+OPS = None          # rumpy_amd._torch_bind, once ops() has bound it
+_BOUND = ('rumpy_residual_norm_fwd', 'rumpy_residual_norm_bwd', 'rumpy_residual_norm_partial_floats', 'rumpy_top_logits', 'rumpy_top_logits_work_bytes',
+          'rumpy_distill_fwd', 'rumpy_distill_bwd', 'rumpy_distill_partial_floats', 'rumpy_last_error')
+
+
+def ops():
+    """The torch binding of the row operators (csrc/torch_bind.cpp -> rumpy_amd/_torch_bind.so) on the loaded kernel library; raises loudly if
+    either is not built."""
+    global OPS
+    if OPS is None:
+        h = lib()
+        try:
+            from rumpy_amd import _torch_bind
+        except ImportError as e:
+            raise RuntimeError('rumpy_amd: the torch binding (%s) cannot be loaded: %s - build it with `python -c "import __graft_entry__ as g; g.build()"` '
+                               '(or make -C rumpy_amd/csrc). There is no fallback.' % (os.path.join(_HERE, '_torch_bind.so'), e))
+        _torch_bind.bind({name: C.cast(getattr(h, name), c_void_p).value for name in _BOUND})
+        OPS = _torch_bind
+    return OPS

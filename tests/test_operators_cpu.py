@@ -166,3 +166,17 @@ def _t(*shape, dtype=torch.float32):
 def test_python_refusals(call, error, text):
     with pytest.raises(error, match=re.escape(text)):
         call()
+
+
+def test_binding_is_loaded_once_and_missing_parts_are_loud(monkeypatch):
+    _lib_or_skip()
+    assert L.ops() is L.ops() is L.OPS
+    for name in L._BOUND:
+        assert name in L.SYMBOLS
+    import sys
+    import rumpy_amd
+    monkeypatch.setattr(L, 'OPS', None)
+    monkeypatch.delattr(rumpy_amd, '_torch_bind')
+    monkeypatch.setitem(sys.modules, 'rumpy_amd._torch_bind', None)         # as if it were not built
+    with pytest.raises(RuntimeError, match='no fallback'):
+        residual_norm(torch.zeros(2, 8), pre_norm='rms')

@@ -8,7 +8,7 @@ cd "$root/rumpy_amd/csrc"
 src=$1; tag=$2; shift 2
 make -s -j6
 d="$root/build_abl/$tag"; mkdir -p "$d"
-nopacked=""; case "$src" in conv_rcab*.hip) nopacked="-Xclang -target-feature -Xclang -packed-fp32-ops";; esac
+nopacked=""; case "$src" in conv_rcab*.hip|residual_norm.hip|distill.hip) nopacked="-Xclang -target-feature -Xclang -packed-fp32-ops";; esac
 /opt/rocm/bin/hipcc -O3 -std=c++17 -fPIC --offload-arch=gfx950 $nopacked "$@" -c "$src" -o "$d/var.o"
 objs=$(ls *.o | grep -v "^${src%.hip}.o$")
 /opt/rocm/bin/hipcc --offload-arch=gfx950 -shared -fPIC -o "$d/librumpy_amd.so" $objs "$d/var.o"
