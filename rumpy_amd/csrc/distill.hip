@@ -330,7 +330,7 @@ template <int FMT, int WG, int NP> __global__ void __launch_bounds__(WG) top_log
 #pragma unroll
       for (int i = 0; i < 8; ++i) mx = fmaxf(mx, v[i]);
     });
-    constexpr int LOW = FMT == RUMPY_FMT_BF16 ? 16 : 0;
+    constexpr int LOW = FMT == RUMPY_FMT_BF16 ? 16 : FMT == RUMPY_FMT_F16 ? 13 : 0;
     T = key_value(bound_of<WG, LOW>(order_key(mx), (k + WG / 64 - 1) / (WG / 64), sh));
     const float m = T * c;
     exact_way = !(fabsf(m) < INFINITY && fabsf(T) < INFINITY);
@@ -775,12 +775,23 @@ template <int FMT> __global__ void __launch_bounds__(DS_WG) distill_join_kernel(
 }
 
 // loss = sum of the rows' (weighted) losses, over the sum of the weights for the mean; a sum of weights of zero gives 0
-__global__ void __launch_bounds__(DS_WG) distill_total_kernel(rumpy_distill_args a) {
-  __shared__ float red[DS_WAVES];
+// (one workgroup: 8 rows a thread are asked for together)
+__global__ void __launch_bounds__(1024) distill_total_kernel(rumpy_distill_args a) {
+  __shared__ float red[16];
   float s = 0.f, w = 0.f;
-  for (int64_t r = threadIdx.x; r < a.rows; r += DS_WG) { s += a.row_loss[r]; w += a.row_weight ? a.row_weight[r] : 1.f; }
-  s = block_sum<DS_WAVES>(s, red);
-  w = block_sum<DS_WAVES>(w, red);
+  for (int64_t r0 = threadIdx.x; r0 < a.rows; r0 += 8 * 1024) {
+    float l[8], wr[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int64_t r = r0 + i * 1024;
+      l[i] = r < a.rows ? a.row_loss[r] : 0.f;
+      wr[i] = r >= a.rows ? 0.f : a.row_weight ? a.row_weight[r] : 1.f;
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) { s += l[i]; w += wr[i]; }
+  }
+  s = block_sum<16>(s, red);
+  w = block_sum<16>(w, red);
   if (threadIdx.x == 0) {
     const float f = !a.mean ? 1.f : w == 0.f ? 0.f : 1.f / w;
     *a.factor = f;
@@ -876,7 +887,7 @@ extern "C" int rumpy_distill_fwd(const rumpy_distill_args* p, void* stream) {
     else if (p->fmt == RUMPY_FMT_BF16) ds_launch_fwd<RUMPY_FMT_BF16>(*p, plan, s);
     else ds_launch_fwd<RUMPY_FMT_F16>(*p, plan, s);
   }
-  if (p->loss) hipLaunchKernelGGL(distill_total_kernel, dim3(1), dim3(DS_WG), 0, s, *p);
+  if (p->loss) hipLaunchKernelGGL(distill_total_kernel, dim3(1), dim3(1024), 0, s, *p);
   return rumpy_check_launch("rumpy_distill_fwd");
 }
 extern "C" int rumpy_distill_bwd(const rumpy_distill_args* p, void* stream) {

@@ -192,6 +192,20 @@ def moco_logits(q, k, queue, temperature, positives, labels=None, queue_labels=N
     return _NormLogitsFn.apply(q, v, qc, 1.0 / temperature)
 
 
+@torch.no_grad()
+def teacher_top(k, queue, temperature, top):
+    """the momentum teacher's side of distillation: the ``top`` largest similarities of each normalised key k [N, C] to the queue [C, K], divided by
+    the temperature -> (values, indices, tail) as rumpy_amd.distill.distill_loss takes them (at temperature 1)"""
+    from rumpy_amd.distill import top_logits
+    _need_gpu(k, queue)
+    k = k.detach().contiguous().float()
+    n, c = k.shape
+    kq = queue.shape[1]
+    logits = torch.empty(n, kq, dtype=torch.float32, device=k.device)
+    sgemm(k, queue, logits, n, kq, c, c, 1, kq, 1, kq, alpha=1.0 / temperature)
+    return top_logits(logits, top)
+
+
 class _CrossEntropyFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, target):

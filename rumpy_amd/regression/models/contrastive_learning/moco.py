@@ -16,15 +16,17 @@ import torch.nn as nn
 
 from rumpy_amd import _lib as L
 from .encoding_models import Encoder
-from .head import moco_logits, normalize_rows
+from .head import moco_logits, normalize_rows, teacher_top
 
 
 class MoCo(nn.Module):
     flat_protocol = True             # BaseModel: param_list / offsets / flat_p / flat_g / attach_grads / engine of the trainable part
     supports_fused_l1 = False
 
-    def __init__(self, base_encoder, dim=256, K=32 * 256, m=0.999, T=0.07, mlp=True, positives=1, dropdown=None):
-        """dim: feature dimension; K: queue size (negative keys); m: momentum of the key encoder; T: softmax temperature (:18-24)"""
+    def __init__(self, base_encoder, dim=256, K=32 * 256, m=0.999, T=0.07, mlp=True, positives=1, dropdown=None, distill_top=None, distill_t=0.04):
+        """dim: feature dimension; K: queue size (negative keys); m: momentum of the key encoder; T: softmax temperature (:18-24).
+        distill_top (not in the reference): a training forward also leaves, in ``distill_targets``, the distill_top largest similarities of each
+        query's first key to the queue, at temperature distill_t: the targets of relational distillation from the momentum encoder"""
         super(MoCo, self).__init__()
         if base_encoder is not Encoder:
             raise RuntimeError('rumpy_amd: only the default (DASR) encoder is on the HIP path, not %r' % (getattr(base_encoder, '__name__', base_encoder),))
@@ -32,6 +34,10 @@ class MoCo(nn.Module):
         self.vector_dim = dim
         self.dropdown = dropdown
         self.positives = positives
+        if distill_top is not None and not 1 <= distill_top <= min(K, 256):
+            raise ValueError('rumpy_amd: distill_top is 1 .. 256 of the %d queue entries, not %r' % (K, distill_top))
+        self.distill_top, self.distill_t = distill_top, distill_t
+        self.distill_targets = None
         self.encoder_q = base_encoder(dropdown)
         self.encoder_k = base_encoder(dropdown)
         for param_q, param_k in zip(self.encoder_q.parameters(), self.encoder_k.parameters()):
@@ -183,6 +189,8 @@ class MoCo(nn.Module):
         # against the queue ; all / T (one positive: q . k / T, :150-151,170-172; several: (sum_p q . k_p / T) / positives, :153-158,174-177):
         # normalisation, both products and their backward pass are HIP (head.py)
         logits = moco_logits(heads['q'], k, self.queue, self.T, self.positives)
+        if self.distill_top is not None:                                        # the queue as the logits saw it: before the enqueue
+            self.distill_targets = teacher_top(k[::self.positives], self.queue, self.distill_t, self.distill_top)
         labels = self._zero_labels(n, logits.device)                            # cross-entropy target: column 0
         self._dequeue_and_enqueue(k, stride=self.positives)                     # one key per query joins the queue (:181-184)
         return embedding, logits, labels

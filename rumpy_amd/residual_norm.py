@@ -26,6 +26,7 @@ def residual_norm(x, branch=None, gate=None, scale=1.0, post_norm=None, post_wei
     gate         None; float32 [C] (a learnt scale per channel); float32 [x.shape[0], C] (one gate per image, as CALayer makes it); or
                  [..., C] like the branch, in its type.
     post_norm, pre_norm   None, 'layer' or 'rms', with weight and bias float32 [C] or None.  pre_norm None: h is None.
+    eps          above zero.
     Gradients go to x, branch, gate and the four parameters.  Statistics and sums are float32; y, h and the gradients are rounded once (h is the
     norm of the unrounded y).  Channels that do not lie side by side, or rows at no common stride, are copied first.
     mirrors and joins rumpy/SISR/models/advanced/common.py:71-75 and architectures.py:41-44, 81-84 (``res += x`` around a scaled or gated branch)"""

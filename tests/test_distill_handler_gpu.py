@@ -1,0 +1,167 @@
+"""Distillation on the contrastive path: the momentum teacher's top similarities, a contrastive training step with them, and the operators together
+- a residual stack with its norms, a teacher's selection, the loss and every gradient."""
+import tempfile
+
+import pytest
+import torch
+
+from oracle import contrastive_oracle as CO
+from rumpy_amd.distill import distill_loss, top_logits
+from rumpy_amd.residual_norm import ResidualNorm
+from rumpy_amd.shared_framework.models import define_model
+
+pytestmark = pytest.mark.gpu
+DEV = 'cuda:0'
+U24 = 2.0 ** -24
+
+
+def _unit(t, dim):
+    return torch.nn.functional.normalize(t, dim=dim)
+
+
+@pytest.mark.parametrize('n,positives,top', [(8, 1, 64), (5, 3, 256), (32, 1, 1)])
+def test_teacher_top_and_the_loss_of_the_contrastive_head(n, positives, top):
+    """moco_logits -> distill_loss(logits[:, 1:]) against 64 bits: similarities to the queue on both sides, loss and d loss / d q"""
+    from rumpy_amd.regression.models.contrastive_learning import head as H
+    g = torch.Generator().manual_seed(n)
+    K, C, T, Tt = 8192, 256, 0.07, 0.04
+    q = torch.randn(n, C, generator=g)
+    k = _unit(torch.randn(n * positives, C, generator=g), 1)
+    queue = _unit(torch.randn(C, K, generator=g), 0)
+    qd = q.to(DEV).requires_grad_()
+    values, indices, tail = H.teacher_top(k.to(DEV)[::positives], queue.to(DEV), Tt, top)
+    logits = H.moco_logits(qd, k.to(DEV), queue.to(DEV), T, positives)
+    loss = distill_loss(logits[:, 1:], values, indices, tail=tail)
+    grad, = torch.autograd.grad(loss, qd)
+    q64 = q.double().requires_grad_()
+    zt = k.double()[::positives] @ queue.double() / Tt
+    # a similarity is a sum of 256 products: off by at most (256 + 8) roundings of the sum of their magnitudes, at most 1 for unit vectors
+    err_t, err_s = 264 * U24 / Tt, 264 * U24 / T + 16 * U24 / T
+    want = torch.sort(zt, 1, descending=True)[0][:, :top]
+    assert float((values.double().cpu() - want).abs().max()) <= err_t * 1.1
+    # from here on with the selection that was made (two similarities within the error may change places)
+    idx = indices.cpu()
+    listed = torch.zeros(n, K, dtype=torch.bool).scatter_(1, idx, True)
+    ninf = torch.full((), -float('inf'), dtype=torch.float64)
+    parts = torch.cat([torch.gather(zt, 1, idx), torch.logsumexp(torch.where(listed, ninf, zt), 1, keepdim=True)], 1)
+    lp = torch.log_softmax(parts, 1)
+    lq = torch.log_softmax(_unit(q64, 1) @ queue.double() / T, 1)
+    lqs = torch.cat([torch.gather(lq, 1, idx), torch.logsumexp(torch.where(listed, ninf, lq), 1, keepdim=True)], 1)
+    ref = (lp.exp() * (lp - lqs)).sum(1).mean()
+    ref_grad, = torch.autograd.grad(ref, q64)
+    # each logarithm of the loss is off by the errors of its similarities, twice (itself and its row's sum); the kernels add 2^-24-relative roundings of
+    # terms of at most 2 / 0.04 = 50 (128 of them)
+    tol = 2 * (err_t + err_s) + 128 * 50 * U24
+    span = float((lp - lqs).detach().abs().max())                   # p's own error, relative 2 err_t, meets the difference of the logarithms
+    assert abs(float(loss.detach()) - float(ref)) <= tol + 2 * err_t * span
+    # d loss / d q: probabilities off by tol relative, times |queue column| / T = 1 / T; the row's gradient is divided by |q| (and n)
+    scale = 2.0 / T / float(q.norm(dim=1).min()) / n
+    assert float((grad.double().cpu() - ref_grad).norm(dim=1).max()) <= 4 * tol * scale
+
+
+def _handler(seed, **kw):
+    h = define_model('mococontrastive', model_save_dir=tempfile.mkdtemp(), device=0, eval_mode=False, model_name='default', crop_count=2, lr=1e-3, **kw)
+    oh = CO.OracleContrastiveHandler('mococontrastive', crop_count=2, lr=1e-3)
+    g = torch.Generator().manual_seed(seed)
+    sd = {k: (torch.randn(v.shape, generator=g) * 0.05 + (1.0 if k.endswith('running_var') else 0.0)).to(v.dtype) if v.is_floating_point() else v
+          for k, v in oh.net.state_dict().items()}
+    sd['queue'] = _unit(torch.randn(sd['queue'].shape, generator=g), 0)
+    h.net.load_state_dict(sd)
+    return h
+
+
+def test_training_step_with_distillation_eager_and_captured(monkeypatch):
+    """steps of define_model('mococontrastive', distill_top=...): the captured step is the eager step bit for bit, the loss is the contrastive loss plus
+    the distillation loss, and without the argument nothing changes"""
+    res = []
+    for mode in ('graph', 'eager'):
+        monkeypatch.setenv('RUMPY_MOCO_STEP_GRAPH', '0' if mode == 'eager' else '1')
+        h = _handler(77, distill_top=32, distill_weight=0.5)
+        out = []
+        for step in range(6):
+            loss, logits = h.run_train(x=CO.contrastive_batch(500 + step, 8, 2).view(8, 6, 32, 32), y=None)
+            targets = [t.clone().cpu() for t in h.net.distill_targets]
+            out.append([float(loss), logits.clone(), h.net.flat_p.clone().cpu(), h.net.flat_g.clone().cpu(), h.net.queue[:, :64].clone().cpu()] + targets)
+            ce = float(torch.nn.functional.cross_entropy(logits.double(), torch.zeros(8, dtype=torch.long)))
+            with torch.no_grad():
+                extra = float(distill_loss(logits.to(DEV)[:, 1:], targets[0].to(DEV), targets[1].to(DEV), tail=targets[2].to(DEV)))
+            assert extra > 0 and abs(float(loss) - ce - 0.5 * extra) < 1e-5 * max(1.0, abs(float(loss)))
+        if mode == 'graph':
+            assert any('graph' in st for st in h._step_graphs.values())
+        res.append(out)
+    for step, (a, b) in enumerate(zip(*res)):
+        assert a[0] == b[0], step
+        for i, (ta, tb) in enumerate(zip(a[1:], b[1:])):
+            assert torch.equal(ta, tb), (step, i)
+    monkeypatch.setenv('RUMPY_MOCO_STEP_GRAPH', '0')
+    x = CO.contrastive_batch(500, 8, 2).view(8, 6, 32, 32)
+    plain = [_handler(77, **kw).run_train(x=x, y=None) for kw in ({}, {'distill_top': None})]
+    assert float(plain[0][0]) == float(plain[1][0]) and torch.equal(plain[0][1], plain[1][1])
+    assert torch.equal(plain[0][1], res[1][0][1])                     # the logits of a first step do not depend on the loss
+    with pytest.raises(ValueError, match='distill_top'):
+        _handler(77, distill_top=257)
+
+
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16], ids=str)
+def test_a_student_of_residual_blocks_learns_from_a_teacher(dtype):
+    """the operators as they are used together: two blocks with norms in front and behind, a gate per image and a learnt scale per channel, logits,
+    the teacher's top logits, the loss, and the gradient of every parameter, against autograd through the definitions in 64 bits"""
+    torch.manual_seed(3)
+    N, P, C, V, k, tau = 4, 36, 96, 1031, 20, 2.0
+    joints = [ResidualNorm(C, pre_norm='layer'), ResidualNorm(C, scale=0.5, post_norm='layer', pre_norm='layer'),
+              ResidualNorm(C, scale=1.0, post_norm='rms', pre_norm='rms', channel_scale=0.3)]
+    mats = [torch.randn(C, C) / C ** 0.5 for _ in range(2)] + [torch.randn(V, C) / C ** 0.5]
+    gate = torch.sigmoid(torch.randn(N, C))
+    x = torch.randn(N, P, C)
+    teacher = torch.randn(N, P, V) * 2
+    weight = (torch.arange(N * P).view(N, P) % 7 != 0).float()
+    for j in joints:
+        for p in j.parameters():
+            p.data += 0.1 * torch.randn_like(p)
+
+    def run(dev, dt, joint, distil, select):
+        leaf = [t.to(dev, dt).requires_grad_() for t in mats] + [gate.to(dev, torch.float64 if dt == torch.float64 else torch.float32).requires_grad_(),
+                                                                x.to(dev, dt).requires_grad_()]
+        params = [p for j in joints for p in j.parameters()]
+        y, h = joint(0, leaf[4], None, None)
+        y, h = joint(1, y, torch.relu(h @ leaf[0].t()), leaf[3])
+        y, h = joint(2, y, torch.relu(h @ leaf[1].t()), None)
+        loss = distil(h @ leaf[2].t(), *select)
+        return loss, torch.autograd.grad(loss, leaf + params)
+
+    # 64 bits, on the CPU
+    for j in joints:
+        j.double()
+
+    def norm64(t, kind, w, b):
+        mu = t.mean(-1, keepdim=True) if kind == 'layer' else 0.0
+        t = (t - mu) / torch.sqrt(((t - mu) ** 2).mean(-1, keepdim=True) + 1e-5) * w
+        return t if b is None else t + b
+
+    def joint64(i, y, t, g):
+        j = joints[i]
+        if t is not None:
+            g = j.gate if j.gate is not None else g[:, None, :] if g is not None else 1.0
+            y = y + j.scale * g * norm64(t, j.post_norm, j.post_weight, j.post_bias)
+        return y, norm64(y, j.pre_norm, j.pre_weight, j.pre_bias)
+
+    values, indices, tail = (t.cpu() for t in top_logits(teacher.to(DEV), k, temperature=tau))
+
+    def distil64(z, v, i, t):
+        lq = torch.log_softmax(z / tau, -1)
+        listed = torch.zeros_like(lq, dtype=torch.bool).scatter_(-1, i, True)
+        lqs = torch.cat([torch.gather(lq, -1, i), torch.logsumexp(lq.masked_fill(listed, -float('inf')), -1, keepdim=True)], -1)
+        lp = torch.log_softmax(torch.cat([v.double() / tau, t.double()[..., None]], -1), -1)
+        rows = tau ** 2 * (lp.exp() * (lp - lqs)).sum(-1)
+        return (rows * weight.double()).sum() / weight.double().sum()
+    ref_loss, ref = run('cpu', torch.float64, joint64, distil64, (values, indices, tail))
+    for j in joints:
+        j.float().to(DEV)
+    got_loss, got = run(DEV, dtype, lambda i, y, t, g: joints[i](y, t, g),
+                        lambda z, v, i, t: distill_loss(z, v, i, tail=t, temperature=tau, row_weight=weight.to(DEV)),
+                        (values.to(DEV), indices.to(DEV), tail.to(DEV)))
+    # storage in between rounds about ten tensors by half a step each (and torch's products, 32 bits inside): 32 half steps of the norm
+    tol = 32 * torch.finfo(dtype).eps / 2 if dtype == torch.bfloat16 else 2e-5
+    assert abs(float(got_loss.detach()) - float(ref_loss.detach())) <= tol * max(1.0, float(ref_loss.detach()))
+    for n, (a, b) in enumerate(zip(got, ref)):
+        assert float((a.double().cpu() - b).norm()) <= tol * float(b.norm()) + 1e-9, n

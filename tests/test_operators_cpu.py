@@ -139,6 +139,7 @@ def _t(*shape, dtype=torch.float32):
     (lambda: residual_norm(_t(3, 8), _t(3, 8), post_weight=_t(8)), ValueError, 'no norm'),
     (lambda: residual_norm(_t(3, 8), _t(3, 8), pre_norm='rms', pre_weight=_t(7)), ValueError, 'pre_weight'),
     (lambda: residual_norm(_t(3, 8), _t(3, 8), pre_norm='rms', pre_bias=_t(8, dtype=torch.bfloat16)), ValueError, 'pre_bias'),
+    (lambda: residual_norm(_t(3, 8), _t(3, 8), pre_norm='rms', eps=0.0), ValueError, 'eps'),
     (lambda: residual_norm(_t(3, 8), _t(3, 8), pre_norm='rms'), RuntimeError, 'no CPU path'),
     (lambda: ResidualNorm(0), ValueError, 'features'),
     (lambda: ResidualNorm(8, pre_norm='group'), ValueError, 'layer'),
