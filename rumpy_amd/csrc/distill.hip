@@ -102,6 +102,23 @@ template <int WG, int LOW> __device__ __forceinline__ uint32_t bound_of(uint32_t
   for (int i = 1; i < WG / 64; ++i) b = min(b, __float_as_uint(sh.red[i]));
   return b;
 }
+// the value that k of the workgroup's `mine` reach: the same search over all waves, a barrier per bit (two buffers in turn)
+template <int WG, int LOW> __device__ __forceinline__ uint32_t bound_of_all(uint32_t mine, int k, TlShared<WG>& sh) {
+  uint32_t t = 0;
+  for (int bit = 31; bit >= LOW; --bit) {
+    const uint32_t trial = t | (1u << bit);
+    uint32_t* n = sh.hist + (bit & 1) * (WG / 64);
+    const uint64_t reach = __ballot(mine >= trial);
+    if ((threadIdx.x & 63) == 0) n[threadIdx.x >> 6] = (uint32_t)__popcll(reach);
+    __syncthreads();
+    uint32_t all = 0;
+#pragma unroll
+    for (int i = 0; i < WG / 64; ++i) all += n[i];
+    if (all >= (uint32_t)k) t = trial;
+  }
+  if (!(t & 0x80000000u)) t |= (1u << LOW) - 1u;
+  return t;
+}
 // the k-th largest of `count` different pairs, 8 bits at a time from the top: needs no assumption about them
 template <int WG, typename At> __device__ __forceinline__ uint64_t radix_kth(At at, int64_t count, int k, TlShared<WG>& sh) {
   const int tid = threadIdx.x;
@@ -221,8 +238,8 @@ template <int WG, typename Emit> __device__ __forceinline__ void place(int k, Tl
 }
 
 // A row (or a piece of one) as whole 16-byte pieces of 8 elements at aligned addresses, and up to 7 elements in front and behind (a row of odd
-// length starts anywhere: pieces at odd addresses run at two thirds of the rate).  NP > 1: a thread's NP pieces stay in registers, so that
-// the row is read once.  NP 1: rows of at most 8 WG elements, element by element over the threads (pieces would leave waves without any).
+// length starts anywhere: pieces at odd addresses run at two thirds of the rate).  NP > 1: a thread's first NP pieces stay in registers, so that
+// they are read once; what a longer row has beyond comes from the caches at every look.  NP 1: rows of at most 8 WG elements, element by element over the threads (pieces would leave waves without any).
 template <int FMT, int WG, int NP> struct RowPieces {
   typedef typename RowElem<FMT>::type E;
   const E* z;
@@ -267,10 +284,14 @@ template <int FMT, int WG, int NP> struct RowPieces {
         }
         fn(v, head + 8 * p, 1);
       }
-    } else {
-      for (int p0 = 0; p0 < count; p0 += WG) {
+    }
+    if (NP * WG < count) {
+      auto piece = [&](int p) { return load_piece<FMT>(z + head + (size_t)8 * min(p, count - 1), 8, 0.f); };
+      RowRaw<FMT> next = piece(NP * WG + (int)threadIdx.x);
+      for (int p0 = NP * WG; p0 < count; p0 += WG) {
         const int p = p0 + (int)threadIdx.x;
-        unpack_piece<FMT>(load_piece<FMT>(z + head + (size_t)8 * min(p, count - 1), 8, 0.f), v);
+        unpack_piece<FMT>(next, v);
+        next = piece(p + WG);
         if (p0 + WG > count) {
 #pragma unroll
           for (int i = 0; i < 8; ++i) v[i] = p < count ? v[i] : -INFINITY;
@@ -284,31 +305,33 @@ template <int FMT, int WG, int NP> struct RowPieces {
       fn(v, first, 1);
     }
   }
-  // fn(inside, value, column): single elements, threads in turn, by whole waves
-  template <typename Fn> __device__ __forceinline__ void each_element(Fn fn) const {
-    for (int64_t j0 = 0; j0 < len; j0 += WG) {
-      const int64_t j = j0 + threadIdx.x;
-      fn(j < len, elem_to_f32<FMT>(z[min(j, (int64_t)len - 1)]), (int)j);
-    }
-  }
 };
 
 // log sum exp(z / tau) over the elements whose pair lies under `kth`, by their maximum; every thread gets it
-template <int FMT, int WG, int NP> __device__ __forceinline__ float rest_below(const RowPieces<FMT, WG, NP>& row, uint64_t kth, float c, float inv_tau, float* red) {
+template <int FMT, int WG> __device__ __forceinline__ float rest_below(const RowPieces<FMT, WG, 0>& row, uint64_t kth, float c, float inv_tau, float* red) {
   float rmx = -INFINITY, bad = 0.f;
-  row.each_element([&](bool in, float v, int j) { if (in && pair_of(v, j) < kth) { rmx = fmaxf(rmx, v); if (v != v) bad = 1.f; } });
+  row.each([&](const float (&v)[8], int j, int stride) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (pair_of(v[i], j + i * stride) < kth) { rmx = fmaxf(rmx, v[i]); if (v[i] != v[i]) bad = 1.f; }
+  });
   rmx = block_max<WG / 64>(rmx, red);
   if (block_max<WG / 64>(bad, red) > 0.f) return NOT_A_NUMBER;
   if (!(fabsf(rmx) < INFINITY)) return rmx;
   float s = 0.f;
-  row.each_element([&](bool in, float v, int j) { if (in && pair_of(v, j) < kth) s += __builtin_amdgcn_exp2f((v - rmx) * c); });
+  row.each([&](const float (&v)[8], int j, int stride) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) s += __builtin_amdgcn_exp2f(pair_of(v[i], j + i * stride) < kth ? (v[i] - rmx) * c : -INFINITY);
+  });
   return fmaf(rmx, inv_tau, __builtin_amdgcn_logf(block_sum<WG / 64>(s, red)) * LN2);
 }
 
-// One workgroup per row or piece, two looks at it: a bound that at least k elements reach, from every thread's maximum; then the few elements
-// that reach the bound (a few times k) and the sum of exp over all others.  Rows whose bound collects too much or is not finite (fewer than about k
-// finite elements), or that hold NaN, take the exact way: the k-th pair by radix search.
-template <int FMT, int WG, int NP> __global__ void __launch_bounds__(WG) top_logits_kernel(rumpy_top_logits_args a, TlPlan plan) {
+// One workgroup per row or piece, two looks at it: a bound T that at least k elements reach, from every thread's maximum; then the few elements
+// that reach the bound (a few times k) and the sum of exp over all others.  Where that does not do - too many reach the bound (columns of equal
+// value), it is infinite or a type's lowest value (fewer than about k columns that no mask holds), or there is NaN - the elements above T and, as
+// far as they do not suffice, those equal to it in the lowest columns; and where those are too many as well, the k-th pair by radix search.
+// Six waves a SIMD: three workgroups of 512 a CU, with most of a row each in registers (with two, 2048 rows of 65521 took 80 us instead of 70).
+template <int FMT, int WG, int NP> __global__ void __launch_bounds__(WG, 6) top_logits_kernel(rumpy_top_logits_args a, TlPlan plan) {
   typedef typename RowElem<FMT>::type E;
   __shared__ TlShared<WG> sh;
   const int tid = threadIdx.x;
@@ -317,24 +340,29 @@ template <int FMT, int WG, int NP> __global__ void __launch_bounds__(WG) top_log
   const int piece = blockIdx.x % plan.splits, c0 = piece * plan.seg;
   RowPieces<FMT, WG, NP> r(reinterpret_cast<const E*>(a.logits) + (size_t)row * a.ld + c0, min(plan.seg, a.V - c0));
   r.load();
+  // the rare ways read the row again, in loops: unrolled over registers like the two looks they made the kernel 10 us slower for every row
+  const RowPieces<FMT, WG, 0> again(r.z, r.len);
   const int len = r.len, k = min(a.k, len);
-  uint32_t n, mine = 0;                                   // candidates of the row, of the wave
+  uint32_t n = ~0u, mine = 0;                             // candidates of the row (~0: a list is too long), of the wave
   float T = 0.f, sum = 0.f;
-  bool exact_way = false;
+  bool summed = false;                                    // `sum` holds everything under T
   if (NP == 1 && len <= WG) {                             // one element per thread: all of them are candidates
     push(tid < len, pair_of(elem_to_f32<FMT>(r.one[0]), tid), mine, sh);
     n = lists_done(mine, sh);
+    summed = true;
   } else {
+    constexpr int LOW = FMT == RUMPY_FMT_BF16 ? 16 : FMT == RUMPY_FMT_F16 ? 13 : 0;
+    auto usable = [&](float b) { return fabsf(b * c) < INFINITY && fabsf(b) < INFINITY; };
     float mx = -INFINITY;                                 // (NaN is passed over here; the second look meets it)
     r.each([&](const float (&v)[8], int, int) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) mx = fmaxf(mx, v[i]);
     });
-    constexpr int LOW = FMT == RUMPY_FMT_BF16 ? 16 : FMT == RUMPY_FMT_F16 ? 13 : 0;
     T = key_value(bound_of<WG, LOW>(order_key(mx), (k + WG / 64 - 1) / (WG / 64), sh));
-    const float m = T * c;
-    exact_way = !(fabsf(m) < INFINITY && fabsf(T) < INFINITY);
-    if (!exact_way) {
+    // (masked columns may leave a wave without enough of its own)
+    if (!usable(T)) T = key_value(bound_of_all<WG, LOW>(order_key(mx), k, sh));
+    if (usable(T)) {
+      const float m = T * c;
       r.each([&](const float (&v)[8], int j, int stride) {
         bool any = false;
 #pragma unroll
@@ -350,13 +378,47 @@ template <int FMT, int WG, int NP> __global__ void __launch_bounds__(WG) top_log
       });
       sum = block_sum<WG / 64>(sum, sh.red);
       n = lists_done(mine, sh);
-      exact_way = n == ~0u || sum != sum;
+      summed = n != ~0u && sum == sum;
+    }
+    if (!summed) {
+      T = key_value(bound_of_all<WG, LOW>(order_key(mx), k, sh));
+      mine = 0;
+      again.each([&](const float (&v)[8], int j, int stride) {
+        bool any = false;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) any |= !(v[i] <= T);            // (NaN counts as largest)
+        if (__ballot(any)) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) push(!(v[i] <= T), pair_of(v[i], j + i * stride), mine, sh);
+        }
+      });
+      n = lists_done(mine, sh);
+      if (n < (uint32_t)k) {
+        // in the order of the columns, WG of them a round, until there are enough
+        int turn = 0;
+        for (int j0 = 0; j0 < len && n < (uint32_t)k; j0 += WG, turn ^= 1) {
+          const int j = j0 + tid;
+          const float v = elem_to_f32<FMT>(r.z[min(j, len - 1)]);
+          push(j < len && v == T, pair_of(v, j), mine, sh);
+          uint32_t* counts = sh.hist + turn * (WG / 64);
+          if ((tid & 63) == 0) counts[tid >> 6] = mine;
+          __syncthreads();
+          n = 0;
+#pragma unroll
+          for (int w = 0; w < WG / 64; ++w) n += counts[w];
+        }
+        n = lists_done(mine, sh);
+      }
     }
   }
-  if (exact_way) {
+  if (n == ~0u) {
     const uint64_t kth = radix_kth([&](int64_t j) { return pair_of(elem_to_f32<FMT>(r.z[j]), (int)j); }, len, k, sh);      // exactly k pairs reach it
     mine = 0;
-    r.each_element([&](bool in, float v, int j) { const uint64_t p = pair_of(v, j); push(in && p >= kth, p, mine, sh); });
+    for (int j0 = 0; j0 < len; j0 += WG) {
+      const int j = j0 + tid;
+      const uint64_t p = pair_of(elem_to_f32<FMT>(r.z[min(j, len - 1)]), j);
+      push(j < len && p >= kth, p, mine, sh);
+    }
     n = lists_done(mine, sh);
   }
   uint64_t* pairs = plan.splits > 1 ? (uint64_t*)a.work + (size_t)blockIdx.x * a.k : nullptr;
@@ -371,9 +433,9 @@ template <int FMT, int WG, int NP> __global__ void __launch_bounds__(WG) top_log
   if (pairs) for (int i = k + tid; i < a.k; i += WG) pairs[i] = 0;       // a piece shorter than k
   float tail;
   if (n == (uint32_t)len && sh.next == 0) tail = -INFINITY;      // everything is chosen
-  else if (sh.next == 0 && (exact_way || sum < 1e-20f)) {
-    // nothing collected beyond the top, and the others lie so far under the bound that their sum has no digits left (or was not made)
-    tail = rest_below(r, sh.kth, c, a.inv_tau, sh.red);
+  else if (!summed || (sh.next == 0 && sum < 1e-20f)) {
+    // no sum was made, or nothing was collected beyond the top and the others lie so far under the bound that their sum has no digits left
+    tail = rest_below(again, sh.kth, c, a.inv_tau, sh.red);
   } else {
     const float next = sh.next ? pair_value(sh.next) : T;
     // relative to the largest that was not chosen: the other candidates, and the sum under the bound with T's distance from it
@@ -457,13 +519,12 @@ extern "C" int64_t rumpy_top_logits_work_bytes(int64_t rows, int32_t V, int32_t 
 template <int FMT, int WG> static void tl_launch_wg(const rumpy_top_logits_args& a, const TlPlan& plan, hipStream_t s) {
   const dim3 grid((unsigned)(a.rows * plan.splits)), wg(WG);
   const int len = a.V < plan.seg ? a.V : plan.seg, np = (len / 8 + WG - 1) / WG;
-  constexpr int MOST = WG == 128 ? 4 : WG == 256 || FMT == RUMPY_FMT_F32 ? 8 : 16;          // pieces in registers (the callers' limits; 64 registers)
+  constexpr int MOST = WG == 128 ? 4 : WG == 256 ? 8 : FMT == RUMPY_FMT_F32 ? 7 : 15;          // pieces in registers: the callers' limits; 60 registers
   if (len <= 8 * WG) hipLaunchKernelGGL((top_logits_kernel<FMT, WG, 1>), grid, wg, 0, s, a, plan);
   else if (np <= 2) hipLaunchKernelGGL((top_logits_kernel<FMT, WG, 2>), grid, wg, 0, s, a, plan);
   else if (np <= 4) hipLaunchKernelGGL((top_logits_kernel<FMT, WG, 4>), grid, wg, 0, s, a, plan);
-  else if (np <= 8 && MOST >= 8) hipLaunchKernelGGL((top_logits_kernel<FMT, WG, MOST >= 8 ? 8 : 1>), grid, wg, 0, s, a, plan);
-  else if (np <= MOST) hipLaunchKernelGGL((top_logits_kernel<FMT, WG, MOST>), grid, wg, 0, s, a, plan);
-  else if constexpr (WG == 512) hipLaunchKernelGGL((top_logits_kernel<FMT, WG, 0>), grid, wg, 0, s, a, plan);
+  else if (np <= 8 && MOST > 8) hipLaunchKernelGGL((top_logits_kernel<FMT, WG, (MOST > 8 ? 8 : MOST)>), grid, wg, 0, s, a, plan);
+  else hipLaunchKernelGGL((top_logits_kernel<FMT, WG, MOST>), grid, wg, 0, s, a, plan);
 }
 template <int FMT> static void tl_launch(const rumpy_top_logits_args& a, const TlPlan& plan, hipStream_t s) {
   // Many short rows: small workgroups, more rows at once (a row is a chain of latencies: bound, lists, places).  At least 2 k threads, so that
@@ -583,7 +644,7 @@ __device__ __forceinline__ void ds_finish(const rumpy_distill_args& a, int64_t r
   vm = wave_max(vm, lane);
   zm = wave_max(zm, lane);
   const float tl = rest ? a.tail[row] : -INFINITY;
-  const bool nan = __ballot(odd || outside) != 0ull || tl != tl;
+  bool nan = __ballot(odd || outside) != 0ull || tl != tl;
   float* st = a.state + row * DS_STATE;
   if (!nan && vm == -INFINITY && tl == -INFINITY) {            // the teacher says nothing about this row
     if (lane == 0) { a.row_loss[row] = 0.f; st[0] = st[1] = st[2] = st[3] = st[4] = 0.f; st[5] = 1.f; }
@@ -600,6 +661,7 @@ __device__ __forceinline__ void ds_finish(const rumpy_distill_args& a, int64_t r
     if (rest && l.first[i]) sl += ds_exp(l.z[i], M, c, Mc);
   }
   p_sum = wave64_sum(p_sum, lane) + (rest ? __builtin_amdgcn_exp2f((tr - up) * LOG2E) : 0.f);
+  nan |= p_sum != p_sum;                                   // (infinite logits of the teacher)
   const float ln_p = __builtin_amdgcn_logf(p_sum) * LN2;
   float S = s;
   if (rest) S = wave64_sum(sl, lane) + (m == -INFINITY ? 0.f : s * ds_rescale(m, M, c));
