@@ -742,13 +742,13 @@ int64_t rumpy_residual_norm_partial_floats(int64_t rows, int64_t group_rows, int
 /* ---- distillation from a teacher's top logits (csrc/distill.hip), beside rumpy_ce_rows: rows of V logits in fp32 / bf16 / fp16 with a row stride
  * (columns contiguous, any alignment of an element), all sums in fp32, fixed orders.
  * rumpy_top_logits: per row the k <= 256 largest logits, descending, equal ones by index (NaN counts as largest), as they are in `values`
- * [rows, k] (the logits' format) with int64 `indices`; tail[r] = log of the sum of exp(logit * inv_tau) over all others (-inf: none).
+ * [rows, k] (the logits' format) with int64 `indices`; tail[r] = log of the sum of exp(logit / tau) over all others (-inf: none).
  * work: rumpy_top_logits_work_bytes(rows, V, k) bytes (0: NULL). */
 typedef struct {
   const void* logits; void* values; void* indices; float* tail; void* work;
   int64_t rows, ld;
-  int32_t V, k, fmt;
-  float inv_tau;
+  int32_t V, k, fmt, pad_;
+  double tau;
 } rumpy_top_logits_args;
 int rumpy_top_logits(const rumpy_top_logits_args* a, void* stream);
 int64_t rumpy_top_logits_work_bytes(int64_t rows, int32_t V, int32_t k);
@@ -766,7 +766,7 @@ typedef struct {
   const float* gout; void* dlogits;
   int64_t rows, ld;
   int32_t V, k, fmt, value_fmt, index64, mean;
-  float tau, inv_tau;
+  double tau;
 } rumpy_distill_args;
 int rumpy_distill_fwd(const rumpy_distill_args* a, void* stream);
 int rumpy_distill_bwd(const rumpy_distill_args* a, void* stream);

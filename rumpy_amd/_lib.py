@@ -326,15 +326,15 @@ class ResidualNormBwdArgs(_S):
 
 
 class TopLogitsArgs(_S):
-    _fields_ = [('logits', c_void_p), ('values', c_void_p), ('indices', c_void_p), ('tail', c_void_p), ('work', c_void_p), ('rows', c_int64), ('ld', c_int64), ('V', c_int32), ('k', c_int32), ('fmt', c_int32),
-                ('inv_tau', c_float)]
+    _fields_ = [('logits', c_void_p), ('values', c_void_p), ('indices', c_void_p), ('tail', c_void_p), ('work', c_void_p), ('rows', c_int64), ('ld', c_int64), ('V', c_int32), ('k', c_int32), ('fmt', c_int32), ('pad_', c_int32),
+                ('tau', C.c_double)]
 
 
 class DistillArgs(_S):
     _fields_ = [('logits', c_void_p), ('top_values', c_void_p), ('top_indices', c_void_p), ('tail', c_void_p), ('row_weight', c_void_p),
                 ('row_loss', c_void_p), ('state', c_void_p), ('loss', c_void_p), ('factor', c_void_p), ('partial', c_void_p), ('gout', c_void_p), ('dlogits', c_void_p),
                 ('rows', c_int64), ('ld', c_int64),
-                ('V', c_int32), ('k', c_int32), ('fmt', c_int32), ('value_fmt', c_int32), ('index64', c_int32), ('mean', c_int32), ('tau', c_float), ('inv_tau', c_float)]
+                ('V', c_int32), ('k', c_int32), ('fmt', c_int32), ('value_fmt', c_int32), ('index64', c_int32), ('mean', c_int32), ('tau', C.c_double)]
 
 
 # every symbol include/rumpy_amd.h declares: name -> (restype, argtypes)

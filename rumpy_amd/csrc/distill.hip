@@ -7,11 +7,13 @@
 // selection's second look, from the caches), the gradient reads it once and writes it once: bound by memory, with one exponential per element
 // and direction beside it.  The sum of exp runs over the row once with a running maximum per thread; q_t is summed directly over the columns
 // that are not listed (a bit map of them lies in LDS): 1 - sum q_i would cancel where the listed columns hold nearly everything.
-// All sums and exponentials are fp32; every reduction has a fixed order, so results are bitwise reproducible.
+// Exponentials and a row's sums are fp32, a row's logarithms and the sums over rows 64-bit.  Every reduction has a fixed order, which goes with the
+// alignment of a row's address alone: results are bitwise reproducible.
 #include "row_vec.hpp"
 
 constexpr int DS_MAXK = 256, DS_MAXV = 1 << 30;
-constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
+constexpr double LOG2E = 1.4426950408889634, LN2 = 0.6931471805599453;
+constexpr float LOG2E_F = (float)LOG2E;
 
 __device__ __forceinline__ float wave_max(float v, int lane) {
   v = fmaxf(v, dpp_quad1(v)); v = fmaxf(v, dpp_quad2(v)); v = fmaxf(v, dpp_half_mirror(v)); v = fmaxf(v, dpp_row_mirror(v));
@@ -58,10 +60,12 @@ constexpr float NOT_A_NUMBER = __builtin_nanf("");
 
 // Rows that are few and long are cut: every piece of a row gives its own k largest pairs and its tail to a workspace, and one more workgroup per
 // row joins them.
-struct TlPlan { int splits, seg; };
+struct TlPlan { int splits, seg; float c; double inv_tau; };          // c = log2(e) / tau, rounded once
 constexpr int TL_MOST_SPLITS = 32;
-static TlPlan tl_plan(int64_t rows, int32_t V) {
+static TlPlan tl_plan(int64_t rows, int32_t V, double tau) {
   TlPlan p;
+  p.c = (float)(LOG2E / tau);
+  p.inv_tau = 1.0 / tau;
   int64_t s = 1;
   if (V >= 32768 && rows > 0) {
     s = (256 + rows - 1) / rows;
@@ -308,7 +312,8 @@ template <int FMT, int WG, int NP> struct RowPieces {
 };
 
 // log sum exp(z / tau) over the elements whose pair lies under `kth`, by their maximum; every thread gets it
-template <int FMT, int WG> __device__ __forceinline__ float rest_below(const RowPieces<FMT, WG, 0>& row, uint64_t kth, float c, float inv_tau, float* red) {
+template <int FMT, int WG> __device__ __forceinline__ float rest_below(const RowPieces<FMT, WG, 0>& row, uint64_t kth, const TlPlan& plan, float* red) {
+  const float c = plan.c;
   float rmx = -INFINITY, bad = 0.f;
   row.each([&](const float (&v)[8], int j, int stride) {
 #pragma unroll
@@ -323,7 +328,7 @@ template <int FMT, int WG> __device__ __forceinline__ float rest_below(const Row
 #pragma unroll
     for (int i = 0; i < 8; ++i) s += __builtin_amdgcn_exp2f(pair_of(v[i], j + i * stride) < kth ? (v[i] - rmx) * c : -INFINITY);
   });
-  return fmaf(rmx, inv_tau, __builtin_amdgcn_logf(block_sum<WG / 64>(s, red)) * LN2);
+  return (float)(rmx * plan.inv_tau + log(block_sum<WG / 64>(s, red)));
 }
 
 // One workgroup per row or piece, two looks at it: a bound T that at least k elements reach, from every thread's maximum; then the few elements
@@ -335,7 +340,7 @@ template <int FMT, int WG, int NP> __global__ void __launch_bounds__(WG, 6) top_
   typedef typename RowElem<FMT>::type E;
   __shared__ TlShared<WG> sh;
   const int tid = threadIdx.x;
-  const float c = a.inv_tau * LOG2E;
+  const float c = plan.c;
   const int64_t row = blockIdx.x / plan.splits;
   const int piece = blockIdx.x % plan.splits, c0 = piece * plan.seg;
   RowPieces<FMT, WG, NP> r(reinterpret_cast<const E*>(a.logits) + (size_t)row * a.ld + c0, min(plan.seg, a.V - c0));
@@ -435,14 +440,14 @@ template <int FMT, int WG, int NP> __global__ void __launch_bounds__(WG, 6) top_
   if (n == (uint32_t)len && sh.next == 0) tail = -INFINITY;      // everything is chosen
   else if (!summed || (sh.next == 0 && sum < 1e-20f)) {
     // no sum was made, or nothing was collected beyond the top and the others lie so far under the bound that their sum has no digits left
-    tail = rest_below(again, sh.kth, c, a.inv_tau, sh.red);
+    tail = rest_below(again, sh.kth, plan, sh.red);
   } else {
     const float next = sh.next ? pair_value(sh.next) : T;
     // relative to the largest that was not chosen: the other candidates, and the sum under the bound with T's distance from it
     float s = 0.f;
     for (uint32_t i = k + tid; i < n; i += WG) s += __builtin_amdgcn_exp2f((sh.after[i] - next) * c);
     s = block_sum<WG / 64>(s, sh.red) + (sum > 0.f ? sum * __builtin_amdgcn_exp2f((T - next) * c) : 0.f);
-    tail = fabsf(next) < INFINITY ? fmaf(next, a.inv_tau, __builtin_amdgcn_logf(s) * LN2) : next;
+    tail = fabsf(next) < INFINITY ? (float)(next * plan.inv_tau + logf(s)) : next;
   }
   if (tid == 0) {
     if (pairs) reinterpret_cast<float*>((uint64_t*)a.work + (size_t)gridDim.x * a.k)[blockIdx.x] = tail;
@@ -495,25 +500,25 @@ template <int FMT> __global__ void __launch_bounds__(512) top_join_kernel(rumpy_
 #pragma unroll
   for (int u = 0; u < NP; ++u) {
     if (mine[u] && mine[u] < kth) {
-      const float v = pair_value(mine[u]) * a.inv_tau;
+      const float v = (float)(pair_value(mine[u]) * plan.inv_tau);
       m = fmaxf(m, v);
       if (v != v) bad = 1.f;
     }
   }
   m = block_max<WG / 64>(m, sh.red);
   bad = block_max<WG / 64>(bad, sh.red);
-  float s = __builtin_amdgcn_exp2f((tail_in - m) * LOG2E);
+  float s = __builtin_amdgcn_exp2f((tail_in - m) * LOG2E_F);
 #pragma unroll
   for (int u = 0; u < NP; ++u) {
-    if (mine[u] && mine[u] < kth) s += __builtin_amdgcn_exp2f((pair_value(mine[u]) * a.inv_tau - m) * LOG2E);
+    if (mine[u] && mine[u] < kth) s += __builtin_amdgcn_exp2f(((float)(pair_value(mine[u]) * plan.inv_tau) - m) * LOG2E_F);
   }
   s = block_sum<WG / 64>(s, sh.red);
-  if (tid == 0) a.tail[row] = bad > 0.f ? NOT_A_NUMBER : fabsf(m) < INFINITY ? m + __builtin_amdgcn_logf(s) * LN2 : m;
+  if (tid == 0) a.tail[row] = bad > 0.f ? NOT_A_NUMBER : fabsf(m) < INFINITY ? m + logf(s) : m;
 }
 
 extern "C" int64_t rumpy_top_logits_work_bytes(int64_t rows, int32_t V, int32_t k) {
   if (rows <= 0 || V < 1 || V > DS_MAXV || k < 1 || k > DS_MAXK) return 0;
-  const TlPlan plan = tl_plan(rows, V);
+  const TlPlan plan = tl_plan(rows, V, 1.0);
   return plan.splits > 1 ? rows * plan.splits * (k * 8 + 4) : 0;
 }
 template <int FMT, int WG> static void tl_launch_wg(const rumpy_top_logits_args& a, const TlPlan& plan, hipStream_t s) {
@@ -540,14 +545,14 @@ extern "C" int rumpy_top_logits(const rumpy_top_logits_args* p, void* stream) {
   if (!bad && (p->fmt != RUMPY_FMT_F32 && p->fmt != RUMPY_FMT_BF16 && p->fmt != RUMPY_FMT_F16)) bad = "fp32, bf16 or fp16 logits";
   if (!bad && (p->rows < 0 || p->V < 1 || p->V > DS_MAXV || p->ld < 0)) bad = "rows of 1 .. 2^30 logits";
   if (!bad && (p->k < 1 || p->k > DS_MAXK || p->k > p->V)) bad = "1 .. 256 top logits, no more than the row has";
-  if (!bad && !(p->inv_tau > 0.f && p->inv_tau < INFINITY)) bad = "a temperature above zero";
+  if (!bad && !(p->tau >= 1e-30 && p->tau <= 1e30)) bad = "a temperature above zero";
   if (!bad && p->rows && (!p->logits || !p->values || !p->indices || !p->tail)) bad = "a tensor is missing";
   if (!bad && rumpy_top_logits_work_bytes(p->rows, p->V, p->k) && (!p->work || ((uintptr_t)p->work & 7)))
     bad = "rows of this length and number are cut and need `work` (rumpy_top_logits_work_bytes, at a multiple of 8)";
   if (!bad && p->rows > 0x7fffffff) bad = "too many rows";
   if (bad) { rumpy_set_error("rumpy_top_logits: %s", bad); return RUMPY_E_ARG; }
   if (p->rows == 0) return RUMPY_OK;
-  const TlPlan plan = tl_plan(p->rows, p->V);
+  const TlPlan plan = tl_plan(p->rows, p->V, p->tau);
   hipStream_t s = (hipStream_t)stream;
   if (p->fmt == RUMPY_FMT_F32) tl_launch<RUMPY_FMT_F32>(*p, plan, s);
   else if (p->fmt == RUMPY_FMT_BF16) tl_launch<RUMPY_FMT_BF16>(*p, plan, s);
@@ -559,12 +564,13 @@ extern "C" int rumpy_top_logits(const rumpy_top_logits_args* p, void* stream) {
 constexpr int DS_WG = 512, DS_WAVES = DS_WG / 64;
 constexpr int DS_STATE = 8;      // per row: reference and coefficient of the streamed columns, maximum and log sum of all, the teacher's log sum, dead, the teacher's maximum
 
-// exp((v - m) / tau) with c = log2(e) / tau.  One fused multiply-add per element needs m c finite: a type's lowest value (a mask) overflows
-// there, and takes the difference first.  fl(m c) is off m c by a rounding, ds_off says how much (in powers of two).
-__device__ __forceinline__ float ds_exp(float v, float m, float c, float mc) {
-  return __builtin_amdgcn_exp2f(fabsf(mc) < INFINITY ? fmaf(v, c, -mc) : (v - m) * c);
+// exp((v - m) / tau) with c + lo = log2(e) / tau: c alone, rounded to 32 bits, is another temperature for the whole row, and its error of up to 2^-25
+// does not average out in the loss (1.8e-6 of it where 32-bit divisions made 2e-7).  Two fused multiply-adds per element; they need m c finite: a
+// type's lowest value (a mask) overflows there, and takes the difference first.  fl(m c) is off m (c + lo), ds_off says how much (in powers of two).
+__device__ __forceinline__ float ds_exp(float v, float m, float c, float lo, float mc) {
+  return __builtin_amdgcn_exp2f(fabsf(mc) < INFINITY ? fmaf(v, c, fmaf(v, lo, -mc)) : (v - m) * c);
 }
-__device__ __forceinline__ float ds_off(float m, float c) { const float mc = m * c; return fabsf(mc) < INFINITY ? fmaf(m, c, -mc) : 0.f; }
+__device__ __forceinline__ float ds_off(float m, float c, float lo) { const float mc = m * c; return fabsf(mc) < INFINITY ? fmaf(m, lo, fmaf(m, c, -mc)) : 0.f; }
 // the factor from a sum relative to m to one relative to M >= m.  Where a product overflows, different values are so far apart that it is 0.
 __device__ __forceinline__ float ds_rescale(float m, float M, float c) {
   if (m == M) return 1.f;
@@ -572,10 +578,17 @@ __device__ __forceinline__ float ds_rescale(float m, float M, float c) {
   return m == -INFINITY || d != d ? 0.f : __builtin_amdgcn_exp2f(d);
 }
 
-struct DsPlan { int splits, seg; };
+struct DsPlan { int splits, seg; float c, lo, near, inv_tau; double inv_tau64; };      // c + lo = log2(e) / tau; near: the nearest float to it
 // rows are cut when there are too few of them to fill the chip; a piece's bit map of listed columns has to fit LDS (2^18 columns: 32 KB)
-static DsPlan ds_plan(int64_t rows, int32_t V) {
+static DsPlan ds_plan(int64_t rows, int32_t V, double tau) {
   DsPlan p;
+  // c is rounded towards zero: a -inf (a masked column) times c and times a positive lo is -inf, where a negative lo would make it NaN
+  const double x = LOG2E / tau;
+  p.near = (float)x;
+  p.c = (double)p.near > x ? nextafterf(p.near, 0.f) : p.near;
+  p.lo = fmaxf((float)(x - p.c), p.c * 1e-12f);
+  p.inv_tau64 = 1.0 / tau;
+  p.inv_tau = (float)p.inv_tau64;
   int64_t s = rows > 0 ? (512 + rows - 1) / rows : 1;
   const int64_t most = (V + 8191) / 8192, least = ((int64_t)V + (1 << 18) - 1) >> 18;
   if (s > most) s = most;
@@ -627,9 +640,10 @@ template <int FMT> __device__ __forceinline__ int ds_load_listed(const rumpy_dis
 }
 
 // one wave: the row's loss and what its gradient needs, from the sum over the streamed columns (all of them, or the unlisted ones when the
-// rest is an outcome): s = sum exp2(z c - fl(m c)).
-__device__ __forceinline__ void ds_finish(const rumpy_distill_args& a, int64_t row, const DsListed& l, float m, float s, int lane) {
-  const float inv_tau = a.inv_tau, c = inv_tau * LOG2E;
+// rest is an outcome): s = sum exp2(z (c + lo) - fl(m c)).  The logarithms and their sum are made in 64 bits: the loss is a small difference of them.
+__device__ __forceinline__ void ds_finish(const rumpy_distill_args& a, const DsPlan& plan, int64_t row, const DsListed& l, float m, float s, int lane) {
+  const float c = plan.c, lo = plan.lo;
+  const double inv_tau = plan.inv_tau64;
   const bool rest = a.tail != nullptr;
   const float w = a.row_weight ? a.row_weight[row] : 1.f;
   float vm = -INFINITY, zm = -INFINITY;
@@ -652,43 +666,44 @@ __device__ __forceinline__ void ds_finish(const rumpy_distill_args& a, int64_t r
   }
   // the teacher's logarithms relative to its largest logit, so that far from zero no digits are lost: lp = (v - vm) / tau - up - ln_p
   if (vm == -INFINITY) vm = 0.f;
-  const float tr = fmaf(-vm, inv_tau, tl), up = fmaxf(0.f, tr);
+  const double tr = tl - vm * inv_tau, up = tr > 0.0 ? tr : 0.0;
   const float M = rest ? fmaxf(m, zm) : m, Mc = M * c;
   float p_sum = 0.f, sl = 0.f;
   for (int i = lane; i < a.k; i += 64) {
     if (l.idx[i] < 0) continue;
-    p_sum += __builtin_amdgcn_exp2f(((l.v[i] - vm) * inv_tau - up) * LOG2E);
-    if (rest && l.first[i]) sl += ds_exp(l.z[i], M, c, Mc);
+    p_sum += __builtin_amdgcn_exp2f((float)((((double)l.v[i] - vm) * inv_tau - up) * LOG2E));
+    if (rest && l.first[i]) sl += ds_exp(l.z[i], M, c, lo, Mc);
   }
-  p_sum = wave64_sum(p_sum, lane) + (rest ? __builtin_amdgcn_exp2f((tr - up) * LOG2E) : 0.f);
+  p_sum = wave64_sum(p_sum, lane) + (rest ? __builtin_amdgcn_exp2f((float)((tr - up) * LOG2E)) : 0.f);
   nan |= p_sum != p_sum;                                   // (infinite logits of the teacher)
-  const float ln_p = __builtin_amdgcn_logf(p_sum) * LN2;
+  const double ln_p = log((double)p_sum);
   float S = s;
   if (rest) S = wave64_sum(sl, lane) + (m == -INFINITY ? 0.f : s * ds_rescale(m, M, c));
-  const float ln_s = (__builtin_amdgcn_logf(S) - ds_off(M, c)) * LN2;
-  float loss = 0.f;
+  const double ln_s = log((double)S) - ds_off(M, c, lo) * LN2;
+  double loss = 0.0;
   for (int i = lane; i < a.k; i += 64) {
     if (l.idx[i] < 0) continue;
-    const float lp = (l.v[i] - vm) * inv_tau - up - ln_p, p = __builtin_amdgcn_exp2f(lp * LOG2E);
-    if (p != 0.f) loss += p * (lp - ((l.z[i] - M) * inv_tau - ln_s));
+    const double lp = ((double)l.v[i] - vm) * inv_tau - up - ln_p;
+    const float p = __builtin_amdgcn_exp2f((float)(lp * LOG2E));
+    if (p != 0.f) loss += p * (lp - (((double)l.z[i] - M) * inv_tau - ln_s));
   }
-  loss = wave64_sum(loss, lane);
+#pragma unroll
+  for (int o = 1; o < 64; o *= 2) loss += __shfl_xor(loss, o);
   float coef = 1.f / S;
   if (rest) {
-    const float lpt = tr - up - ln_p, pt = __builtin_amdgcn_exp2f(lpt * LOG2E);
-    const float lqt = m == -INFINITY ? -INFINITY : (m - M) * inv_tau + (__builtin_amdgcn_logf(s) - ds_off(m, c)) * LN2 - ln_s;
-    const float qt = __builtin_amdgcn_exp2f(lqt * LOG2E);
+    const double lpt = tr - up - ln_p, lqt = m == -INFINITY ? (double)-INFINITY : ((double)m - M) * inv_tau + log((double)s) - ds_off(m, c, lo) * LN2 - ln_s;
+    const float pt = __builtin_amdgcn_exp2f((float)(lpt * LOG2E)), qt = __builtin_amdgcn_exp2f((float)(lqt * LOG2E));
     if (pt != 0.f) loss += pt * (lpt - lqt);
     coef = m == -INFINITY ? 0.f : (qt - pt) / s;
   }
-  if (nan) loss = coef = __uint_as_float(0x7fc00000u);
+  if (nan) loss = coef = NOT_A_NUMBER;
   if (lane == 0) {
-    a.row_loss[row] = w == 0.f ? 0.f : w * loss * a.tau * a.tau;
+    a.row_loss[row] = w == 0.f ? 0.f : (float)(w * loss * a.tau * a.tau);
     st[0] = m == -INFINITY ? 0.f : m;
-    st[1] = coef;
+    st[1] = m == -INFINITY ? coef : coef * __builtin_amdgcn_exp2f(ds_off(m, c, lo) - ds_off(m, plan.near, 0.f));      // (the gradient's exponentials are of z near - fl(m near))
     st[2] = M;
-    st[3] = nan ? coef : ln_s;
-    st[4] = up + ln_p;
+    st[3] = nan ? coef : (float)ln_s;
+    st[4] = (float)(up + ln_p);
     st[5] = w == 0.f ? 1.f : 0.f;
     st[6] = vm;
   }
@@ -734,7 +749,7 @@ template <int FMT, bool REST> __global__ void __launch_bounds__(DS_WG) distill_f
     if (mine >= j0 && mine < j1) { const int bit = (int)(mine - j0) + shift; atomicOr(&bits[bit >> 5], 1u << (bit & 31)); }
     __syncthreads();
   }
-  const float c = a.inv_tau * LOG2E;
+  const float c = plan.c, lo = plan.lo;
   float m = -INFINITY, s = 0.f, mc = 0.f;
   auto sum_up = [&](auto& v) {
     constexpr int N = sizeof(v) / sizeof(v[0]);
@@ -752,7 +767,7 @@ template <int FMT, bool REST> __global__ void __launch_bounds__(DS_WG) distill_f
 #pragma unroll
       for (int u = 0; u < N; ++u)
 #pragma unroll
-        for (int i = 0; i < 8; ++i) s += __builtin_amdgcn_exp2f(fmaf(v[u][i], c, -mc));
+        for (int i = 0; i < 8; ++i) s += __builtin_amdgcn_exp2f(fmaf(v[u][i], c, fmaf(v[u][i], lo, -mc)));
     } else {
 #pragma unroll
       for (int u = 0; u < N; ++u)
@@ -807,7 +822,7 @@ template <int FMT, bool REST> __global__ void __launch_bounds__(DS_WG) distill_f
     if (tid == 0) { a.partial[blockIdx.x * (size_t)2] = M; a.partial[blockIdx.x * (size_t)2 + 1] = s; }
     return;
   }
-  if (tid < 64) ds_finish(a, row, l, M, s, tid);
+  if (tid < 64) ds_finish(a, plan, row, l, M, s, tid);
 }
 
 // rows that were cut: their pieces' sums, then the row
@@ -822,7 +837,7 @@ template <int FMT> __global__ void __launch_bounds__(DS_WG) distill_join_kernel(
     return;
   }
   ds_load_listed<FMT>(a, row, reinterpret_cast<const E*>(a.logits) + (size_t)row * a.ld, l);
-  const float c = a.inv_tau * LOG2E;
+  const float c = plan.c;
   const float* part = a.partial + (size_t)row * plan.splits * 2;
   float m = -INFINITY;
   for (int i = tid; i < plan.splits; i += DS_WG) m = fmaxf(m, part[2 * i]);
@@ -833,14 +848,14 @@ template <int FMT> __global__ void __launch_bounds__(DS_WG) distill_join_kernel(
     s += mi == -INFINITY ? part[2 * i + 1] : part[2 * i + 1] * ds_rescale(mi, M, c);
   }
   s = block_sum<DS_WAVES>(s, red);
-  if (tid < 64) ds_finish(a, row, l, M, s, tid);
+  if (tid < 64) ds_finish(a, plan, row, l, M, s, tid);
 }
 
 // loss = sum of the rows' (weighted) losses, over the sum of the weights for the mean; a sum of weights of zero gives 0
 // (one workgroup: 8 rows a thread are asked for together)
 __global__ void __launch_bounds__(1024) distill_total_kernel(rumpy_distill_args a) {
-  __shared__ float red[16];
-  float s = 0.f, w = 0.f;
+  __shared__ double red[2][16];
+  double s = 0.0, w = 0.0;
   for (int64_t r0 = threadIdx.x; r0 < a.rows; r0 += 8 * 1024) {
     float l[8], wr[8];
 #pragma unroll
@@ -852,12 +867,16 @@ __global__ void __launch_bounds__(1024) distill_total_kernel(rumpy_distill_args 
 #pragma unroll
     for (int i = 0; i < 8; ++i) { s += l[i]; w += wr[i]; }
   }
-  s = block_sum<16>(s, red);
-  w = block_sum<16>(w, red);
+#pragma unroll
+  for (int o = 1; o < 64; o *= 2) { s += __shfl_xor(s, o); w += __shfl_xor(w, o); }
+  if ((threadIdx.x & 63) == 0) { red[0][threadIdx.x >> 6] = s; red[1][threadIdx.x >> 6] = w; }
+  __syncthreads();
   if (threadIdx.x == 0) {
-    const float f = !a.mean ? 1.f : w == 0.f ? 0.f : 1.f / w;
-    *a.factor = f;
-    *a.loss = f == 0.f ? 0.f : s * f;
+    s = w = 0.0;
+    for (int i = 0; i < 16; ++i) { s += red[0][i]; w += red[1][i]; }
+    const double f = !a.mean ? 1.0 : w == 0.0 ? 0.0 : 1.0 / w;
+    *a.factor = (float)f;
+    *a.loss = f == 0.0 ? 0.f : (float)(s * f);
   }
 }
 
@@ -877,15 +896,15 @@ template <int FMT> __global__ void __launch_bounds__(DS_WG) distill_bwd_kernel(r
     for (int64_t j = j0 + tid * 8; j < j1; j += DS_WG * 8) store8<FMT>(a.dlogits, out + j, (int)min((int64_t)8, j1 - j), zero);
     return;
   }
-  const float c = a.inv_tau * LOG2E;
-  float g = (a.loss ? *a.gout * *a.factor : a.gout[row]) * a.tau;
+  const float c = plan.near;
+  float g = (a.loss ? *a.gout * *a.factor : a.gout[row]) * (float)a.tau;
   if (a.row_weight) g *= a.row_weight[row];
   const float m = st[0], mc = m * c, coef = g * st[1];
   const bool fused = fabsf(mc) < INFINITY;
   if (tid < a.k) {
     const int64_t i = ds_index(a, row, tid);
     idx[tid] = i >= j0 && i < j1 ? (int)i : -1;
-    p[tid] = i < 0 ? 0.f : __builtin_amdgcn_exp2f(((ds_value(a, row, tid) - st[6]) * a.inv_tau - st[4]) * LOG2E);
+    p[tid] = i < 0 ? 0.f : __builtin_amdgcn_exp2f(((ds_value(a, row, tid) - st[6]) * plan.inv_tau - st[4]) * LOG2E_F);
   }
   for (int64_t j = j0 + tid * 8; j < j1; j += DS_WG * 8) {
     const int n = (int)min((int64_t)8, j1 - j);
@@ -907,7 +926,7 @@ template <int FMT> __global__ void __launch_bounds__(DS_WG) distill_bwd_kernel(r
 #pragma unroll
       for (int i = 0; i < 16; ++i) share += o + i < a.k && other[i] == mine ? po[i] : 0.f;
     }
-    const float q = __builtin_amdgcn_exp2f(((elem_to_f32<FMT>(z[idx[tid]]) - st[2]) * a.inv_tau - st[3]) * LOG2E);
+    const float q = __builtin_amdgcn_exp2f(((elem_to_f32<FMT>(z[idx[tid]]) - st[2]) * plan.inv_tau - st[3]) * LOG2E_F);
     reinterpret_cast<E*>(a.dlogits)[out + idx[tid]] = f32_to_elem<FMT>(g * (q - share));
   }
 }
@@ -918,17 +937,17 @@ static const char* ds_check(const rumpy_distill_args* p) {
   if (!ds_fmt(p->fmt) || !ds_fmt(p->value_fmt)) return "fp32, bf16 or fp16 logits and top logits";
   if (p->rows < 0 || p->V < 1 || p->V > DS_MAXV || p->ld < 0) return "rows of 1 .. 2^30 logits";
   if (p->k < 1 || p->k > DS_MAXK) return "1 .. 256 top logits a row";
-  if (!(p->tau > 0.f && p->tau < INFINITY && p->inv_tau > 0.f && p->inv_tau < INFINITY)) return "a temperature above zero";
+  if (!(p->tau >= 1e-30 && p->tau <= 1e30)) return "a temperature above zero";
   if (p->rows && (!p->logits || !p->top_values || !p->top_indices || !p->row_loss || !p->state)) return "a tensor is missing";
   if (p->loss && !p->factor) return "the reduction's factor is missing";
-  const DsPlan plan = ds_plan(p->rows, p->V);
+  const DsPlan plan = ds_plan(p->rows, p->V, p->tau);
   if (p->rows * plan.splits > 0x7fffffff) return "too many rows";
   if (plan.splits > 1 && !p->partial) return "rows of this length and number are cut and need `partial` (rumpy_distill_partial_floats)";
   return nullptr;
 }
 extern "C" int64_t rumpy_distill_partial_floats(int64_t rows, int32_t V) {
   if (rows <= 0 || V < 1 || V > DS_MAXV) return 0;
-  const DsPlan plan = ds_plan(rows, V);
+  const DsPlan plan = ds_plan(rows, V, 1.0);
   return plan.splits > 1 ? rows * plan.splits * 2 : 0;
 }
 
@@ -944,7 +963,7 @@ extern "C" int rumpy_distill_fwd(const rumpy_distill_args* p, void* stream) {
   if (bad) { rumpy_set_error("rumpy_distill_fwd: %s", bad); return RUMPY_E_ARG; }
   hipStream_t s = (hipStream_t)stream;
   if (p->rows) {
-    const DsPlan plan = ds_plan(p->rows, p->V);
+    const DsPlan plan = ds_plan(p->rows, p->V, p->tau);
     if (p->fmt == RUMPY_FMT_F32) ds_launch_fwd<RUMPY_FMT_F32>(*p, plan, s);
     else if (p->fmt == RUMPY_FMT_BF16) ds_launch_fwd<RUMPY_FMT_BF16>(*p, plan, s);
     else ds_launch_fwd<RUMPY_FMT_F16>(*p, plan, s);
@@ -957,7 +976,7 @@ extern "C" int rumpy_distill_bwd(const rumpy_distill_args* p, void* stream) {
   if (!bad && p->rows && (!p->dlogits || !p->gout)) bad = "a tensor is missing";
   if (bad) { rumpy_set_error("rumpy_distill_bwd: %s", bad); return RUMPY_E_ARG; }
   if (p->rows == 0) return RUMPY_OK;
-  const DsPlan plan = ds_plan(p->rows, p->V);
+  const DsPlan plan = ds_plan(p->rows, p->V, p->tau);
   hipStream_t s = (hipStream_t)stream;
   const dim3 grid((unsigned)(p->rows * plan.splits));
   if (p->fmt == RUMPY_FMT_F32) hipLaunchKernelGGL((distill_bwd_kernel<RUMPY_FMT_F32>), grid, dim3(DS_WG), 0, s, *p, plan);

@@ -266,16 +266,16 @@ std::pair<Tensor, optional<Tensor>> residual_norm(const Tensor& x, const optiona
 }
 
 // ================================================================================================================ distillation
-float check_logits(const char* name, const Tensor& logits, double temperature) {
+double check_logits(const char* name, const Tensor& logits, double temperature) {
   TORCH_CHECK(fmt_of(logits) >= 0, "rumpy_amd: ", name, " takes float32, bfloat16 or float16 logits, not ", name_of(logits));
   TORCH_CHECK_VALUE(logits.dim() >= 1 && logits.size(-1) >= 1 && logits.size(-1) <= MAX_COLUMNS, "rumpy_amd: ", name, " takes [..., V] logits with V >= 1, not ",
                     logits.sizes());
   TORCH_CHECK_VALUE(temperature > 1e-30 && temperature < 1e30, "rumpy_amd: ", name, " takes a temperature above zero, not ", temperature);
-  return (float)temperature;
+  return temperature;
 }
 
 std::tuple<Tensor, Tensor, Tensor> top_logits(const Tensor& logits, int64_t k, double temperature) {
-  const float tau = check_logits("top_logits", logits, temperature);
+  const double tau = check_logits("top_logits", logits, temperature);
   const int64_t v = logits.size(-1), rows = logits.numel() / v;
   TORCH_CHECK_VALUE(k >= 1 && k <= std::min(v, MAX_TOP), "rumpy_amd: top_logits takes 1 <= k <= ", MAX_TOP, " of rows of ", v, " logits, not ", k);
   need_gpu("top_logits", logits);
@@ -291,7 +291,7 @@ std::tuple<Tensor, Tensor, Tensor> top_logits(const Tensor& logits, int64_t k, d
     const Tensor work = bytes ? new_floats({(bytes + 3) / 4}, logits) : Tensor();
     rumpy_top_logits_args a{};
     a.logits = ptr(z.t); a.values = out_ptr(values); a.indices = out_ptr(indices); a.tail = out_fptr(tail); a.work = out_ptr(work);
-    a.rows = rows; a.ld = z.ld; a.V = (int32_t)v; a.k = (int32_t)k; a.fmt = fmt_of(logits); a.inv_tau = 1.f / tau;
+    a.rows = rows; a.ld = z.ld; a.V = (int32_t)v; a.k = (int32_t)k; a.fmt = fmt_of(logits); a.tau = tau;
     launch("rumpy_top_logits", lib.top, a, logits.device());
   }
   return {values, indices, tail};
@@ -301,7 +301,7 @@ enum Reduction { NONE, SUM, MEAN };
 
 // what both directions give to the kernels; state: [rows, 8], the reduction's factor, the workspace of rows that are cut, the rows' losses
 rumpy_distill_args distill_args(const Rows& z, int64_t v, const Tensor& values, const Tensor& indices, const Tensor& tail, const Tensor& weight, const Tensor& state,
-                                Reduction reduction, float tau) {
+                                Reduction reduction, double tau) {
   const int64_t rows = z.t.numel() / v;
   rumpy_distill_args a{};
   a.logits = ptr(z.t); a.top_values = ptr(values); a.top_indices = ptr(indices); a.tail = fptr(tail); a.row_weight = fptr(weight);
@@ -310,13 +310,13 @@ rumpy_distill_args distill_args(const Rows& z, int64_t v, const Tensor& values, 
   a.partial = pf ? a.factor + 1 : nullptr;
   a.row_loss = a.factor + 1 + pf;
   a.rows = rows; a.ld = z.ld; a.V = (int32_t)v; a.k = (int32_t)values.size(-1); a.fmt = fmt_of(z.t); a.value_fmt = fmt_of(values);
-  a.index64 = indices.scalar_type() == at::kLong; a.mean = reduction == MEAN; a.tau = tau; a.inv_tau = 1.f / tau;
+  a.index64 = indices.scalar_type() == at::kLong; a.mean = reduction == MEAN; a.tau = tau;
   return a;
 }
 
 struct DistillBackward : public torch::autograd::Node {
   Reduction reduction;
-  float tau;
+  double tau;
   SavedVariable logits_, values_, indices_, tail_, weight_;
   Tensor state_;
   std::string name() const override { return "DistillBackward"; }
@@ -347,7 +347,7 @@ struct DistillBackward : public torch::autograd::Node {
 
 Tensor distill_loss(const Tensor& logits, const Tensor& top_values, const Tensor& top_indices, const optional<Tensor>& tail_, double temperature,
                     const optional<Tensor>& weight_, const std::string& reduction_) {
-  const float tau = check_logits("distill_loss", logits, temperature);
+  const double tau = check_logits("distill_loss", logits, temperature);
   TORCH_CHECK_VALUE(reduction_ == "mean" || reduction_ == "sum" || reduction_ == "none", "rumpy_amd: distill_loss reduces by 'mean', 'sum' or 'none', not '", reduction_, "'");
   const Reduction reduction = reduction_ == "mean" ? MEAN : reduction_ == "sum" ? SUM : NONE;
   const auto lead = logits.sizes().slice(0, logits.dim() - 1);

@@ -150,8 +150,11 @@ def test_offsets_beyond_32_bits():
     z.copy_(torch.randn(3, cols, generator=g).to(BF16))
     _check_top(z, 20, 1.0)
     values, indices, tail = top_logits(z, 20)
-    near = z.clone()
-    assert torch.equal(distill_loss(z, values, indices, tail=tail, reduction='none'), distill_loss(near, values, indices, tail=tail, reduction='none'))
+    # (the order of a row's sum goes with the alignment of its address: not the same bits as for a copy of the rows)
+    got = distill_loss(z, values, indices, tail=tail, reduction='none').double().cpu()
+    one = torch.ones(3, dtype=torch.float64)
+    loss, _, _, err, _ = _loss_reference(z.cpu(), values.cpu(), indices.cpu(), tail.cpu(), 1.0, one, one)
+    assert ((got - loss).abs() <= 3 * err).all()
 
 
 # ---------------------------------------------------------------------------------------------------------------- distill_loss

@@ -78,24 +78,24 @@ def test_norm_backward_entry_point_refuses(bad):
     assert b'rumpy_residual_norm_bwd' in lib.rumpy_last_error()
 
 
-@pytest.mark.parametrize('bad', [dict(k=0), dict(k=257), dict(V=9, k=10), dict(V=0), dict(V=2 ** 30 + 1), dict(rows=-1), dict(ld=-1), dict(fmt=2), dict(inv_tau=0.0),
-                                 dict(inv_tau=float('inf')), dict(inv_tau=float('nan')), dict(logits=None), dict(values=None), dict(indices=None), dict(tail=None),
+@pytest.mark.parametrize('bad', [dict(k=0), dict(k=257), dict(V=9, k=10), dict(V=0), dict(V=2 ** 30 + 1), dict(rows=-1), dict(ld=-1), dict(fmt=2), dict(tau=0.0),
+                                 dict(tau=float('inf')), dict(tau=float('nan')), dict(logits=None), dict(values=None), dict(indices=None), dict(tail=None),
                                  dict(V=200000, rows=1), dict(V=200000, rows=1, work=P + 4), dict(rows=2 ** 31)], ids=str)
 def test_top_logits_entry_point_refuses(bad):
     lib = _lib_or_skip()
-    d = dict(logits=P, values=P, indices=P, tail=P, rows=3, ld=500, V=500, k=10, fmt=L.FMT_F32, inv_tau=1.0)
+    d = dict(logits=P, values=P, indices=P, tail=P, rows=3, ld=500, V=500, k=10, fmt=L.FMT_F32, tau=1.0)
     d.update(bad)
     assert lib.rumpy_top_logits(ctypes.byref(L.TopLogitsArgs(**d)), None) == E_ARG
     assert b'rumpy_top_logits' in lib.rumpy_last_error()
 
 
 @pytest.mark.parametrize('bad', [dict(k=0), dict(k=257), dict(V=0), dict(V=2 ** 30 + 1), dict(rows=-1), dict(ld=-1), dict(fmt=2), dict(value_fmt=5), dict(tau=0.0),
-                                 dict(tau=float('nan')), dict(inv_tau=-1.0), dict(logits=None), dict(top_values=None), dict(top_indices=None), dict(row_loss=None),
+                                 dict(tau=float('nan')), dict(tau=-1.0), dict(logits=None), dict(top_values=None), dict(top_indices=None), dict(row_loss=None),
                                  dict(state=None), dict(factor=None), dict(V=200000, partial=None), dict(rows=2 ** 32)], ids=str)
 def test_distill_entry_points_refuse(bad):
     lib = _lib_or_skip()
     d = dict(logits=P, top_values=P, top_indices=P, row_loss=P, state=P, loss=P, factor=P, partial=P, gout=P, dlogits=P, rows=3, ld=500, V=500, k=10, fmt=L.FMT_F32,
-             value_fmt=L.FMT_F32, index64=1, mean=1, tau=1.0, inv_tau=1.0)
+             value_fmt=L.FMT_F32, index64=1, mean=1, tau=1.0)
     d.update(bad)
     for name in ('rumpy_distill_fwd', 'rumpy_distill_bwd'):
         assert getattr(lib, name)(ctypes.byref(L.DistillArgs(**d)), None) == E_ARG
