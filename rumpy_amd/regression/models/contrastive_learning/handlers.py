@@ -48,6 +48,8 @@ def _graphed_step(handler, forward_backward, inputs, dev):
     key = tuple((tuple(t.shape), t.dtype) for t in inputs) + (net.flat_p.data_ptr(), net.encoder_k.flat_p.data_ptr(), net.queue.data_ptr(),
                                                                net.queue_ptr.data_ptr()) + \
         tuple(getattr(net, n).data_ptr() for n in ('queue_labels', 'queue_vectors') if getattr(net, n, None) is not None)
+    if getattr(net, 'distill_top', None) is not None:           # numbers that the capture holds: another weight or temperature is another step
+        key += (net.distill_top, net.distill_t, handler.distill_weight)
     # ... and plan buffers of both trunks (z / a / dz / da, BatchNorm partials): when an encoder has dropped cached plans since, every captured
     # step may point into freed memory - all of them go (the next two calls of a shape run eagerly and rebuild what they need)
     ev = (net.encoder_q._evictions, net.encoder_k._evictions)
@@ -65,6 +67,7 @@ def _graphed_step(handler, forward_backward, inputs, dev):
         with torch.cuda.graph(g):
             st['loss'], st['out'] = forward_backward(*st['in'], dev)
         st['graph'] = g
+        st['targets'] = getattr(net, 'distill_targets', None)
         st['n_keys'] = handler.net.__dict__['_slot_state'][0]
         # capture does not execute: what the host-side bookkeeping recorded during it is taken back, the replay below redoes it
         handler.net._moved(-st['n_keys'])
@@ -72,6 +75,8 @@ def _graphed_step(handler, forward_backward, inputs, dev):
     for buf, t in zip(st['in'], inputs):
         buf.copy_(t)
     st['graph'].replay()
+    if st['targets'] is not None:
+        net.distill_targets = st['targets']                     # (of this batch shape's capture: the replay has filled them anew)
     handler.net._moved(st['n_keys'])
     handler.net.encoder_q._stats_epoch += 1
     handler.net.encoder_k._stats_epoch += 1

@@ -36,6 +36,8 @@ class MoCo(nn.Module):
         self.positives = positives
         if distill_top is not None and not 1 <= distill_top <= min(K, 256):
             raise ValueError('rumpy_amd: distill_top is 1 .. 256 of the %d queue entries, not %r' % (K, distill_top))
+        if distill_top is not None and not 0.0 < distill_t < float('inf'):
+            raise ValueError('rumpy_amd: distill_t is a temperature above zero, not %r' % (distill_t,))
         self.distill_top, self.distill_t = distill_top, distill_t
         self.distill_targets = None
         self.encoder_q = base_encoder(dropdown)

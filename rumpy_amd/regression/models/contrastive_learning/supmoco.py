@@ -13,6 +13,8 @@ from .moco import MoCo
 class SupMoCo(MoCo):
     def __init__(self, device, positives_per_class=4, contrastive_dropdown=True, **kwargs):
         super(SupMoCo, self).__init__(**kwargs)
+        if self.distill_top is not None:
+            raise ValueError('rumpy_amd: %s makes no distillation targets: distill_top is MoCo\'s alone' % type(self).__name__)
         self.num_classes = 0
         self.positives_per_class = positives_per_class
         self.device = device

@@ -165,3 +165,24 @@ def test_a_student_of_residual_blocks_learns_from_a_teacher(dtype):
     assert abs(float(got_loss.detach()) - float(ref_loss.detach())) <= tol * max(1.0, float(ref_loss.detach()))
     for n, (a, b) in enumerate(zip(got, ref)):
         assert float((a.double().cpu() - b).norm()) <= tol * float(b.norm()) + 1e-9, n
+
+
+def test_captured_steps_of_two_batch_shapes_and_a_changed_weight(monkeypatch):
+    """a replayed step leaves its own batch's targets, and a weight that is changed between the steps counts from the next step on"""
+    def loss_of(h, step, n):
+        loss, logits = h.run_train(x=CO.contrastive_batch(900 + step, n, 2).view(n, 6, 32, 32), y=None)
+        return float(loss), logits.clone(), [t.clone() for t in h.net.distill_targets]
+    plan = [(8, 0.5)] * 4 + [(4, 0.5)] * 4 + [(8, 0.5), (4, 0.5), (8, 2.0), (4, 2.0), (8, 2.0), (8, 2.0), (8, 0.5)]
+    res = []
+    for eager in ('0', '1'):
+        monkeypatch.setenv('RUMPY_MOCO_STEP_GRAPH', eager)
+        h = _handler(78, distill_top=16)
+        out = []
+        for step, (n, weight) in enumerate(plan):
+            h.distill_weight = weight
+            out.append(loss_of(h, step, n))
+        res.append(out)
+    assert sum('graph' in st for st in h._step_graphs.values()) == 3
+    for step, (a, b) in enumerate(zip(*res)):
+        assert a[0] == b[0] and torch.equal(a[1], b[1]), step
+        assert a[2][0].shape[0] == plan[step][0] and all(torch.equal(s, t) for s, t in zip(a[2], b[2])), step

@@ -181,3 +181,16 @@ def test_binding_is_loaded_once_and_missing_parts_are_loud(monkeypatch):
     monkeypatch.setitem(sys.modules, 'rumpy_amd._torch_bind', None)         # as if it were not built
     with pytest.raises(RuntimeError, match='no fallback'):
         residual_norm(torch.zeros(2, 8), pre_norm='rms')
+
+
+def test_contrastive_models_refuse_targets_they_do_not_make():
+    from rumpy_amd.regression.models.contrastive_learning.encoding_models import Encoder
+    from rumpy_amd.regression.models.contrastive_learning.moco import MoCo
+    from rumpy_amd.regression.models.contrastive_learning.supmoco import SupMoCo
+    from rumpy_amd.regression.models.contrastive_learning.weak_con import WeakCon
+    for kw in ({'distill_top': 0}, {'distill_top': 65}, {'distill_top': 8, 'distill_t': 0.0}, {'distill_top': 8, 'distill_t': float('nan')}):
+        with pytest.raises(ValueError, match='distill_t'):
+            MoCo(base_encoder=Encoder, K=64, **kw)
+    for kind in (SupMoCo, WeakCon):
+        with pytest.raises(ValueError, match='%s makes no distillation targets' % kind.__name__):
+            kind(device='cpu', base_encoder=Encoder, K=64, distill_top=8)
