@@ -461,3 +461,66 @@ def test_no_second_derivative():
     loss = distill_loss(z, *top_logits(z.detach(), 4)[:2])
     with pytest.raises(RuntimeError, match='second derivative'):
         torch.autograd.grad(loss, z, create_graph=True)
+
+
+def test_more_than_2_31_elements():
+    """rows do not know of each other: those at the end of a large tensor are the rows of a small call (of as many whole workgroups a row), bit for bit"""
+    rows, cols, k = 20000, 131072, 40                              # 2.6e9 elements
+    g = torch.Generator(device=DEV).manual_seed(23)
+    z = torch.randn((rows, cols), generator=g, device=DEV, dtype=BF16)
+    pick = torch.cat([torch.arange(0, 400), torch.arange(16300, 16484), torch.arange(rows - 100, rows)]).to(DEV)          # more rows than are cut
+    res = []
+    for some in (None, pick):
+        zs = z if some is None else z[some]
+        values, indices, tail = top_logits(zs, k)
+        leaf = zs.detach().requires_grad_()
+        loss = distill_loss(leaf, values * 0.5, indices, tail=tail, reduction='none')
+        grad, = torch.autograd.grad(loss, leaf, torch.ones_like(loss))
+        res.append([v if some is not None else v[pick] for v in (values, indices, tail, loss.detach(), grad)])
+        del grad, loss, leaf
+    assert all(torch.equal(a, b) for a, b in zip(*res))
+
+
+def test_modes_around_the_call():
+    z, t = torch.randn(4, 300, device=DEV), torch.randn(4, 300, device=DEV)
+    with torch.inference_mode():
+        values, indices, tail = top_logits(t, 5)
+        a = distill_loss(z, values, indices, tail=tail)
+    values, indices, tail = top_logits(t, 5)
+    leaf = z.clone().requires_grad_()
+    b = distill_loss(leaf, values, indices, tail=tail)
+    assert torch.equal(a, b.detach()) and not a.requires_grad
+    b.backward()
+    with pytest.raises(RuntimeError, match='second time'):
+        b.backward()
+    c = distill_loss(leaf, values, indices, tail=tail)
+    values.mul_(2.0)                                                # a saved tensor is changed before the backward pass
+    with pytest.raises(RuntimeError, match='modified by an inplace operation'):
+        c.backward()
+    weight = torch.tensor([True, False, True, True], device=DEV)
+    d = distill_loss(z, values, indices, row_weight=weight)
+    assert torch.equal(d, distill_loss(z, values, indices, row_weight=weight.float()))
+
+
+def test_two_graphs_at_once_share_nothing():
+    """two captured calls, replayed on two streams at the same time"""
+    g = torch.Generator().manual_seed(25)
+    zs = [torch.randn(3, 100000, generator=g).to(DEV) for _ in range(2)]
+    graphs, outs = [], []
+    for z in zs:
+        _pass(z, z, 20, 1.0)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append(_pass(z, z.flip(0), 20, 1.0))
+        graphs.append(graph)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for i in range(4):
+        for z in zs:
+            z.copy_(torch.randn(3, 100000, generator=g))
+        torch.cuda.synchronize()
+        for s, graph in zip(streams, graphs):
+            with torch.cuda.stream(s):
+                graph.replay()
+        torch.cuda.synchronize()
+        for z, out in zip(zs, outs):
+            assert all(torch.equal(a, b) for a, b in zip(out, _pass(z, z.flip(0), 20, 1.0)))

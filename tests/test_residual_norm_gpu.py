@@ -9,6 +9,7 @@ import itertools
 
 import pytest
 import torch
+import torch.utils.checkpoint
 
 from rumpy_amd.residual_norm import ResidualNorm, residual_norm
 
@@ -429,3 +430,90 @@ def test_no_second_derivative():
     y, h = residual_norm(x, t, post_norm='rms', pre_norm='rms')
     with pytest.raises(RuntimeError, match='second derivative'):
         torch.autograd.grad(y.sum() + h.sum(), [x, t], create_graph=True)
+
+
+def test_more_than_2_31_elements():
+    """rows do not know of each other: those at the end of a large tensor are the rows of a small call, bit for bit"""
+    rows, c = 300000, 8192                                        # 2.4e9 elements
+    g = torch.Generator(device=DEV).manual_seed(21)
+    x, t = (torch.randn((rows, c), generator=g, device=DEV, dtype=BF16) for _ in range(2))
+    pick = torch.tensor([0, 1, 131071, 262143, 262144, 299998, 299999], device=DEV)
+    res = []
+    for some in (None, pick):
+        xs, ts = (v if some is None else v[some] for v in (x, t))
+        xs, ts = xs.detach().requires_grad_(), ts.detach().requires_grad_()
+        y, h = residual_norm(xs, ts, scale=0.3, post_norm='rms', pre_norm='layer')
+        dx, dt = torch.autograd.grad([y, h], [xs, ts], [xs.detach(), ts.detach()])
+        res.append([v if some is not None else v[pick] for v in (y.detach(), h.detach(), dx, dt)])
+        del y, h, dx, dt
+    assert all(torch.equal(a, b) for a, b in zip(*res))
+
+
+def test_one_tensor_in_several_places():
+    """x as the branch and as its own gate: the gradients of all places come together"""
+    g = torch.Generator().manual_seed(22)
+    v, dy, dh = (torch.randn(5, 130, generator=g) for _ in range(3))
+    d = v.to(DEV).requires_grad_()
+    y, h = residual_norm(d, d, gate=d, scale=0.5, post_norm='layer', pre_norm='rms')
+    got, = torch.autograd.grad([y, h], d, [dy.to(DEV), dh.to(DEV)])
+    ref = _reference(v.double(), v.double(), v.double(), None, 0.5, 'layer', None, None, 'rms', None, None, dy.double(), dh.double())
+    _check('y', y, ref['y'], F32)
+    parts = [ref[n] for n in ('d_x', 'd_branch', 'd_gate')]
+    _check('gradient', got, (sum(p[0] for p in parts), sum(p[1] for p in parts), 3), F32)
+
+
+def test_modes_around_the_call():
+    """inference mode, checkpointing, accumulation into .grad by backward(), a graph that is freed"""
+    x, t = torch.randn(6, 72, device=DEV), torch.randn(6, 72, device=DEV)
+    w = torch.ones(72, device=DEV, requires_grad=True)
+    with torch.inference_mode():
+        y0, h0 = residual_norm(x, t, post_norm='rms', post_weight=w, pre_norm='rms')
+    y, h = residual_norm(x, t, post_norm='rms', post_weight=w, pre_norm='rms')
+    assert torch.equal(y, y0) and torch.equal(h, h0) and not y0.requires_grad and y.requires_grad
+    (y.sum() + h.sum()).backward()
+    once = w.grad.clone()
+    with pytest.raises(RuntimeError, match='second time'):
+        y.sum().backward()
+    out = torch.utils.checkpoint.checkpoint(lambda a: sum(v.sum() for v in residual_norm(x, t, post_norm='rms', post_weight=a, pre_norm='rms')), w, use_reentrant=False)
+    out.backward()
+    assert torch.equal(w.grad, 2 * once)
+    y, h = residual_norm(x, t, post_norm='rms', post_weight=w, pre_norm='rms')
+    t.add_(1.0)                                                   # a saved tensor is changed before the backward pass
+    with pytest.raises(RuntimeError, match='modified by an inplace operation'):
+        h.sum().backward()
+    with pytest.raises(RuntimeError, match='forward-mode'):
+        with torch.autograd.forward_ad.dual_level():
+            residual_norm(torch.autograd.forward_ad.make_dual(x, x), t, pre_norm='rms')
+
+
+def test_captured_backward_accumulates_into_grad():
+    """a whole step - forward, loss, backward() into .grad - as one graph, replayed with other inputs and eager steps of other tensors in between"""
+    torch.manual_seed(5)
+    m = ResidualNorm(64, scale=0.5, post_norm='layer', pre_norm='layer', channel_scale=0.3).to(DEV)
+    x, t = torch.randn(40, 64, device=DEV), torch.randn(40, 64, device=DEV)
+
+    def step(m, x, t):
+        for p in m.parameters():
+            p.grad.zero_()
+        y, h = m(x, t)
+        (y.square().sum() + (h * x).sum()).backward()
+    for p in m.parameters():
+        p.grad = torch.zeros_like(p)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        step(m, x, t)
+    torch.cuda.current_stream().wait_stream(s)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step(m, x, t)
+    other = ResidualNorm(64, scale=0.5, post_norm='layer', pre_norm='layer', channel_scale=0.3).to(DEV)
+    other.load_state_dict(m.state_dict())
+    for p in other.parameters():
+        p.grad = torch.zeros_like(p)
+    for i in range(3):
+        t.copy_(torch.randn(40, 64) * (i + 1))
+        graph.replay()
+        torch.cuda.synchronize()
+        step(other, x, t)
+        assert all(torch.equal(a.grad, b.grad) for a, b in zip(m.parameters(), other.parameters()))
