@@ -49,17 +49,18 @@ template <int TPR> struct RowSum {
 
 // Where a lane's 8 channels lie.  The last piece of a row is moved back to end with the row, and lanes behind it repeat it: every access is one
 // whole 16- or 32-byte access inside the row, with no branch around it.  What two lanes both hold they compute and store alike; in a row's sums
-// the repeated elements (the first `lo` of a lane) count zero times (`m`).  Rows of less than 8 channels have one lane (TPR 1) and partial accesses.
+// the repeated elements count zero times (`m`, bits and not factors: an infinity is not made NaN).  Rows of less than 8 channels have one lane (TPR 1) and partial accesses.
 template <int TPR> struct RnLane {
   int at, n;             // first channel; channels of a partial access (TPR 1)
-  float m[8];
+  uint32_t m[8];
   __device__ __forceinline__ explicit RnLane(int C) {
     const int col = ((int)threadIdx.x % TPR) * 8;
     at = TPR == 1 ? 0 : min(col, C - 8);
     n = TPR == 1 ? C : 8;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) m[i] = (TPR == 1 ? i < C : i >= col - at) ? 1.f : 0.f;
+    for (int i = 0; i < 8; ++i) m[i] = (TPR == 1 ? i < C : i >= col - at) ? 0xffffffffu : 0u;
   }
+  __device__ __forceinline__ float once(float v, int i) const { return __uint_as_float(__float_as_uint(v) & m[i]); }
   template <int FMT> __device__ __forceinline__ RowRaw<FMT> load(const void* base, size_t row_off) const {
     return load_piece<FMT>((const typename RowElem<FMT>::type*)base + row_off + at, TPR == 1 ? n : 8, 0.f);
   }
@@ -78,18 +79,18 @@ template <int TPR> struct RnLane {
 
 // mean and 1 / sqrt(var + eps) of a row.  The variance is taken around the mean in a second sum (the row is in registers): no cancellation
 // where the mean is large.  v_rsq_f32 is right to one unit in the last place for normal arguments (eps is one).
-template <int TPR> __device__ __forceinline__ void row_stats(RowSum<TPR>& sum, const float (&v)[8], const float (&m)[8], int kind, float inv_c, float eps,
+template <int TPR> __device__ __forceinline__ void row_stats(RowSum<TPR>& sum, const float (&v)[8], const RnLane<TPR>& lane, int kind, float inv_c, float eps,
                                                              float& mu, float& rs) {
   mu = 0.f;
   if (kind == RN_LAYER) {
     float s = 0.f;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) s = fmaf(v[i], m[i], s);
+    for (int i = 0; i < 8; ++i) s += lane.once(v[i], i);
     mu = sum.one(s) * inv_c;
   }
   float q = 0.f;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) { const float d = (v[i] - mu) * m[i]; q = fmaf(d, d, q); }
+  for (int i = 0; i < 8; ++i) { const float d = lane.once(v[i] - mu, i); q = fmaf(d, d, q); }
   rs = __builtin_amdgcn_rsqf(sum.one(q) * inv_c + eps);
 }
 
@@ -154,13 +155,13 @@ template <int XF, int TF, int TPR, int MODE> __global__ void __launch_bounds__(T
     ask(more ? rb + step : rb);
     float4 st = make_float4(0.f, 1.f, 0.f, 1.f);
     if (has_t) {
-      if (a.post != RN_NONE) row_stats<TPR>(sum, t, lane.m, a.post, inv_c, a.eps, st.x, st.y);
+      if (a.post != RN_NONE) row_stats<TPR>(sum, t, lane, a.post, inv_c, a.eps, st.x, st.y);
 #pragma unroll
       for (int i = 0; i < 8; ++i) x[i] = fmaf(a.scale * g[i], fmaf((t[i] - st.x) * st.y, wp[i], bp[i]), x[i]);
       lane.template store<XF>(a.y, r * a.C, x);
     }
     if (has_pre) {
-      row_stats<TPR>(sum, x, lane.m, a.pre, inv_c, a.eps, st.z, st.w);
+      row_stats<TPR>(sum, x, lane, a.pre, inv_c, a.eps, st.z, st.w);
 #pragma unroll
       for (int i = 0; i < 8; ++i) x[i] = fmaf((x[i] - st.z) * st.w, w[i], b[i]);
       lane.template store<TF>(a.h, r * a.C, x);
@@ -175,7 +176,7 @@ template <int XF, int TF, int TPR, int MODE> __global__ void __launch_bounds__(T
 // ---- backward ----
 // Work of one launch: `wgs` workgroups of `rpw` contiguous rows each.  A gate row that serves a group of rows is summed over a workgroup's part
 // of the group and stored as partial row (workgroup + group): over the walk of all (workgroup, group) pairs that number grows strictly.  Groups
-// shorter than a workgroup's step store one partial row per row instead.
+// shorter than a workgroup's step store one partial row per row instead (groups of one row: the gradient itself).
 struct RnPlan { int tpr, sub, wgs, rpw; bool direct; };
 static RnPlan rn_plan(int64_t rows, int64_t group_rows, int32_t C, int gate_mode) {
   RnPlan p;
@@ -189,7 +190,7 @@ static RnPlan rn_plan(int64_t rows, int64_t group_rows, int32_t C, int gate_mode
   if (wgs > most) wgs = most;
   p.rpw = (int)((steps + wgs - 1) / wgs * p.sub);
   p.wgs = (int)((rows + p.rpw - 1) / p.rpw);
-  p.direct = gate_mode == RN_GATE_GROUP && group_rows < p.sub;
+  p.direct = gate_mode == RN_GATE_GROUP && (group_rows < p.sub || group_rows == 1);
   return p;
 }
 
@@ -242,7 +243,8 @@ template <int XF, int TF, int TPR, int MODE> __global__ void __launch_bounds__(T
   const int sub = (int)threadIdx.x / TPR;
   const float inv_c = 1.f / (float)a.C;
   const uint32_t rows = (uint32_t)a.rows, r0 = min(rows, blockIdx.x * (uint32_t)plan.rpw), r1 = min(rows, r0 + (uint32_t)plan.rpw);
-  float* gpart = a.partial + (size_t)4 * plan.wgs * a.C;               // partial: [4][wgs][C], then the gate's partial rows
+  // partial: [4][wgs][C], then the gate's partial rows
+  float* gpart = plan.direct && a.group_rows == 1 ? (float*)a.dgate : a.partial + (size_t)4 * plan.wgs * a.C;
   const bool has_t = MODE != RN_ANY || a.t, has_dy = MODE != RN_ANY || a.dy, has_dh = MODE != RN_ANY || a.dh;
   const bool full = MODE == RN_ALL_FULL || (MODE == RN_ANY && a.gate_mode == RN_GATE_FULL);
   const bool direct = MODE != RN_ALL_FULL && plan.direct, group_sums = MODE != RN_ALL_FULL && a.gate_mode == RN_GATE_GROUP && !plan.direct;
@@ -298,7 +300,7 @@ template <int XF, int TF, int TPR, int MODE> __global__ void __launch_bounds__(T
         ab[i] += ea;
         aw[i] = fmaf(ea, x[i], aw[i]);
         e[i] *= w[i];
-        const float em = e[i] * lane.m[i];
+        const float em = lane.once(e[i], i);
         s1 += em;
         s2 = fmaf(em, x[i], s2);
       }
@@ -320,7 +322,7 @@ template <int XF, int TF, int TPR, int MODE> __global__ void __launch_bounds__(T
         const float dz = g[i] * dd;
         if (!TAIL || live) { ag[i] += gr[i]; abp[i] += dz; awp[i] = fmaf(dz, t[i], awp[i]); }
         d[i] = dz * wp[i];
-        const float dm = d[i] * lane.m[i];
+        const float dm = lane.once(d[i], i);
         s1 += dm;
         s2 = fmaf(dm, t[i], s2);
       }
@@ -494,7 +496,7 @@ extern "C" int64_t rumpy_residual_norm_partial_floats(int64_t rows, int64_t grou
   if (rows <= 0 || C < 1 || C > RN_MAXC || (gate_mode == RN_GATE_GROUP && group_rows < 1)) return 0;
   const RnPlan plan = rn_plan(rows, group_rows, C, gate_mode);
   int64_t n = (int64_t)4 * plan.wgs;
-  if (gate_mode == RN_GATE_GROUP) n += plan.direct ? rows : plan.wgs + (rows + group_rows - 1) / group_rows;
+  if (gate_mode == RN_GATE_GROUP) n += plan.direct ? (group_rows == 1 ? 0 : rows) : plan.wgs + (rows + group_rows - 1) / group_rows;
   return n * C;
 }
 
@@ -509,12 +511,12 @@ extern "C" int rumpy_residual_norm_bwd(const rumpy_residual_norm_bwd_args* p, vo
   if (!bad && (!p->t && (p->dt || p->dgate || p->d_post_w || p->d_post_b))) bad = "a gradient of a branch that is not there";
   if (!bad && (p->gate_mode == RN_GATE_NONE && p->dgate)) bad = "a gradient of a gate that is not there";
   if (!bad && ((p->post == RN_NONE && (p->d_post_w || p->d_post_b)) || (!p->dh && (p->d_pre_w || p->d_pre_b)))) bad = "a gradient of a norm that is not there";
-  const bool gate_rows = !bad && p->gate_mode == RN_GATE_GROUP && p->dgate;
+  const RnPlan plan = bad ? RnPlan{} : rn_plan(p->rows, p->group_rows, p->C, p->gate_mode);
+  const bool gate_rows = !bad && p->gate_mode == RN_GATE_GROUP && p->dgate && !(plan.direct && p->group_rows == 1);
   const int tiles = bad ? 0 : (p->C + 63) / 64;
   const int64_t items = 4 + (gate_rows ? p->rows / p->group_rows : 0);
   if (!bad && items * tiles > 0x7fffffff) bad = "too many gate rows";
   if (bad) { rumpy_set_error("rumpy_residual_norm_bwd: %s", bad); return RUMPY_E_ARG; }
-  const RnPlan plan = rn_plan(p->rows, p->group_rows, p->C, p->gate_mode);
   hipStream_t s = (hipStream_t)stream;
   RN_BY_FORMAT(rn_launch_bwd, *p, plan, s);
   if (gate_rows || p->d_post_w || p->d_post_b || p->d_pre_w || p->d_pre_b)

@@ -517,3 +517,36 @@ def test_captured_backward_accumulates_into_grad():
         torch.cuda.synchronize()
         step(other, x, t)
         assert all(torch.equal(a.grad, b.grad) for a, b in zip(m.parameters(), other.parameters()))
+
+
+@pytest.mark.parametrize('shape', [(1, 64), (37, 5), (301, 72), (1000, 64), (33, 700), (21, 1032), (3, 8192)])
+def test_gate_row_for_every_row(shape):
+    """a float32 gate beside 16-bit rows: each gate row serves one row, and its gradient is stored, not summed"""
+    _run_and_check(shape, BF16, BF16, 'group', 'layer', 'rms', True, 0.7)
+    _run_and_check(shape, F32, F16, 'group', None, 'layer', False, 0.7, with_dy=False)
+
+
+@pytest.mark.parametrize('c', [5, 64, 72, 130, 1000, 4104])
+@pytest.mark.parametrize('kind', ['layer', 'rms'])
+def test_an_infinity_in_a_row_stays_in_it(kind, c):
+    """(v - mean) / sqrt(var + eps) of a row with one infinity: 'rms' has 0 beside NaN, 'layer' NaN alone, at every row length; other rows as without it"""
+    g = torch.Generator().manual_seed(c)
+    x, t = torch.randn(6, c, generator=g), torch.randn(6, c, generator=g)
+    clean = residual_norm(x.to(DEV), t.to(DEV), post_norm=kind, pre_norm=kind)
+    alone = residual_norm(x.to(DEV), pre_norm=kind)[1]
+    x2, t2 = x.clone(), t.clone()
+    x2[1, c - 1] = float('inf')
+    t2[4, 0] = -float('inf')
+    want = torch.full((c,), float('nan')) if kind == 'layer' else torch.zeros(c)
+    keep = torch.tensor([0, 2, 3, 5])
+    h = residual_norm(x2.to(DEV), pre_norm=kind)[1]
+    last, first = want.clone(), want.clone()
+    last[-1] = first[0] = float('nan')
+    assert torch.equal(h[1].cpu().isnan(), last.isnan()) and float(h[1].cpu().nan_to_num().abs().max()) == 0.0
+    y2, h2 = residual_norm(x.to(DEV), t2.to(DEV), post_norm=kind, pre_norm=kind)
+    assert torch.equal(y2[4].cpu().isnan(), first.isnan()) and bool(h2[4].isnan().all())
+    if kind == 'rms':
+        assert torch.equal(y2[4, 1:].cpu(), x[4, 1:])                     # N_post is 0 there
+    for a, b in ((y2, clean[0]), (h2, clean[1])):
+        assert torch.equal(a[[0, 1, 2, 3, 5]], b[[0, 1, 2, 3, 5]])
+    assert torch.equal(h[keep], alone[keep])
