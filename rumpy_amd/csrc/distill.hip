@@ -569,13 +569,15 @@ constexpr int DS_STATE = 8;      // per row: reference and coefficient of the st
 
 // exp((v - m) / tau) with c + lo = log2(e) / tau: c alone, rounded to 32 bits, is another temperature for the whole row, and its error of up to 2^-25
 // does not average out in the loss (1.8e-6 of it where 32-bit divisions made 2e-7).  Two fused multiply-adds per element; they need m c finite: a
-// type's lowest value (a mask) overflows there, and takes the difference first.  fl(m c) is off m (c + lo), ds_off says how much (in powers of two).
+// type's lowest value (a mask) overflows there, and takes the difference first.  The large product meets fl(m c) first: the other way round its last
+// digits are gone, for the whole row, where the logits lie far from zero (2^-25 of m c: 5e-5 at logits of 60 and a temperature of 0.07).  fl(m c) is off m (c + lo), ds_off says how much (in powers of two).
 __device__ __forceinline__ float ds_exp(float v, float m, float c, float lo, float mc) {
-  return __builtin_amdgcn_exp2f(fabsf(mc) < INFINITY ? fmaf(v, c, fmaf(v, lo, -mc)) : (v - m) * c);
+  return __builtin_amdgcn_exp2f(fabsf(mc) < INFINITY ? fmaf(v, lo, fmaf(v, c, -mc)) : (v - m) * c);
 }
 __device__ __forceinline__ float ds_off(float m, float c, float lo) { const float mc = m * c; return fabsf(mc) < INFINITY ? fmaf(m, lo, fmaf(m, c, -mc)) : 0.f; }
-// the factor from a sum relative to m to one relative to M >= m.  Where a product overflows, different values are so far apart that it is 0.
+// the factor from a sum relative to fl(m c) to one relative to fl(M c), M >= m.  Where a product overflows, different values are so far apart that it is 0.
 __device__ __forceinline__ float ds_rescale(float m, float M, float c) {
+#pragma clang fp contract(off)                       // (both products rounded, as the sums have them)
   if (m == M) return 1.f;
   const float d = m * c - M * c;
   return m == -INFINITY || d != d ? 0.f : __builtin_amdgcn_exp2f(d);
@@ -772,7 +774,7 @@ template <int FMT, bool REST> __global__ void __launch_bounds__(DS_WG) distill_f
 #pragma unroll
       for (int u = 0; u < N; ++u)
 #pragma unroll
-        for (int i = 0; i < 8; ++i) s += __builtin_amdgcn_exp2f(fmaf(v[u][i], c, fmaf(v[u][i], lo, -mc)));
+        for (int i = 0; i < 8; ++i) s += __builtin_amdgcn_exp2f(fmaf(v[u][i], lo, fmaf(v[u][i], c, -mc)));
     } else {
 #pragma unroll
       for (int u = 0; u < N; ++u)

@@ -524,3 +524,17 @@ def test_two_graphs_at_once_share_nothing():
         torch.cuda.synchronize()
         for z, out in zip(zs, outs):
             assert all(torch.equal(a, b) for a, b in zip(out, _pass(z, z.flip(0), 20, 1.0)))
+
+
+@pytest.mark.parametrize('dtype', [F32, BF16, F16], ids=str)
+@pytest.mark.parametrize('rest', [False, True])
+@pytest.mark.parametrize('cols', [2, 25, 660, 9000, 70001])
+def test_logits_far_from_zero_at_a_small_temperature(cols, rest, dtype):
+    """the loss depends on differences: a row that is moved as a whole loses no digits (constant, close together, rising by thousands of widths)"""
+    g = torch.Generator().manual_seed(cols)
+    k = min(cols, 17)
+    z = torch.stack([torch.full((cols,), -60.0), torch.full((cols,), 60.0), -60.0 + 0.1 * torch.randn(cols, generator=g), 91.7 + 0.1 * torch.randn(cols, generator=g),
+                     torch.linspace(-60.5, -59.5, cols), torch.linspace(61.0, 60.0, cols)]).to(dtype)
+    for tau in (0.07, 0.3):
+        values, indices, tail = _teacher(z, k, tau, rest, g)
+        _check_loss(z, values, indices, tail, tau)
