@@ -670,8 +670,10 @@ __device__ __forceinline__ void ds_finish(const rumpy_distill_args& a, const DsP
     return;
   }
   // the teacher's logarithms relative to its largest logit, so that far from zero no digits are lost: lp = (v - vm) / tau - up - ln_p
-  if (vm == -INFINITY) vm = 0.f;
-  const double tr = tl - vm * inv_tau, up = tr > 0.0 ? tr : 0.0;
+  // (up: the tail where it is the larger, or all there is)
+  const bool tail_alone = vm == -INFINITY;
+  if (tail_alone) vm = 0.f;
+  const double tr = tl - vm * inv_tau, up = tr > 0.0 || tail_alone ? tr : 0.0;
   const float M = rest ? fmaxf(m, zm) : m, Mc = M * c;
   float p_sum = 0.f, sl = 0.f;
   for (int i = lane; i < a.k; i += 64) {

@@ -538,3 +538,18 @@ def test_logits_far_from_zero_at_a_small_temperature(cols, rest, dtype):
     for tau in (0.07, 0.3):
         values, indices, tail = _teacher(z, k, tau, rest, g)
         _check_loss(z, values, indices, tail, tau)
+
+
+@pytest.mark.parametrize('cols', [30, 20000, 70001])
+def test_the_tail_alone_wherever_it_lies(cols):
+    """no entry is used: the teacher says 'one of all columns' however large or small its tail's logarithm; listed values of -inf beside it count nothing"""
+    g = torch.Generator().manual_seed(cols)
+    z = torch.randn(6, cols, generator=g)
+    tail = torch.tensor([-846.0, -3e5, -1.0, 0.0, 700.0, 4e6])
+    values, indices = torch.randn(6, 3, generator=g), torch.full((6, 3), -1)
+    indices[1, 0], values[1, 0] = 7, -INF
+    indices[4, 1], values[4, 1] = 7, -INF
+    for tau in (0.07, 1.0):
+        _check_loss(z, values, indices, tail, tau)
+    got = distill_loss(z.to(DEV), values.to(DEV), indices.to(DEV), tail=tail.to(DEV), reduction='none')
+    assert float(got[[0, 2, 3, 5]].abs().max()) <= 1e-5                     # nothing is left out: -log(all of it)
