@@ -12,7 +12,7 @@
 #include "row_vec.hpp"
 
 constexpr int DS_MAXK = 256, DS_MAXV = 1 << 30;
-constexpr double LOG2E = 1.4426950408889634, LN2 = 0.6931471805599453;
+constexpr double LOG2E = 1.4426950408889634;
 constexpr float LOG2E_F = (float)LOG2E;
 
 __device__ __forceinline__ float wave_max(float v, int lane) {
@@ -567,21 +567,15 @@ extern "C" int rumpy_top_logits(const rumpy_top_logits_args* p, void* stream) {
 constexpr int DS_WG = 512, DS_WAVES = DS_WG / 64;
 constexpr int DS_STATE = 8;      // per row: reference and coefficient of the streamed columns, maximum and log sum of all, the teacher's log sum, dead, the teacher's maximum
 
-// exp((v - m) / tau) with c + lo = log2(e) / tau: c alone, rounded to 32 bits, is another temperature for the whole row, and its error of up to 2^-25
-// does not average out in the loss (1.8e-6 of it where 32-bit divisions made 2e-7).  Two fused multiply-adds per element; they need m c finite: a
-// type's lowest value (a mask) overflows there, and takes the difference first.  The large product meets fl(m c) first: the other way round its last
-// digits are gone, for the whole row, where the logits lie far from zero (2^-25 of m c: 5e-5 at logits of 60 and a temperature of 0.07).  fl(m c) is off m (c + lo), ds_off says how much (in powers of two).
-__device__ __forceinline__ float ds_exp(float v, float m, float c, float lo, float mc) {
-  return __builtin_amdgcn_exp2f(fabsf(mc) < INFINITY ? fmaf(v, lo, fmaf(v, c, -mc)) : (v - m) * c);
+// exp((v - m) / tau), v <= m, with c + lo = log2(e) / tau: c alone, rounded to 32 bits, is another temperature for the whole row, and its error of up to
+// 2^-25 does not average out in the loss (1.8e-6 of it where 32-bit divisions made 2e-7).  The difference first: no digits are lost where a row lies
+// far from zero, and none of it overflows (lowest values of a type as masks).  v = -inf gives 0, which is why lo is positive; m is finite.
+__device__ __forceinline__ float ds_exp(float v, float m, float c, float lo) {
+  const float d = v - m;
+  return __builtin_amdgcn_exp2f(fmaf(d, lo, d * c));
 }
-__device__ __forceinline__ float ds_off(float m, float c, float lo) { const float mc = m * c; return fabsf(mc) < INFINITY ? fmaf(m, lo, fmaf(m, c, -mc)) : 0.f; }
-// the factor from a sum relative to fl(m c) to one relative to fl(M c), M >= m.  Where a product overflows, different values are so far apart that it is 0.
-__device__ __forceinline__ float ds_rescale(float m, float M, float c) {
-#pragma clang fp contract(off)                       // (both products rounded, as the sums have them)
-  if (m == M) return 1.f;
-  const float d = m * c - M * c;
-  return m == -INFINITY || d != d ? 0.f : __builtin_amdgcn_exp2f(d);
-}
+// the factor from a sum relative to m to one relative to M >= m (m = -inf: there is no sum yet; M = inf: NaN, by the sum itself)
+__device__ __forceinline__ float ds_rescale(float m, float M, float c, float lo) { return m == -INFINITY ? 0.f : m == M ? 1.f : ds_exp(m, M, c, lo); }
 
 struct DsPlan { int splits, seg; float c, lo, near, inv_tau; double inv_tau64; };      // c + lo = log2(e) / tau; near: the nearest float to it
 // rows are cut when there are too few of them to fill the chip; a piece's bit map of listed columns has to fit LDS (2^18 columns: 32 KB)
@@ -645,7 +639,7 @@ template <int FMT> __device__ __forceinline__ int ds_load_listed(const rumpy_dis
 }
 
 // one wave: the row's loss and what its gradient needs, from the sum over the streamed columns (all of them, or the unlisted ones when the
-// rest is an outcome): s = sum exp2(z (c + lo) - fl(m c)).  The logarithms and their sum are made in 64 bits: the loss is a small difference of them.
+// rest is an outcome): s = sum exp((z - m) / tau).  The logarithms and their sum are made in 64 bits: the loss is a small difference of them.
 __device__ __forceinline__ void ds_finish(const rumpy_distill_args& a, const DsPlan& plan, int64_t row, const DsListed& l, float m, float s, int lane) {
   const float c = plan.c, lo = plan.lo;
   const double inv_tau = plan.inv_tau64;
@@ -674,19 +668,19 @@ __device__ __forceinline__ void ds_finish(const rumpy_distill_args& a, const DsP
   const bool tail_alone = vm == -INFINITY;
   if (tail_alone) vm = 0.f;
   const double tr = tl - vm * inv_tau, up = tr > 0.0 || tail_alone ? tr : 0.0;
-  const float M = rest ? fmaxf(m, zm) : m, Mc = M * c;
+  const float M = rest ? fmaxf(m, zm) : m;
   float p_sum = 0.f, sl = 0.f;
   for (int i = lane; i < a.k; i += 64) {
     if (l.idx[i] < 0) continue;
     p_sum += __builtin_amdgcn_exp2f((float)((((double)l.v[i] - vm) * inv_tau - up) * LOG2E));
-    if (rest && l.first[i]) sl += ds_exp(l.z[i], M, c, lo, Mc);
+    if (rest && l.first[i]) sl += ds_exp(l.z[i], M, c, lo);
   }
   p_sum = wave64_sum(p_sum, lane) + (rest ? __builtin_amdgcn_exp2f((float)((tr - up) * LOG2E)) : 0.f);
   nan |= p_sum != p_sum;                                   // (infinite logits of the teacher)
   const double ln_p = log((double)p_sum);
   float S = s;
-  if (rest) S = wave64_sum(sl, lane) + (m == -INFINITY ? 0.f : s * ds_rescale(m, M, c));
-  const double ln_s = log((double)S) - ds_off(M, c, lo) * LN2;
+  if (rest) S = wave64_sum(sl, lane) + (m == -INFINITY ? 0.f : s * ds_rescale(m, M, c, lo));
+  const double ln_s = log((double)S);
   double loss = 0.0;
   for (int i = lane; i < a.k; i += 64) {
     if (l.idx[i] < 0) continue;
@@ -698,7 +692,7 @@ __device__ __forceinline__ void ds_finish(const rumpy_distill_args& a, const DsP
   for (int o = 1; o < 64; o *= 2) loss += __shfl_xor(loss, o);
   float coef = 1.f / S;
   if (rest) {
-    const double lpt = tr - up - ln_p, lqt = m == -INFINITY ? (double)-INFINITY : ((double)m - M) * inv_tau + log((double)s) - ds_off(m, c, lo) * LN2 - ln_s;
+    const double lpt = tr - up - ln_p, lqt = m == -INFINITY ? (double)-INFINITY : ((double)m - M) * inv_tau + log((double)s) - ln_s;
     const float pt = __builtin_amdgcn_exp2f((float)(lpt * LOG2E)), qt = __builtin_amdgcn_exp2f((float)(lqt * LOG2E));
     if (pt != 0.f) loss += pt * (lpt - lqt);
     coef = m == -INFINITY ? 0.f : (qt - pt) / s;
@@ -707,7 +701,7 @@ __device__ __forceinline__ void ds_finish(const rumpy_distill_args& a, const DsP
   if (lane == 0) {
     a.row_loss[row] = w == 0.f ? 0.f : (float)(w * loss * a.tau * a.tau);
     st[0] = m == -INFINITY ? 0.f : m;
-    st[1] = m == -INFINITY ? coef : coef * __builtin_amdgcn_exp2f(ds_off(m, c, lo) - ds_off(m, plan.near, 0.f));      // (the gradient's exponentials are of z near - fl(m near))
+    st[1] = coef;
     st[2] = M;
     st[3] = nan ? coef : (float)ln_s;
     st[4] = (float)(up + ln_p);
@@ -759,7 +753,7 @@ template <int FMT, bool REST> __global__ void __launch_bounds__(DS_WG) distill_f
     __syncthreads();
   }
   const float c = plan.c, lo = plan.lo;
-  float m = -INFINITY, s = 0.f, mc = 0.f;
+  float m = -INFINITY, ref = 0.f, s = 0.f;            // ref: m, or 0 as long as there is nothing but -inf
   auto sum_up = [&](auto& v) {
     constexpr int N = sizeof(v) / sizeof(v[0]);
     float top = v[0][0];
@@ -768,21 +762,13 @@ template <int FMT, bool REST> __global__ void __launch_bounds__(DS_WG) distill_f
 #pragma unroll
       for (int i = 0; i < 8; ++i) top = fmaxf(top, v[u][i]);
     if (top > m) {
-      s *= ds_rescale(m, top, c);
-      m = top;
-      mc = top * c;
+      s *= ds_rescale(m, top, c, lo);
+      m = ref = top;
     }
-    if (fabsf(mc) < INFINITY) {
 #pragma unroll
-      for (int u = 0; u < N; ++u)
+    for (int u = 0; u < N; ++u)
 #pragma unroll
-        for (int i = 0; i < 8; ++i) s += __builtin_amdgcn_exp2f(fmaf(v[u][i], lo, fmaf(v[u][i], c, -mc)));
-    } else {
-#pragma unroll
-      for (int u = 0; u < N; ++u)
-#pragma unroll
-        for (int i = 0; i < 8; ++i) s += __builtin_amdgcn_exp2f((v[u][i] - m) * c);
-    }
+      for (int i = 0; i < 8; ++i) s += ds_exp(v[u][i], ref, c, lo);
   };
   auto leave_out = [&](float (&v)[8], uint32_t here) {
     if (here) {
@@ -826,7 +812,7 @@ template <int FMT, bool REST> __global__ void __launch_bounds__(DS_WG) distill_f
     sum_up(v);
   }
   const float M = block_max<DS_WAVES>(m, red);
-  s = block_sum<DS_WAVES>(m == -INFINITY ? s : s * ds_rescale(m, M, c), red);
+  s = block_sum<DS_WAVES>(m == -INFINITY ? s : s * ds_rescale(m, M, c, lo), red);
   if (plan.splits > 1) {
     if (tid == 0) { a.partial[blockIdx.x * (size_t)2] = M; a.partial[blockIdx.x * (size_t)2 + 1] = s; }
     return;
@@ -846,7 +832,7 @@ template <int FMT> __global__ void __launch_bounds__(DS_WG) distill_join_kernel(
     return;
   }
   ds_load_listed<FMT>(a, row, reinterpret_cast<const E*>(a.logits) + (size_t)row * a.ld, l);
-  const float c = plan.c;
+  const float c = plan.c, lo = plan.lo;
   const float* part = a.partial + (size_t)row * plan.splits * 2;
   float m = -INFINITY;
   for (int i = tid; i < plan.splits; i += DS_WG) m = fmaxf(m, part[2 * i]);
@@ -854,7 +840,7 @@ template <int FMT> __global__ void __launch_bounds__(DS_WG) distill_join_kernel(
   float s = 0.f;
   for (int i = tid; i < plan.splits; i += DS_WG) {
     const float mi = part[2 * i];
-    s += mi == -INFINITY ? part[2 * i + 1] : part[2 * i + 1] * ds_rescale(mi, M, c);
+    s += mi == -INFINITY ? part[2 * i + 1] : part[2 * i + 1] * ds_rescale(mi, M, c, lo);
   }
   s = block_sum<DS_WAVES>(s, red);
   if (tid < 64) ds_finish(a, plan, row, l, M, s, tid);
@@ -909,8 +895,7 @@ template <int FMT> __global__ void __launch_bounds__(DS_WG) distill_bwd_kernel(r
   const float c = plan.near;
   float g = (a.loss ? *a.gout * *a.factor : a.gout[row]) * (float)a.tau;
   if (a.row_weight) g *= a.row_weight[row];
-  const float m = st[0], mc = m * c, coef = g * st[1];
-  const bool fused = fabsf(mc) < INFINITY;
+  const float m = st[0], coef = g * st[1];
   if (tid < a.k) {
     const int64_t i = ds_index(a, row, tid);
     idx[tid] = i >= j0 && i < j1 ? (int)i : -1;
@@ -921,7 +906,7 @@ template <int FMT> __global__ void __launch_bounds__(DS_WG) distill_bwd_kernel(r
     float v[8];
     unpack_piece<FMT>(load_piece<FMT>(z + j, n, 0.f), v);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = coef * __builtin_amdgcn_exp2f(fused ? fmaf(v[i], c, -mc) : (v[i] - m) * c);
+    for (int i = 0; i < 8; ++i) v[i] = coef * __builtin_amdgcn_exp2f((v[i] - m) * c);
     store8<FMT>(a.dlogits, out + j, n, v);
   }
   __syncthreads();          // the listed columns are written over (same workgroup, behind the barrier); a column listed twice takes both shares

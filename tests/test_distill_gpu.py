@@ -553,3 +553,45 @@ def test_the_tail_alone_wherever_it_lies(cols):
         _check_loss(z, values, indices, tail, tau)
     got = distill_loss(z.to(DEV), values.to(DEV), indices.to(DEV), tail=tail.to(DEV), reduction='none')
     assert float(got[[0, 2, 3, 5]].abs().max()) <= 1e-5                     # nothing is left out: -log(all of it)
+
+
+@pytest.mark.parametrize('dtype', [F32, BF16, F16], ids=str)
+@pytest.mark.parametrize('rest', [False, True])
+@pytest.mark.parametrize('cols', [8, 3000, 70001])
+def test_lowest_values_as_masks_at_every_temperature(cols, rest, dtype):
+    """columns that the student masks with its type's lowest value or -inf: few, most, whole stretches of a row, all that are not listed"""
+    g = torch.Generator().manual_seed(cols)
+    k = 3
+    for mask in (LOWEST[dtype], -INF):
+        for tau in (0.07, 1.0, 4.0, 50.0):
+            z = torch.randn(5, cols, generator=g).to(dtype)
+            values, indices, tail = _teacher(z, k, tau, rest, g)
+            out = torch.rand(5, cols, generator=g) < torch.tensor([0.05, 0.5, 0.95, 0.0, 1.0])[:, None]
+            out[3, cols // 4:] = True
+            out.scatter_(1, indices, False)
+            z[out] = mask
+            if rest:
+                tail[4] = -INF                                      # (the teacher's whole mass is listed, as the student's)
+            if mask == -INF:
+                _check_loss(z, values, indices, tail, tau)
+                continue
+            # a probability under the smallest float is 0: bit for bit what -inf gives, unless nothing unlisted is left of a row that needs it
+            res = []
+            for m in (mask, -INF):
+                zd = z.masked_fill(out, m).to(DEV).requires_grad_()
+                loss = distill_loss(zd, values.to(DEV), indices.to(DEV), tail=tail.to(DEV) if rest else None, temperature=tau, reduction='none')
+                res.append((loss.detach().cpu(), torch.autograd.grad(loss.sum(), zd)[0].cpu()))
+            nothing = out.sum(1) == cols - k
+            same = ~nothing if rest else torch.ones(5, dtype=torch.bool)
+            if rest:
+                same[4] = True
+            if dtype == F16 and tau > 1.0:                          # (its lowest value over such a temperature is not that low)
+                _check_loss(z, values, indices, tail, tau)
+                continue
+            assert torch.equal(res[0][0][same], res[1][0][same]) and torch.equal(res[0][1][same], res[1][1][same])
+            if (~same).any():                                       # finite where float32 can hold it: tau p_t |lowest|, p_t right to a few times 2^-24 |u|
+                want = _loss_reference(z, values, indices, tail, tau, torch.ones(5), torch.ones(5))[0][~same]
+                big = want > torch.finfo(F32).max
+                got = res[0][0][~same].double()
+                assert bool((got[big] == INF).all()) and bool(((got - want).abs() <= 1e-4 * want)[~big].all())
+                assert not res[0][1].isnan().any()
