@@ -186,3 +186,30 @@ def test_captured_steps_of_two_batch_shapes_and_a_changed_weight(monkeypatch):
     for step, (a, b) in enumerate(zip(*res)):
         assert a[0] == b[0] and torch.equal(a[1], b[1]), step
         assert a[2][0].shape[0] == plan[step][0] and all(torch.equal(s, t) for s, t in zip(a[2], b[2])), step
+
+
+def test_calls_from_several_threads_at_once():
+    """each thread on a stream of its own, forward and backward: every result is that of the calls one after another"""
+    from concurrent.futures import ThreadPoolExecutor
+    from rumpy_amd.residual_norm import residual_norm
+    g = torch.Generator().manual_seed(31)
+    data = [(torch.randn(3, 70000 + 13 * i, generator=g).to(DEV), torch.randn(200, 100 + i, generator=g).to(DEV)) for i in range(4)]
+
+    def work(i):
+        z, x = data[i]
+        with torch.cuda.stream(torch.cuda.Stream()):
+            out = []
+            for _ in range(5):
+                leaf, t = z.clone().requires_grad_(), x.clone().requires_grad_()
+                values, indices, tail = top_logits(z.flip(0), 30)
+                loss = distill_loss(leaf, values, indices, tail=tail)
+                y, h = residual_norm(x, t, gate=x[0].clone(), post_norm='rms', pre_norm='layer')
+                out = [values, indices, tail, loss.detach(), y.detach(), h.detach()] + list(torch.autograd.grad(loss + (y * h).sum(), [leaf, t]))
+            torch.cuda.current_stream().synchronize()
+        return out
+    torch.cuda.synchronize()
+    want = [work(i) for i in range(4)]
+    with ThreadPoolExecutor(4) as pool:
+        got = list(pool.map(work, range(4)))
+    for a, b in zip(want, got):
+        assert all(torch.equal(s, t) for s, t in zip(a, b))
