@@ -8,7 +8,7 @@
 // and direction beside it.  The sum of exp runs over the row once with a running maximum per thread; q_t is summed directly over the columns
 // that are not listed (a bit map of them lies in LDS): 1 - sum q_i would cancel where the listed columns hold nearly everything.
 // Exponentials and a row's sums are fp32, a row's logarithms and the sums over rows 64-bit.  Every reduction has a fixed order, which goes with the
-// alignment of a row's address alone: results are bitwise reproducible.
+// call's sizes and the alignment of a row's address alone: results are bitwise reproducible.
 #include "row_vec.hpp"
 
 constexpr int DS_MAXK = 256, DS_MAXV = 1 << 30;
@@ -19,6 +19,16 @@ __device__ __forceinline__ float wave_max(float v, int lane) {
   v = fmaxf(v, dpp_quad1(v)); v = fmaxf(v, dpp_quad2(v)); v = fmaxf(v, dpp_half_mirror(v)); v = fmaxf(v, dpp_row_mirror(v));
   v = fmaxf(v, lane_xor16(v, lane >> 4));
   return fmaxf(v, lane_xor32(v, lane));
+}
+// maximum over, and any of, the L neighbouring lanes of a row (16 or 64), in every one of them
+template <int L> __device__ __forceinline__ float lanes_max(float v, int lane) {
+  if constexpr (L == 64) return wave_max(v, lane);
+  v = fmaxf(v, dpp_quad1(v)); v = fmaxf(v, dpp_quad2(v)); v = fmaxf(v, dpp_half_mirror(v));
+  return fmaxf(v, dpp_row_mirror(v));
+}
+template <int L> __device__ __forceinline__ bool lanes_any(bool b, int lane) {
+  const uint64_t all = __ballot(b);
+  return (L == 64 ? all : all >> (lane & ~(L - 1)) & ((1ull << (L & 63)) - 1ull)) != 0ull;
 }
 template <int WAVES> __device__ __forceinline__ float block_sum(float v, float* red) {
   v = wave64_sum(v, threadIdx.x & 63);
@@ -565,7 +575,8 @@ extern "C" int rumpy_top_logits(const rumpy_top_logits_args* p, void* stream) {
 
 // ================================================================================================================ loss and gradient
 constexpr int DS_WG = 512, DS_WAVES = DS_WG / 64;
-constexpr int DS_STATE = 8;      // per row: reference and coefficient of the streamed columns, maximum and log sum of all, the teacher's log sum, dead, the teacher's maximum
+constexpr int DS_STATE = 8;      // per row: reference and coefficient of the streamed columns, maximum and log sum of all, the teacher's log sum, dead, the teacher's maximum,
+                                 // whether a column may be listed twice
 
 // exp((v - m) / tau), v <= m, with c + lo = log2(e) / tau: c alone, rounded to 32 bits, is another temperature for the whole row, and its error of up to
 // 2^-25 does not average out in the loss (1.8e-6 of it where 32-bit divisions made 2e-7).  The difference first: no digits are lost where a row lies
@@ -638,29 +649,32 @@ template <int FMT> __device__ __forceinline__ int ds_load_listed(const rumpy_dis
   return mine;
 }
 
-// one wave: the row's loss and what its gradient needs, from the sum over the streamed columns (all of them, or the unlisted ones when the
+// L lanes of one wave: the row's loss and what its gradient needs, from the sum over the streamed columns (all of them, or the unlisted ones when the
 // rest is an outcome): s = sum exp((z - m) / tau).  The logarithms and their sum are made in 64 bits: the loss is a small difference of them.
-__device__ __forceinline__ void ds_finish(const rumpy_distill_args& a, const DsPlan& plan, int64_t row, const DsListed& l, float m, float s, int lane) {
+// idx, v, z: what the teacher lists, in LDS; first(i): no earlier entry names entry i's column; doubled: some column may be named twice.
+template <int L, typename First>
+__device__ __forceinline__ void ds_finish(const rumpy_distill_args& a, const DsPlan& plan, int64_t row, const int* idx, const float* v, const float* z, First first,
+                                          bool doubled, float m, float s, int lane) {
   const float c = plan.c, lo = plan.lo;
   const double inv_tau = plan.inv_tau64;
   const bool rest = a.tail != nullptr;
   const float w = a.row_weight ? a.row_weight[row] : 1.f;
   float vm = -INFINITY, zm = -INFINITY;
   bool odd = false, outside = false;
-  for (int i = lane; i < a.k; i += 64) {
-    if (l.idx[i] == -1) continue;
-    outside |= l.idx[i] == -2;
-    odd |= l.v[i] != l.v[i];
-    vm = fmaxf(vm, l.v[i]);
-    zm = fmaxf(zm, l.z[i]);
+  for (int i = lane % L; i < a.k; i += L) {
+    if (idx[i] == -1) continue;
+    outside |= idx[i] == -2;
+    odd |= v[i] != v[i];
+    vm = fmaxf(vm, v[i]);
+    zm = fmaxf(zm, z[i]);
   }
-  vm = wave_max(vm, lane);
-  zm = wave_max(zm, lane);
+  vm = lanes_max<L>(vm, lane);
+  zm = lanes_max<L>(zm, lane);
   const float tl = rest ? a.tail[row] : -INFINITY;
-  bool nan = __ballot(odd || outside) != 0ull || tl != tl;
+  bool nan = lanes_any<L>(odd || outside, lane) || tl != tl;
   float* st = a.state + row * DS_STATE;
   if (!nan && vm == -INFINITY && tl == -INFINITY) {            // the teacher says nothing about this row
-    if (lane == 0) { a.row_loss[row] = 0.f; st[0] = st[1] = st[2] = st[3] = st[4] = 0.f; st[5] = 1.f; }
+    if (lane % L == 0) { a.row_loss[row] = 0.f; st[0] = st[1] = st[2] = st[3] = st[4] = 0.f; st[5] = 1.f; }
     return;
   }
   // the teacher's logarithms relative to its largest logit, so that far from zero no digits are lost: lp = (v - vm) / tau - up - ln_p
@@ -670,35 +684,36 @@ __device__ __forceinline__ void ds_finish(const rumpy_distill_args& a, const DsP
   const double tr = tl - vm * inv_tau, up = tr > 0.0 || tail_alone ? tr : 0.0;
   const float M = rest ? fmaxf(m, zm) : m;
   float p_sum = 0.f, sl = 0.f;
-  for (int i = lane; i < a.k; i += 64) {
-    if (l.idx[i] < 0) continue;
-    p_sum += __builtin_amdgcn_exp2f((float)((((double)l.v[i] - vm) * inv_tau - up) * LOG2E));
-    if (rest && l.first[i]) sl += ds_exp(l.z[i], M, c, lo);
+  for (int i = lane % L; i < a.k; i += L) {
+    if (idx[i] < 0) continue;
+    p_sum += __builtin_amdgcn_exp2f((float)((((double)v[i] - vm) * inv_tau - up) * LOG2E));
+    if (rest && first(i)) sl += ds_exp(z[i], M, c, lo);
   }
-  p_sum = wave64_sum(p_sum, lane) + (rest ? __builtin_amdgcn_exp2f((float)((tr - up) * LOG2E)) : 0.f);
+  p_sum = lanes_sum<L>(p_sum, lane) + (rest ? __builtin_amdgcn_exp2f((float)((tr - up) * LOG2E)) : 0.f);
   nan |= p_sum != p_sum;                                   // (infinite logits of the teacher)
-  const double ln_p = log((double)p_sum);
   float S = s;
-  if (rest) S = wave64_sum(sl, lane) + (m == -INFINITY ? 0.f : s * ds_rescale(m, M, c, lo));
-  const double ln_s = log((double)S);
+  if (rest) S = lanes_sum<L>(sl, lane) + (m == -INFINITY ? 0.f : s * ds_rescale(m, M, c, lo));
+  // (the three logarithms in three lanes at once: one after another they were a third of a short row's time)
+  const double ln = log((double)(lane % 4 == 0 ? p_sum : lane % 4 == 1 ? S : s));
+  const double ln_p = __shfl(ln, 0, L), ln_s = __shfl(ln, 1, L), ln_r = __shfl(ln, 2, L);
   double loss = 0.0;
-  for (int i = lane; i < a.k; i += 64) {
-    if (l.idx[i] < 0) continue;
-    const double lp = ((double)l.v[i] - vm) * inv_tau - up - ln_p;
+  for (int i = lane % L; i < a.k; i += L) {
+    if (idx[i] < 0) continue;
+    const double lp = ((double)v[i] - vm) * inv_tau - up - ln_p;
     const float p = __builtin_amdgcn_exp2f((float)(lp * LOG2E));
-    if (p != 0.f) loss += p * (lp - (((double)l.z[i] - M) * inv_tau - ln_s));
+    if (p != 0.f) loss += p * (lp - (((double)z[i] - M) * inv_tau - ln_s));
   }
 #pragma unroll
-  for (int o = 1; o < 64; o *= 2) loss += __shfl_xor(loss, o);
+  for (int o = 1; o < L; o *= 2) loss += __shfl_xor(loss, o);
   float coef = 1.f / S;
   if (rest) {
-    const double lpt = tr - up - ln_p, lqt = m == -INFINITY ? (double)-INFINITY : ((double)m - M) * inv_tau + log((double)s) - ln_s;
+    const double lpt = tr - up - ln_p, lqt = m == -INFINITY ? (double)-INFINITY : ((double)m - M) * inv_tau + ln_r - ln_s;
     const float pt = __builtin_amdgcn_exp2f((float)(lpt * LOG2E)), qt = __builtin_amdgcn_exp2f((float)(lqt * LOG2E));
     if (pt != 0.f) loss += pt * (lpt - lqt);
     coef = m == -INFINITY ? 0.f : (qt - pt) / s;
   }
   if (nan) loss = coef = NOT_A_NUMBER;
-  if (lane == 0) {
+  if (lane % L == 0) {
     a.row_loss[row] = w == 0.f ? 0.f : (float)(w * loss * a.tau * a.tau);
     st[0] = m == -INFINITY ? 0.f : m;
     st[1] = coef;
@@ -707,6 +722,7 @@ __device__ __forceinline__ void ds_finish(const rumpy_distill_args& a, const DsP
     st[4] = (float)(up + ln_p);
     st[5] = w == 0.f ? 1.f : 0.f;
     st[6] = vm;
+    st[7] = doubled ? 1.f : 0.f;
   }
 }
 
@@ -817,7 +833,7 @@ template <int FMT, bool REST> __global__ void __launch_bounds__(DS_WG) distill_f
     if (tid == 0) { a.partial[blockIdx.x * (size_t)2] = M; a.partial[blockIdx.x * (size_t)2 + 1] = s; }
     return;
   }
-  if (tid < 64) ds_finish(a, plan, row, l, M, s, tid);
+  if (tid < 64) ds_finish<64>(a, plan, row, l.idx, l.v, l.z, [&](int i) { return l.first[i]; }, true, M, s, tid);
 }
 
 // rows that were cut: their pieces' sums, then the row
@@ -843,7 +859,89 @@ template <int FMT> __global__ void __launch_bounds__(DS_WG) distill_join_kernel(
     s += mi == -INFINITY ? part[2 * i + 1] : part[2 * i + 1] * ds_rescale(mi, M, c, lo);
   }
   s = block_sum<DS_WAVES>(s, red);
-  if (tid < 64) ds_finish(a, plan, row, l, M, s, tid);
+  if (tid < 64) ds_finish<64>(a, plan, row, l.idx, l.v, l.z, [&](int i) { return l.first[i]; }, true, M, s, tid);
+}
+
+// ---- many short rows: TPR lanes of a wave a row, 8 columns each at a time; several rows a workgroup, none of which waits for another.
+// A row's fixed work (what is listed, three 64-bit logarithms, the state) is as long as its columns': with a workgroup a row, 65536 x 100 fp32 took 468 us
+// forward and 218 backward, with 16 lanes 20 and 11.  Pieces are laid out as in a row of channels: the last one is moved back to end with the row, what it repeats is left out.
+template <int FMT, int TPR> struct DsShortRow {
+  const typename RowElem<FMT>::type* z;
+  int V, l;
+  __device__ __forceinline__ int col(int i) const { return (i * TPR + l) * 8; }
+  __device__ __forceinline__ int at(int i) const { return V < 8 ? 0 : min(col(i), V - 8); }
+  __device__ __forceinline__ int rounds() const { return (V + TPR * 8 - 1) / (TPR * 8); }
+  __device__ __forceinline__ RowRaw<FMT> load(int i) const { return load_piece<FMT>(z + at(i), min(V, 8), 0.f); }
+};
+__device__ __forceinline__ int ds_short_words(int V) { return V / 32 + 2; }         // (8 bits from any column on lie inside)
+// (16 rows of 512 columns and 256 entries, 4 of 8192 and 256: at most 50 KB)
+static size_t ds_short_lds(int V, int k, int sub, bool fwd) { return (size_t)4 * sub * (fwd ? V / 32 + 2 + 3 * k : 3 * k); }
+
+template <int FMT, bool REST, int TPR> __global__ void __launch_bounds__(256) distill_short_fwd_kernel(rumpy_distill_args a, DsPlan plan) {
+  typedef typename RowElem<FMT>::type E;
+  extern __shared__ uint32_t bits_of_rows[];
+  const int tid = threadIdx.x, lane = tid & 63, l = tid % TPR, words = ds_short_words(a.V);
+  const int64_t row = (int64_t)blockIdx.x * (256 / TPR) + tid / TPR;
+  const bool in = row < a.rows, live = in && !(a.row_weight && a.row_weight[row] == 0.f);       // a row that does not count is not looked at
+  if (in && !live && l == 0) { a.row_loss[row] = 0.f; a.state[row * DS_STATE + 5] = 1.f; }
+  uint32_t* bits = bits_of_rows + (size_t)(tid / TPR) * (words + 3 * a.k);
+  int* idx = reinterpret_cast<int*>(bits + words);
+  float* v = reinterpret_cast<float*>(idx + a.k);
+  float* zl = v + a.k;
+  const DsShortRow<FMT, TPR> r{reinterpret_cast<const E*>(a.logits) + (size_t)(live ? row : 0) * a.ld, a.V, l};
+  RowRaw<FMT> raw;
+  if (live) raw = r.load(0);
+  for (int i = l; i < words; i += TPR) bits[i] = 0;
+  __syncthreads();
+  bool twice = false;
+  if (live) {
+    for (int i = l; i < a.k; i += TPR) {
+      const int64_t j = ds_index(a, row, i);
+      const bool inside = j >= 0 && j < a.V;
+      idx[i] = j < 0 ? -1 : inside ? (int)j : -2;
+      v[i] = ds_value(a, row, i);
+      zl[i] = inside ? elem_to_f32<FMT>(r.z[j]) : 0.f;
+      if (inside) twice |= atomicOr(&bits[j >> 5], 1u << (j & 31)) >> (j & 31) & 1u;
+    }
+  }
+  __syncthreads();
+  if (!live) return;
+  const float c = plan.c, lo = plan.lo;
+  float m = -INFINITY, ref = 0.f, s = 0.f;
+  const int rounds = r.rounds();
+  for (int b = 0; b < rounds; ++b) {
+    float x[8];
+    unpack_piece<FMT>(raw, x);
+    if (b + 1 < rounds) raw = r.load(b + 1);
+    const int col = r.col(b), at = r.at(b);
+    uint32_t out = 0;
+    if constexpr (REST) {
+      const uint32_t* w = bits + (at >> 5);
+      out = (uint32_t)((((uint64_t)w[1] << 32) | w[0]) >> (at & 31));
+    }
+    float top = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      if ((out >> i & 1u) || at + i < col || at + i >= a.V) x[i] = -INFINITY;
+      top = fmaxf(top, x[i]);
+    }
+    if (top > m) {
+      s *= ds_rescale(m, top, c, lo);
+      m = ref = top;
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) s += ds_exp(x[i], ref, c, lo);
+  }
+  const float M = lanes_max<TPR>(m, lane);
+  s = lanes_sum<TPR>(m == -INFINITY ? s : s * ds_rescale(m, M, c, lo), lane);
+  const bool doubled = lanes_any<TPR>(twice, lane);
+  // (the row's columns are looked through only where one is named twice)
+  auto first = [&](int i) {
+    if (doubled)
+      for (int o = 0; o < i; ++o) if (idx[o] == idx[i]) return false;
+    return true;
+  };
+  ds_finish<TPR>(a, plan, row, idx, v, zl, first, doubled, M, s, lane);
 }
 
 // loss = sum of the rows' (weighted) losses, over the sum of the weights for the mean; a sum of weights of zero gives 0
@@ -926,6 +1024,58 @@ template <int FMT> __global__ void __launch_bounds__(DS_WG) distill_bwd_kernel(r
   }
 }
 
+// many short rows, as in the forward pass: the listed columns' gradients are made first and stored over the others'
+template <int FMT, int TPR> __global__ void __launch_bounds__(256) distill_short_bwd_kernel(rumpy_distill_args a, DsPlan plan) {
+  typedef typename RowElem<FMT>::type E;
+  extern __shared__ uint32_t listed_of_rows[];
+  const int tid = threadIdx.x, l = tid % TPR;
+  const int64_t row = (int64_t)blockIdx.x * (256 / TPR) + tid / TPR;
+  const bool in = row < a.rows;
+  int* idx = reinterpret_cast<int*>(listed_of_rows + (size_t)(tid / TPR) * 3 * a.k);
+  float* p = reinterpret_cast<float*>(idx + a.k);
+  float* q = p + a.k;
+  const DsShortRow<FMT, TPR> r{reinterpret_cast<const E*>(a.logits) + (size_t)(in ? row : 0) * a.ld, a.V, l};
+  const float* st = a.state + (in ? row : 0) * DS_STATE;
+  const bool live = in && st[5] == 0.f, doubled = st[7] != 0.f;
+  const float c = plan.near;
+  float g = 0.f;
+  E* out = reinterpret_cast<E*>(a.dlogits) + (size_t)(in ? row : 0) * a.V;
+  if (live) {
+    g = (a.loss ? *a.gout * *a.factor : a.gout[row]) * (float)a.tau;
+    if (a.row_weight) g *= a.row_weight[row];
+    for (int i = l; i < a.k; i += TPR) {
+      const int64_t j = ds_index(a, row, i);
+      const bool inside = j >= 0 && j < a.V;
+      idx[i] = inside ? (int)j : -1;
+      p[i] = j < 0 ? 0.f : __builtin_amdgcn_exp2f(((ds_value(a, row, i) - st[6]) * plan.inv_tau - st[4]) * LOG2E_F);
+      q[i] = inside ? __builtin_amdgcn_exp2f(((elem_to_f32<FMT>(r.z[j]) - st[2]) * plan.inv_tau - st[3]) * LOG2E_F) : 0.f;
+    }
+  }
+  if (in) {
+    const float m = live ? st[0] : 0.f, coef = live ? g * st[1] : 0.f;
+    for (int b = 0; b < r.rounds(); ++b) {
+      if (r.col(b) >= a.V) break;
+      float x[8];
+      if (live) unpack_piece<FMT>(r.load(b), x);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] = live ? coef * __builtin_amdgcn_exp2f((x[i] - m) * c) : 0.f;
+      store8<FMT>(out, r.at(b), min(a.V, 8), x);
+    }
+  }
+  __syncthreads();
+  if (!live) return;
+  for (int i = l; i < a.k; i += TPR) {
+    const int mine = idx[i];
+    if (mine < 0) continue;
+    float share = p[i];
+    if (doubled) {
+      share = 0.f;
+      for (int o = 0; o < a.k; ++o) share += idx[o] == mine ? p[o] : 0.f;
+    }
+    out[mine] = f32_to_elem<FMT>(g * (q[i] - share));
+  }
+}
+
 static bool ds_fmt(int f) { return f == RUMPY_FMT_F32 || f == RUMPY_FMT_BF16 || f == RUMPY_FMT_F16; }
 static const char* ds_check(const rumpy_distill_args* p) {
   if (!p) return "no arguments";
@@ -946,7 +1096,33 @@ extern "C" int64_t rumpy_distill_partial_floats(int64_t rows, int32_t V) {
   return plan.splits > 1 ? rows * plan.splits * 2 : 0;
 }
 
+// Lanes of a short row; 0: a workgroup a row, or more.  us, bf16, forward + gradient, 16 lanes | 64 lanes | a workgroup a row:
+//   65536 x 100, k 8: 20 + 11 | 87 + 29 | 468 + 218     4096 x 256, k 64: 11 + 7 | 9 + 5 | 40 + 13      300 x 1000, k 8: 11 + 6 | 6 + 4 | 8 + 4
+//   16384 x 1000, k 8: 18 + 14 | 30 + 15 | 113 + 45      1200 x 2000, k 8: 9 + 6 (64) | 14 + 6      300 x 4000, k 8: 11 + 7 (64) | 7 + 4
+//   16384 x 4000, k 64: 50 + 68 (64) | 153 + 59          4096 x 8000, k 64: 27 + 26 (64) | 47 + 27   1200 x 8000, k 8: 19 + 13 (64) | 14 + 9
+// So 16 lanes while a row's columns and entries are few a lane and there are rows for all lanes of the chip; 64 while the rows fill it with a wave each.
+static int ds_short(int64_t rows, int32_t V, int32_t k) {
+  if (rows >= 8192 ? V <= (k <= 32 ? 1024 : 512) : V <= 256 && k <= 16) return 16;
+  return V <= 1024 || (V <= 8192 && rows * 4 >= V) ? 64 : 0;
+}
+template <int FMT, int TPR> static void ds_launch_short_fwd(const rumpy_distill_args& a, const DsPlan& plan, hipStream_t s) {
+  constexpr int SUB = 256 / TPR;
+  const dim3 grid((unsigned)((a.rows + SUB - 1) / SUB));
+  const size_t lds = ds_short_lds(a.V, a.k, SUB, true);
+  if (a.tail) hipLaunchKernelGGL((distill_short_fwd_kernel<FMT, true, TPR>), grid, dim3(256), lds, s, a, plan);
+  else hipLaunchKernelGGL((distill_short_fwd_kernel<FMT, false, TPR>), grid, dim3(256), lds, s, a, plan);
+}
+template <int FMT> static void ds_launch_bwd(const rumpy_distill_args& a, const DsPlan& plan, hipStream_t s) {
+  const int tpr = ds_short(a.rows, a.V, a.k);
+  const size_t lds = tpr ? ds_short_lds(a.V, a.k, 256 / tpr, false) : 0;
+  if (tpr == 16) hipLaunchKernelGGL((distill_short_bwd_kernel<FMT, 16>), dim3((unsigned)((a.rows + 15) / 16)), dim3(256), lds, s, a, plan);
+  else if (tpr == 64) hipLaunchKernelGGL((distill_short_bwd_kernel<FMT, 64>), dim3((unsigned)((a.rows + 3) / 4)), dim3(256), lds, s, a, plan);
+  else hipLaunchKernelGGL((distill_bwd_kernel<FMT>), dim3((unsigned)(a.rows * plan.splits)), dim3(DS_WG), 0, s, a, plan);
+}
 template <int FMT> static void ds_launch_fwd(const rumpy_distill_args& a, const DsPlan& plan, hipStream_t s) {
+  const int tpr = ds_short(a.rows, a.V, a.k);
+  if (tpr == 16) return ds_launch_short_fwd<FMT, 16>(a, plan, s);
+  if (tpr == 64) return ds_launch_short_fwd<FMT, 64>(a, plan, s);
   const dim3 grid((unsigned)(a.rows * plan.splits));
   const size_t lds = a.tail ? ((size_t)(plan.splits == 1 ? a.V : plan.seg) + 7 + 31) / 32 * 4 : 0;
   if (a.tail) hipLaunchKernelGGL((distill_fwd_kernel<FMT, true>), grid, dim3(DS_WG), lds, s, a, plan);
@@ -973,9 +1149,8 @@ extern "C" int rumpy_distill_bwd(const rumpy_distill_args* p, void* stream) {
   if (p->rows == 0) return RUMPY_OK;
   const DsPlan plan = ds_plan(p->rows, p->V, p->tau);
   hipStream_t s = (hipStream_t)stream;
-  const dim3 grid((unsigned)(p->rows * plan.splits));
-  if (p->fmt == RUMPY_FMT_F32) hipLaunchKernelGGL((distill_bwd_kernel<RUMPY_FMT_F32>), grid, dim3(DS_WG), 0, s, *p, plan);
-  else if (p->fmt == RUMPY_FMT_BF16) hipLaunchKernelGGL((distill_bwd_kernel<RUMPY_FMT_BF16>), grid, dim3(DS_WG), 0, s, *p, plan);
-  else hipLaunchKernelGGL((distill_bwd_kernel<RUMPY_FMT_F16>), grid, dim3(DS_WG), 0, s, *p, plan);
+  if (p->fmt == RUMPY_FMT_F32) ds_launch_bwd<RUMPY_FMT_F32>(*p, plan, s);
+  else if (p->fmt == RUMPY_FMT_BF16) ds_launch_bwd<RUMPY_FMT_BF16>(*p, plan, s);
+  else ds_launch_bwd<RUMPY_FMT_F16>(*p, plan, s);
   return rumpy_check_launch("rumpy_distill_bwd");
 }

@@ -595,3 +595,35 @@ def test_lowest_values_as_masks_at_every_temperature(cols, rest, dtype):
                 got = res[0][0][~same].double()
                 assert bool((got[big] == INF).all()) and bool(((got - want).abs() <= 1e-4 * want)[~big].all())
                 assert not res[0][1].isnan().any()
+
+
+@pytest.mark.parametrize('dtype', [F32, BF16, F16], ids=str)
+@pytest.mark.parametrize('rest', [False, True])
+@pytest.mark.parametrize('rows,cols,k', [(8197, 100, 64), (8200, 600, 8), (8193, 7, 7), (8209, 1, 1), (1201, 4800, 256), (501, 2000, 3), (4099, 256, 16)])
+def test_many_short_rows(rows, cols, k, rest, dtype):
+    """rows that share a wave or hold one alone, the last group not full: padded rows, unused entries, columns named twice, slices at any address"""
+    g = torch.Generator().manual_seed(rows + cols)
+    z = (torch.randn(rows, cols, generator=g) * 2).to(dtype)
+    values, indices, tail = _teacher(z, k, 0.5, rest, g)
+    if k > 2:
+        indices[::3, 1] = indices[::3, 0]
+        indices[1::5, 2] = -1
+    weight = torch.rand(rows, generator=g) / 64 * (torch.rand(rows, generator=g) < 0.8)         # (fp16 gradients of 'sum' stay in range)
+    _check_loss(z, values, indices, tail, 0.5, weight, lay=lambda t: torch.nn.functional.pad(t, (3, 2))[:, 3:3 + cols])
+
+
+def test_short_rows_beyond_2_31_elements():
+    rows, cols, k = 2200000, 1000, 4
+    g = torch.Generator(device=DEV).manual_seed(29)
+    z = torch.randn((rows, cols), generator=g, device=DEV, dtype=BF16)
+    pick = torch.cat([torch.arange(0, 8192), torch.arange(rows - 300, rows)]).to(DEV)
+    res = []
+    for some in (None, pick):
+        zs = z if some is None else z[some]
+        values, indices, tail = top_logits(zs, k)
+        leaf = zs.detach().requires_grad_()
+        loss = distill_loss(leaf, values * 0.5, indices, tail=tail, reduction='none')
+        grad, = torch.autograd.grad(loss, leaf, torch.ones_like(loss))
+        res.append([v if some is not None else v[pick] for v in (values, indices, tail, loss.detach(), grad)])
+        del grad, loss, leaf
+    assert all(torch.equal(a, b) for a, b in zip(*res))
