@@ -345,7 +345,7 @@ template <int FMT, int WG> __device__ __forceinline__ float rest_below(const Row
 // that reach the bound (a few times k) and the sum of exp over all others.  Where that does not do - too many reach the bound (columns of equal
 // value), it is infinite or a type's lowest value (fewer than about k columns that no mask holds), or there is NaN - the elements above T and, as
 // far as they do not suffice, those equal to it in the lowest columns; and where those are too many as well, the k-th pair by radix search.
-// Measured (MI355X): 2048 x 65521 bf16, k 100: 73 us = 3.7 TB/s (k 1: 62); 4096 x 8192 bf16, k 64: 28 us; 16384 x 1000 fp32, k 64: 37 us; 32 x 8192
+// Measured (MI355X): 2048 x 65521 bf16, k 100: 73 us = 3.7 TB/s (k 1: 62); 4096 x 8192 bf16, k 64: 28 us; 16384 x 1000 fp32, k 64: 37 us, k 4: 15; 32 x 8192
 // fp32: 8 us, one row's chain of latencies.  256 x 65521 with 100 valid columns or constant: 34 - 50 us (by radix search: 430 - 560; ascending
 // rows still go that way).
 // Six waves a SIMD: three workgroups of 512 a CU, with most of a row each in registers (with two, 2048 rows of 65521 took 80 us instead of 70).
@@ -537,7 +537,7 @@ extern "C" int64_t rumpy_top_logits_work_bytes(int64_t rows, int32_t V, int32_t 
 template <int FMT, int WG> static void tl_launch_wg(const rumpy_top_logits_args& a, const TlPlan& plan, hipStream_t s) {
   const dim3 grid((unsigned)(a.rows * plan.splits)), wg(WG);
   const int len = a.V < plan.seg ? a.V : plan.seg, np = (len / 8 + WG - 1) / WG;
-  constexpr int MOST = WG == 128 ? 4 : WG == 256 ? 8 : FMT == RUMPY_FMT_F32 ? 7 : 15;          // pieces in registers: the callers' limits; 60 registers
+  constexpr int MOST = WG <= 128 ? 4 : WG == 256 ? 8 : FMT == RUMPY_FMT_F32 ? 7 : 15;          // pieces in registers: the callers' limits; 60 registers
   if (len <= 8 * WG) hipLaunchKernelGGL((top_logits_kernel<FMT, WG, 1>), grid, wg, 0, s, a, plan);
   else if (np <= 2) hipLaunchKernelGGL((top_logits_kernel<FMT, WG, 2>), grid, wg, 0, s, a, plan);
   else if (np <= 4) hipLaunchKernelGGL((top_logits_kernel<FMT, WG, 4>), grid, wg, 0, s, a, plan);
@@ -545,11 +545,15 @@ template <int FMT, int WG> static void tl_launch_wg(const rumpy_top_logits_args&
   else hipLaunchKernelGGL((top_logits_kernel<FMT, WG, MOST>), grid, wg, 0, s, a, plan);
 }
 template <int FMT> static void tl_launch(const rumpy_top_logits_args& a, const TlPlan& plan, hipStream_t s) {
-  // Many short rows: small workgroups, more rows at once (a row is a chain of latencies: bound, lists, places).  At least 2 k threads, so that
-  // the bound comes from the better half of the threads' maxima.
-  const bool many = a.rows * plan.splits >= 1024;
-  if (many && a.V <= 4096 && a.k <= 64) tl_launch_wg<FMT, 128>(a, plan, s);
-  else if (many && a.V <= 16384 && a.k <= 128) tl_launch_wg<FMT, 256>(a, plan, s);
+  // Short rows: small workgroups, more rows at once (a row is a chain of latencies: bound, lists, places) and no barriers in one of 64.  At least 2 k threads,
+  // so that the bound comes from the better half of the threads' maxima (with k threads the lists run over: 65536 x 1000, k 64: 808 us with 64).
+  // us, bf16, 64 | 128 | 256 | 512 threads a row:  65536 x 300, k 16: 47 | 85 | 178 | 414     16384 x 1000, k 4: 15 | 23 | 46 | 112
+  // 4096 x 1000, k 64: - | 14 | 18 | 37     4096 x 4000, k 48: - | 17 | 22 | 38     4096 x 8000, k 96: - | - | 33 | 48     4096 x 600, k 192: - | - | 39 | 49
+  // 32 x 1000, k 4: 4.8 | 4.7 | 5.2 | 6.8     32 x 4000, k 64: - | 9.7 | 6.5 | 6.6     32 x 16000, k 64: - | - | 10 | 8
+  const bool few = a.rows < 256, many = a.rows >= 1024;
+  if (a.k <= 32 && a.V <= (many ? 2048 : 1024)) tl_launch_wg<FMT, 64>(a, plan, s);
+  else if (a.k <= 64 && a.V <= (many ? 4096 : 2048)) tl_launch_wg<FMT, 128>(a, plan, s);
+  else if (few ? a.k <= 96 && a.V <= 4096 : a.k <= 128 ? a.V <= 16384 : many && a.k <= 192 && a.V <= 2048) tl_launch_wg<FMT, 256>(a, plan, s);
   else tl_launch_wg<FMT, 512>(a, plan, s);
   if (plan.splits > 1) hipLaunchKernelGGL((top_join_kernel<FMT>), dim3((unsigned)a.rows), dim3(512), 0, s, a, plan);
 }

@@ -39,6 +39,8 @@ def _check_top(z, k, tau):
     got = torch.gather(zc, -1, order)
     assert torch.equal(values.cpu().nan_to_num(7.0, 8.0, 9.0), got.nan_to_num(7.0, 8.0, 9.0))
     tail = tail.double().cpu()
+    # (float32 holds it: a type's lowest value over a temperature under 1, -3.4e38 / 0.5, lies beyond the largest number 2^128 (1 - 2^-24) and rounds to -inf)
+    want = want.masked_fill(want < -(2.0 ** 128) * (1 - 2.0 ** -25), -INF)
     finite = torch.isfinite(want)
     assert torch.equal(torch.isnan(tail), torch.isnan(want)) and torch.equal(tail[~finite].nan_to_num(1.0), want[~finite].nan_to_num(1.0))
     if finite.any():
@@ -627,3 +629,21 @@ def test_short_rows_beyond_2_31_elements():
         res.append([v if some is not None else v[pick] for v in (values, indices, tail, loss.detach(), grad)])
         del grad, loss, leaf
     assert all(torch.equal(a, b) for a, b in zip(*res))
+
+
+@pytest.mark.parametrize('dtype', [F32, BF16, F16], ids=str)
+@pytest.mark.parametrize('rows,cols,ks', [(3, 64, (1, 32, 64)), (70, 65, (5, 33, 65)), (1025, 300, (3, 32, 64, 130)), (2050, 2047, (16, 60, 190)), (1100, 513, (32, 256)),
+                                          (300, 4097, (96, 128)), (8200, 40, (7, 40))])
+def test_top_logits_of_short_rows(rows, cols, ks, dtype):
+    """a wave to eight waves a row: values with many equal ones, masks, NaN, rows at any address"""
+    g = torch.Generator().manual_seed(rows + cols)
+    z = torch.randn(rows, cols + 5, generator=g) * 3
+    z[1::7] = z[1::7].round()                       # a few distinct values
+    z[2::11] = (z[2::11] > 3).float()
+    z[2, :cols // 2] = -INF
+    z[0, 7:] = LOWEST[dtype]
+    z[5 % rows, 9::3] = INF
+    z[6 % rows, 11] = NAN
+    z = z.to(dtype).to(DEV)[:, 3:3 + cols]
+    for k in ks:
+        _check_top(z, k, 0.5)
