@@ -878,7 +878,7 @@ template <int FMT, int TPR> struct DsShortRow {
   __device__ __forceinline__ RowRaw<FMT> load(int i) const { return load_piece<FMT>(z + at(i), min(V, 8), 0.f); }
 };
 __device__ __forceinline__ int ds_short_words(int V) { return V / 32 + 2; }         // (8 bits from any column on lie inside)
-// (16 rows of 512 columns and 256 entries, 4 of 8192 and 256: at most 50 KB)
+// (16 rows of 512 columns and 256 entries, 4 of 16384 and 256: at most 50 KB)
 static size_t ds_short_lds(int V, int k, int sub, bool fwd) { return (size_t)4 * sub * (fwd ? V / 32 + 2 + 3 * k : 3 * k); }
 
 template <int FMT, bool REST, int TPR> __global__ void __launch_bounds__(256) distill_short_fwd_kernel(rumpy_distill_args a, DsPlan plan) {
@@ -1103,11 +1103,14 @@ extern "C" int64_t rumpy_distill_partial_floats(int64_t rows, int32_t V) {
 // Lanes of a short row; 0: a workgroup a row, or more.  us, bf16, forward + gradient, 16 lanes | 64 lanes | a workgroup a row:
 //   65536 x 100, k 8: 20 + 11 | 87 + 29 | 468 + 218     4096 x 256, k 64: 11 + 7 | 9 + 5 | 40 + 13      300 x 1000, k 8: 11 + 6 | 6 + 4 | 8 + 4
 //   16384 x 1000, k 8: 18 + 14 | 30 + 15 | 113 + 45      1200 x 2000, k 8: 9 + 6 (64) | 14 + 6      300 x 4000, k 8: 11 + 7 (64) | 7 + 4
-//   16384 x 4000, k 64: 50 + 68 (64) | 153 + 59          4096 x 8000, k 64: 27 + 26 (64) | 47 + 27   1200 x 8000, k 8: 19 + 13 (64) | 14 + 9
-// So 16 lanes while a row's columns and entries are few a lane and there are rows for all lanes of the chip; 64 while the rows fill it with a wave each.
-static int ds_short(int64_t rows, int32_t V, int32_t k) {
+//   4096 x 4000, k 64: 18 + 14 (64) | 43 + 18            4096 x 8192, k 8: 24 + 24 (64) | 35 + 23     1200 x 8000, k 8: 19 + 13 (64) | 14 + 9
+//   8192 x 12001, k 8: 54 + 83 (64) | 91 + 75            2048 x 16000, k 8: 28 + 25 (64) | 24 + 22
+// So 16 lanes while a row's columns and entries are few a lane and there are rows for all lanes of the chip; 64 while the rows fill it with a wave each
+// (the gradient, which streams more and has less to do for a row, up to 4096 columns).
+static int ds_short(int64_t rows, int32_t V, int32_t k, bool fwd) {
   if (rows >= 8192 ? V <= (k <= 32 ? 1024 : 512) : V <= 256 && k <= 16) return 16;
-  return V <= 1024 || (V <= 8192 && rows * 4 >= V) ? 64 : 0;
+  if (V <= 1024) return 64;
+  return rows * 4 >= V && V <= (!fwd ? 4096 : rows >= 4096 ? 16384 : 8192) ? 64 : 0;
 }
 template <int FMT, int TPR> static void ds_launch_short_fwd(const rumpy_distill_args& a, const DsPlan& plan, hipStream_t s) {
   constexpr int SUB = 256 / TPR;
@@ -1117,14 +1120,14 @@ template <int FMT, int TPR> static void ds_launch_short_fwd(const rumpy_distill_
   else hipLaunchKernelGGL((distill_short_fwd_kernel<FMT, false, TPR>), grid, dim3(256), lds, s, a, plan);
 }
 template <int FMT> static void ds_launch_bwd(const rumpy_distill_args& a, const DsPlan& plan, hipStream_t s) {
-  const int tpr = ds_short(a.rows, a.V, a.k);
+  const int tpr = ds_short(a.rows, a.V, a.k, false);
   const size_t lds = tpr ? ds_short_lds(a.V, a.k, 256 / tpr, false) : 0;
   if (tpr == 16) hipLaunchKernelGGL((distill_short_bwd_kernel<FMT, 16>), dim3((unsigned)((a.rows + 15) / 16)), dim3(256), lds, s, a, plan);
   else if (tpr == 64) hipLaunchKernelGGL((distill_short_bwd_kernel<FMT, 64>), dim3((unsigned)((a.rows + 3) / 4)), dim3(256), lds, s, a, plan);
   else hipLaunchKernelGGL((distill_bwd_kernel<FMT>), dim3((unsigned)(a.rows * plan.splits)), dim3(DS_WG), 0, s, a, plan);
 }
 template <int FMT> static void ds_launch_fwd(const rumpy_distill_args& a, const DsPlan& plan, hipStream_t s) {
-  const int tpr = ds_short(a.rows, a.V, a.k);
+  const int tpr = ds_short(a.rows, a.V, a.k, true);
   if (tpr == 16) return ds_launch_short_fwd<FMT, 16>(a, plan, s);
   if (tpr == 64) return ds_launch_short_fwd<FMT, 64>(a, plan, s);
   const dim3 grid((unsigned)(a.rows * plan.splits));

@@ -601,7 +601,7 @@ def test_lowest_values_as_masks_at_every_temperature(cols, rest, dtype):
 
 @pytest.mark.parametrize('dtype', [F32, BF16, F16], ids=str)
 @pytest.mark.parametrize('rest', [False, True])
-@pytest.mark.parametrize('rows,cols,k', [(8197, 100, 64), (8200, 600, 8), (8193, 7, 7), (8209, 1, 1), (1201, 4800, 256), (501, 2000, 3), (4099, 256, 16)])
+@pytest.mark.parametrize('rows,cols,k', [(8197, 100, 64), (8200, 600, 8), (8193, 7, 7), (8209, 1, 1), (1201, 4800, 256), (501, 2000, 3), (4099, 256, 16), (4100, 8193, 20)])
 def test_many_short_rows(rows, cols, k, rest, dtype):
     """rows that share a wave or hold one alone, the last group not full: padded rows, unused entries, columns named twice, slices at any address"""
     g = torch.Generator().manual_seed(rows + cols)
