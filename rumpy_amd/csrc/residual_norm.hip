@@ -371,26 +371,43 @@ template <int XF, int TF, int TPR, int MODE> __global__ void __launch_bounds__(T
 }
 
 // out[c] = sum over consecutive partial rows: items 0..3 = the parameters (all workgroups), 4.. = the gate rows.  16 waves share a column's rows:
-// with four a sum of 461 rows took 7 us of dependent loads.
-constexpr int RN_SLICES = 16;
-__global__ void __launch_bounds__(64 * RN_SLICES) residual_norm_reduce_kernel(rumpy_residual_norm_bwd_args a, RnPlan plan, int tiles) {
+// with four a sum of 461 rows took 7 us of dependent loads.  Where there are many gate rows (`flat`), each of a few partial rows, a thread takes an element
+// of one: a workgroup for 64 of them took 81 us for 32768 gate rows of 64 channels, 1650 for 700000 of 3; so 9 and 11.
+constexpr int RN_SLICES = 16, RN_REDUCE_WG = 64 * RN_SLICES;
+constexpr int64_t RN_FLAT = 16384;            // elements of gate rows from which on a thread takes one
+__device__ __forceinline__ const float* gate_partials(const rumpy_residual_norm_bwd_args& a, const RnPlan& plan, int64_t group, int64_t& count) {
+  const int64_t first = group * a.group_rows, last = min(a.rows, first + a.group_rows) - 1;
+  const float* src = a.partial + (size_t)4 * plan.wgs * a.C;
+  if (plan.direct) { count = last - first + 1; return src + (size_t)first * a.C; }
+  const int64_t w0 = first / plan.rpw, w1 = last / plan.rpw;
+  count = w1 - w0 + 1;
+  return src + (size_t)(w0 + group) * a.C;
+}
+__global__ void __launch_bounds__(RN_REDUCE_WG) residual_norm_reduce_kernel(rumpy_residual_norm_bwd_args a, RnPlan plan, int tiles, int64_t flat) {
   __shared__ float red[RN_SLICES][64];
   const size_t item = blockIdx.x / tiles;
-  const int lane = threadIdx.x & 63, slice = threadIdx.x >> 6, c = (blockIdx.x % tiles) * 64 + lane;
-  const size_t wc = (size_t)plan.wgs * a.C;
   const float* src;
   float* dst;
   int64_t count;
+  if (item >= 4 && flat) {
+    const int64_t e0 = (int64_t)(blockIdx.x - 4 * tiles) * RN_REDUCE_WG, e = e0 + threadIdx.x, g0 = e0 / a.C;
+    if (e >= flat) return;                                     // (no barrier on this way)
+    const uint32_t off = (uint32_t)(e0 - g0 * a.C) + threadIdx.x;
+    src = gate_partials(a, plan, g0 + off / (uint32_t)a.C, count) + off % (uint32_t)a.C;
+    float s = 0.f;
+#pragma unroll 4
+    for (int64_t i = 0; i < count; ++i) s += src[(size_t)i * a.C];
+    ((float*)a.dgate)[e] = s;
+    return;
+  }
+  const int lane = threadIdx.x & 63, slice = threadIdx.x >> 6, c = (blockIdx.x % tiles) * 64 + lane;
   if (item < 4) {
     dst = item == 0 ? a.d_post_w : item == 1 ? a.d_post_b : item == 2 ? a.d_pre_w : a.d_pre_b;
-    src = a.partial + item * wc;
+    src = a.partial + item * (size_t)plan.wgs * a.C;
     count = plan.wgs;
   } else {
-    const int64_t group = (int64_t)item - 4, first = group * a.group_rows, last = min(a.rows, first + a.group_rows) - 1;
-    dst = a.dgate ? (float*)a.dgate + group * a.C : nullptr;
-    src = a.partial + 4 * wc;
-    if (plan.direct) { src += (size_t)first * a.C; count = last - first + 1; }
-    else { const int64_t w0 = first / plan.rpw, w1 = last / plan.rpw; src += (size_t)(w0 + group) * a.C; count = w1 - w0 + 1; }
+    dst = (float*)a.dgate + (item - 4) * a.C;
+    src = gate_partials(a, plan, (int64_t)item - 4, count);
   }
   if (!dst) return;                                            // (the whole workgroup)
   float s = 0.f;
@@ -514,12 +531,13 @@ extern "C" int rumpy_residual_norm_bwd(const rumpy_residual_norm_bwd_args* p, vo
   const RnPlan plan = bad ? RnPlan{} : rn_plan(p->rows, p->group_rows, p->C, p->gate_mode);
   const bool gate_rows = !bad && p->gate_mode == RN_GATE_GROUP && p->dgate && !(plan.direct && p->group_rows == 1);
   const int tiles = bad ? 0 : (p->C + 63) / 64;
-  const int64_t items = 4 + (gate_rows ? p->rows / p->group_rows : 0);
-  if (!bad && items * tiles > 0x7fffffff) bad = "too many gate rows";
+  const int64_t groups = gate_rows ? p->rows / p->group_rows : 0, elements = groups > 1 ? groups * p->C : 0, flat = elements >= RN_FLAT ? elements : 0;
+  const int64_t blocks = (flat ? 4 : 4 + groups) * tiles + (flat + RN_REDUCE_WG - 1) / RN_REDUCE_WG;
+  if (!bad && blocks > 0x7fffffff) bad = "too many gate rows";
   if (bad) { rumpy_set_error("rumpy_residual_norm_bwd: %s", bad); return RUMPY_E_ARG; }
   hipStream_t s = (hipStream_t)stream;
   RN_BY_FORMAT(rn_launch_bwd, *p, plan, s);
   if (gate_rows || p->d_post_w || p->d_post_b || p->d_pre_w || p->d_pre_b)
-    hipLaunchKernelGGL(residual_norm_reduce_kernel, dim3((unsigned)(items * tiles)), dim3(64 * RN_SLICES), 0, s, *p, plan, tiles);
+    hipLaunchKernelGGL(residual_norm_reduce_kernel, dim3((unsigned)blocks), dim3(RN_REDUCE_WG), 0, s, *p, plan, tiles, flat);
   return rumpy_check_launch("rumpy_residual_norm_bwd");
 }

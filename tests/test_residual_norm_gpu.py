@@ -550,3 +550,10 @@ def test_an_infinity_in_a_row_stays_in_it(kind, c):
     for a, b in ((y2, clean[0]), (h2, clean[1])):
         assert torch.equal(a[[0, 1, 2, 3, 5]], b[[0, 1, 2, 3, 5]])
     assert torch.equal(h[keep], alone[keep])
+
+
+@pytest.mark.parametrize('shape', [(700, 40, 64), (3000, 2, 130), (9000, 3, 5), (513, 4, 40), (40, 3, 8192), (5, 1000, 4100), (300, 33, 513)])
+def test_many_gate_rows(shape):
+    """gate rows that serve a few rows each, in number: their partial rows lie in one workgroup's part or at the border of two"""
+    _run_and_check(shape, BF16, BF16, 'group', 'layer', 'layer', True, 0.7)
+    _run_and_check(shape, F32, F32, 'group', None, 'rms', True, -0.4, with_dy=False)
