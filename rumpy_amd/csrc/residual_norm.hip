@@ -234,8 +234,17 @@ template <int TPR> __device__ __forceinline__ void flush_columns(const RnLane<TP
 constexpr int RN_ALL = 1, RN_ALL_FULL = 2;
 template <int XF, int TF, int TPR, int MODE> __global__ void __launch_bounds__(TPR <= 64 ? 256 : TPR) residual_norm_bwd_kernel(rumpy_residual_norm_bwd_args a, RnPlan plan) {
   constexpr int WG = TPR <= 64 ? 256 : TPR, SUB = WG / TPR;
-  // 1024 threads leave 128 registers each: the sums alone stay there, parameters come from the caches per row and nothing is asked for ahead
+  // 1024 threads leave 128 registers each: the parameters' sums lie in LDS (each thread's own, 128 KB; 1024 x 8192 bf16:
+  // 56 us with spills instead, 30), parameters come from the caches per row and nothing is asked for ahead
   constexpr bool HOLD = TPR <= 512;
+  __shared__ float4 sums[HOLD ? 1 : 4 * 2 * TPR];
+  auto add = [&](int which, const float (&v)[8]) {
+    float4* p = sums + which * 2 * TPR + threadIdx.x;
+    float4 lo = p[0], hi = p[TPR];
+    lo.x += v[0]; lo.y += v[1]; lo.z += v[2]; lo.w += v[3];
+    hi.x += v[4]; hi.y += v[5]; hi.z += v[6]; hi.w += v[7];
+    p[0] = lo; p[TPR] = hi;
+  };
   __shared__ float red[2][2 * RowSum<TPR>::WAVES];
   __shared__ float cols[TPR <= 64 ? 4 * TPR * 8 : 1];
   RowSum<TPR> sum{red, 0};
@@ -274,6 +283,9 @@ template <int XF, int TF, int TPR, int MODE> __global__ void __launch_bounds__(T
 #pragma unroll
   for (int i = 0; i < 8; ++i) { aw[i] = ab[i] = awp[i] = abp[i] = ag[i] = t[i] = d[i] = e[i] = 0.f; g[i] = 1.f; }
   if (HOLD) { lane.params(a.post_w, 1.f, wp); lane.params(a.post_b, 0.f, bp); lane.params(a.pre_w, 1.f, w); }
+  else {
+    for (int i = 0; i < 8; ++i) sums[i * TPR + threadIdx.x] = make_float4(0.f, 0.f, 0.f, 0.f);
+  }
   // one step: SUB rows; those behind the segment repeat its last row, `live` takes them out of the column sums (TAIL steps alone have any)
   auto step = [&](size_t r, bool live, auto tail) {
     constexpr bool TAIL = decltype(tail)::value;
@@ -297,12 +309,16 @@ template <int XF, int TF, int TPR, int MODE> __global__ void __launch_bounds__(T
       for (int i = 0; i < 8; ++i) {
         x[i] = (x[i] - st.z) * st.w;                                              // yhat
         const float ea = TAIL && !live ? 0.f : e[i];
-        ab[i] += ea;
-        aw[i] = fmaf(ea, x[i], aw[i]);
+        if (HOLD) { ab[i] += ea; aw[i] = fmaf(ea, x[i], aw[i]); }
+        else { ab[i] = ea; aw[i] = ea * x[i]; }
         e[i] *= w[i];
         const float em = lane.once(e[i], i);
         s1 += em;
         s2 = fmaf(em, x[i], s2);
+      }
+      if (!HOLD) {
+        if (a.d_pre_w) add(2, aw);
+        if (a.d_pre_b) add(3, ab);
       }
       sum.two(s1, s2);
       s1 = a.pre == RN_LAYER ? s1 * inv_c : 0.f;
@@ -320,11 +336,16 @@ template <int XF, int TF, int TPR, int MODE> __global__ void __launch_bounds__(T
         const float dd = a.scale * d[i];
         gr[i] = dd * fmaf(t[i], wp[i], bp[i]);
         const float dz = g[i] * dd;
-        if (!TAIL || live) { ag[i] += gr[i]; abp[i] += dz; awp[i] = fmaf(dz, t[i], awp[i]); }
+        if (!HOLD) { ag[i] += gr[i]; abp[i] = dz; awp[i] = dz * t[i]; }
+        else if (!TAIL || live) { ag[i] += gr[i]; abp[i] += dz; awp[i] = fmaf(dz, t[i], awp[i]); }
         d[i] = dz * wp[i];
         const float dm = lane.once(d[i], i);
         s1 += dm;
         s2 = fmaf(dm, t[i], s2);
+      }
+      if (!HOLD) {
+        if (a.d_post_w) add(0, awp);
+        if (a.d_post_b) add(1, abp);
       }
       if (MODE == RN_ALL_FULL || (full && a.dgate)) lane.template store<TF>(a.dgate, r * a.C, gr);
       else if (direct && a.dgate) lane.template store<RUMPY_FMT_F32>(gpart, r * a.C, gr);
@@ -361,6 +382,13 @@ template <int XF, int TF, int TPR, int MODE> __global__ void __launch_bounds__(T
     }
     if (group_sums && a.dgate) flush_columns<TPR>(lane, ag, gpart + (blockIdx.x + group) * a.C, cols);
     seg = end;
+  }
+  if (!HOLD) {
+    auto get = [&](int which, float (&v)[8]) {
+      const float4 lo = sums[which * 2 * TPR + threadIdx.x], hi = sums[(which * 2 + 1) * TPR + threadIdx.x];
+      v[0] = lo.x; v[1] = lo.y; v[2] = lo.z; v[3] = lo.w; v[4] = hi.x; v[5] = hi.y; v[6] = hi.z; v[7] = hi.w;
+    };
+    get(0, awp); get(1, abp); get(2, aw); get(3, ab);
   }
   const size_t wc = (size_t)plan.wgs * a.C;
   float* mine = a.partial + (size_t)blockIdx.x * a.C;
