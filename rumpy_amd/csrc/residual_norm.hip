@@ -49,9 +49,10 @@ template <int TPR> struct RowSum {
 
 // Where a lane's 8 channels lie.  The last piece of a row is moved back to end with the row, and lanes behind it repeat it: every access is one
 // whole 16- or 32-byte access inside the row, with no branch around it.  What two lanes both hold they compute and store alike; in a row's sums
-// the repeated elements count zero times (`m`, bits and not factors: an infinity is not made NaN).  Rows of less than 8 channels have one lane (TPR 1) and partial accesses.
+// the repeated elements count zero times (`m`, bits and not factors: an infinity is not made NaN).  Rows of up to 8 channels have one lane
+// (TPR 1), with partial accesses under 8.
 template <int TPR> struct RnLane {
-  int at, n;             // first channel; channels of a partial access (TPR 1)
+  int at, n;             // first channel; channels of an access (TPR 1)
   uint32_t m[8];
   __device__ __forceinline__ explicit RnLane(int C) {
     const int col = ((int)threadIdx.x % TPR) * 8;
@@ -178,9 +179,11 @@ template <int XF, int TF, int TPR, int MODE> __global__ void __launch_bounds__(T
 // of the group and stored as partial row (workgroup + group): over the walk of all (workgroup, group) pairs that number grows strictly.  Groups
 // shorter than a workgroup's step store one partial row per row instead (groups of one row: the gradient itself).
 struct RnPlan { int tpr, sub, wgs, rpw; bool direct; };
+// As few lanes a row as hold it: with 8 at the least, 1048576 x 8 bf16 took 51 us forward and 102 backward, now 15 and 32; 524288 x 16 29 and 55, now 13 and 22
+// (rows of 3 channels, in partial accesses, stay at 2.5 and 5 times their bytes).
 static RnPlan rn_plan(int64_t rows, int64_t group_rows, int32_t C, int gate_mode) {
   RnPlan p;
-  p.tpr = C < 8 ? 1 : 8;
+  p.tpr = 1;
   while (p.tpr * 8 < C) p.tpr *= 2;
   p.sub = p.tpr <= 64 ? 256 / p.tpr : 1;
   const int64_t steps = (rows + p.sub - 1) / p.sub;
@@ -197,6 +200,11 @@ static RnPlan rn_plan(int64_t rows, int64_t group_rows, int32_t C, int gate_mode
 // sum over the lanes of a wave that hold the same channels of different rows (every TPR-th lane), in each of them, without the LDS crossbar
 template <int TPR> __device__ __forceinline__ float steps_sum(float v, int lane) {
   if constexpr (TPR == 1) return wave64_sum(v, lane);
+  if constexpr (TPR == 2) v += dpp_quad2(v);                                             // lane ^ 2
+  if constexpr (TPR <= 4) {
+    const int i = __float_as_int(v);
+    v += __int_as_float(__builtin_amdgcn_update_dpp(i, i, 0x124, 0xF, 0xF, false));      // row_ror 4: with the next step all four of a row's
+  }
   if constexpr (TPR <= 8) {
     const int i = __float_as_int(v);
     v += __int_as_float(__builtin_amdgcn_update_dpp(i, i, 0x128, 0xF, 0xF, false));      // row_ror 8: lane ^ 8
@@ -469,7 +477,7 @@ static const char* rn_check(int64_t rows, int64_t group_rows, int32_t C, int x_f
   return nullptr;
 }
 
-// the usual calls have kernels of their own, from 8 channels on
+// the usual calls have kernels of their own, from 9 channels on
 template <int XF, int TF, int TPR> static void rn_launch_fwd_tpr(const rumpy_residual_norm_args& a, const dim3& grid, hipStream_t s) {
   const dim3 wg(TPR <= 64 ? 256 : TPR);
   if (TPR > 1 && a.t && a.pre != RN_NONE) {
@@ -493,6 +501,8 @@ template <int XF, int TF> static void rn_launch_fwd(const rumpy_residual_norm_ar
   const dim3 grid((unsigned)(steps < most ? steps : most));
   switch (p.tpr) {
     case 1: return rn_launch_fwd_tpr<XF, TF, 1>(a, grid, s);
+    case 2: return rn_launch_fwd_tpr<XF, TF, 2>(a, grid, s);
+    case 4: return rn_launch_fwd_tpr<XF, TF, 4>(a, grid, s);
     case 8: return rn_launch_fwd_tpr<XF, TF, 8>(a, grid, s);
     case 16: return rn_launch_fwd_tpr<XF, TF, 16>(a, grid, s);
     case 32: return rn_launch_fwd_tpr<XF, TF, 32>(a, grid, s);
@@ -506,6 +516,8 @@ template <int XF, int TF> static void rn_launch_fwd(const rumpy_residual_norm_ar
 template <int XF, int TF> static void rn_launch_bwd(const rumpy_residual_norm_bwd_args& a, const RnPlan& p, hipStream_t s) {
   switch (p.tpr) {
     case 1: return rn_launch_bwd_tpr<XF, TF, 1>(a, p, s);
+    case 2: return rn_launch_bwd_tpr<XF, TF, 2>(a, p, s);
+    case 4: return rn_launch_bwd_tpr<XF, TF, 4>(a, p, s);
     case 8: return rn_launch_bwd_tpr<XF, TF, 8>(a, p, s);
     case 16: return rn_launch_bwd_tpr<XF, TF, 16>(a, p, s);
     case 32: return rn_launch_bwd_tpr<XF, TF, 32>(a, p, s);

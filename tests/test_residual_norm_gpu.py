@@ -557,3 +557,11 @@ def test_many_gate_rows(shape):
     """gate rows that serve a few rows each, in number: their partial rows lie in one workgroup's part or at the border of two"""
     _run_and_check(shape, BF16, BF16, 'group', 'layer', 'layer', True, 0.7)
     _run_and_check(shape, F32, F32, 'group', None, 'rms', True, -0.4, with_dy=False)
+
+
+@pytest.mark.parametrize('c', [7, 8, 9, 15, 16, 17, 31, 32, 33])
+def test_few_channels(c):
+    """one, two, four and eight lanes a row, their rows summed over a wave and over workgroups; groups that end inside a wave's step"""
+    for gate, shape in (('none', (1, 1031, c)), ('channel', (3, 700, c)), ('group', (9, 130, c)), ('group', (5, 300, c)), ('full', (1, 517, c))):
+        _run_and_check(shape, BF16, BF16, gate, 'layer', 'rms', True, 0.7)
+        _run_and_check(shape, F32, F16, gate, 'rms', 'layer', True, 0.7, lay=lambda n, t: torch.nn.functional.pad(t, (1, 2))[..., 1:-2] if t.dim() > 2 else t)
