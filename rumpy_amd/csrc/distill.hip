@@ -3,7 +3,7 @@
 // when `tail` is given, the rest of the columns as one more outcome of probability p_t):
 //   l = tau^2 [ sum_i p_i (log p_i - log q_i) + p_t (log p_t - log q_t) ],   q_t = sum of q over the columns that are not listed
 //   dl/dz_j = tau (q_j - p_j) listed ;  tau q_j (1 - p_t / q_t) not listed       (no tail: p_t = 0, sum p = 1)
-// Rows are [V] fp32 / bf16 / fp16 of 8192 (the contrastive queue) to a few 100 000 columns.  Selection and loss read each row once (the
+// Rows are [V] fp32 / bf16 / fp16 of a few classes, 8192 keys (the contrastive queue) or a few 100 000 columns.  Selection and loss read each row once (the
 // selection's second look comes from registers), the gradient reads it once and writes it once: bound by memory, with one exponential per element
 // and direction beside it.  The sum of exp runs over the row once with a running maximum per thread; q_t is summed directly over the columns
 // that are not listed (a bit map of them lies in LDS): 1 - sum q_i would cancel where the listed columns hold nearly everything.

@@ -647,3 +647,23 @@ def test_top_logits_of_short_rows(rows, cols, ks, dtype):
     z = z.to(dtype).to(DEV)[:, 3:3 + cols]
     for k in ks:
         _check_top(z, k, 0.5)
+
+
+@pytest.mark.parametrize('rows,cols', [(9000, 300), (700, 900)])
+def test_short_rows_captured_and_on_other_streams(rows, cols):
+    g = torch.Generator().manual_seed(rows)
+    z, t = (torch.randn(rows, cols, generator=g).to(DEV) for _ in range(2))
+    _pass(z, t, 20, 1.0)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = _pass(z, t, 20, 1.0)
+    for i in range(3):
+        z.copy_(torch.randn(rows, cols, generator=g))
+        graph.replay()
+        torch.cuda.synchronize()
+        side = torch.cuda.Stream()
+        with torch.cuda.stream(side):
+            other = _pass(z, t, 20, 1.0)
+        side.synchronize()
+        want = _pass(z, t, 20, 1.0)
+        assert all(torch.equal(a, b) and torch.equal(b, c) for a, b, c in zip(out, want, other))
