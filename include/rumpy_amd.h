@@ -740,7 +740,8 @@ int rumpy_residual_norm_bwd(const rumpy_residual_norm_bwd_args* a, void* stream)
 int64_t rumpy_residual_norm_partial_floats(int64_t rows, int64_t group_rows, int32_t C, int32_t gate_mode);
 
 /* ---- distillation from a teacher's top logits (csrc/distill.hip), beside rumpy_ce_rows: rows of V logits in fp32 / bf16 / fp16 with a row stride
- * (columns contiguous, any alignment of an element), all sums in fp32, fixed orders.
+ * (columns contiguous, any alignment of an element); the columns' exponentials and sums in fp32, a row's listed entries, logarithms and joins and the sums
+ * over rows in 64 bits, fixed orders.
  * rumpy_top_logits: per row the k <= 256 largest logits, descending, equal ones by index (NaN counts as largest), as they are in `values`
  * [rows, k] (the logits' format) with int64 `indices`; tail[r] = log of the sum of exp(logit / tau) over all others (-inf: none).
  * work: rumpy_top_logits_work_bytes(rows, V, k) bytes (0: NULL). */

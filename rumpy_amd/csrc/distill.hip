@@ -7,8 +7,8 @@
 // selection's second look comes from registers), the gradient reads it once and writes it once: bound by memory, with one exponential per element
 // and direction beside it.  The sum of exp runs over the row once with a running maximum per thread; q_t is summed directly over the columns
 // that are not listed (a bit map of them lies in LDS): 1 - sum q_i would cancel where the listed columns hold nearly everything.
-// Exponentials and a row's sums are fp32, a row's logarithms and the sums over rows 64-bit.  Every reduction has a fixed order, which goes with the
-// call's sizes and the alignment of a row's address alone: results are bitwise reproducible.
+// The columns' exponentials and their sum are fp32; what is listed, a row's logarithms and joins and the sums over rows are 64-bit.  Every reduction has a
+// fixed order, which goes with the call's sizes and the alignment of a row's address alone: results are bitwise reproducible.
 #include "row_vec.hpp"
 
 constexpr int DS_MAXK = 256, DS_MAXV = 1 << 30;
@@ -579,8 +579,9 @@ extern "C" int rumpy_top_logits(const rumpy_top_logits_args* p, void* stream) {
 
 // ================================================================================================================ loss and gradient
 constexpr int DS_WG = 512, DS_WAVES = DS_WG / 64;
-constexpr int DS_STATE = 8;      // per row: reference and coefficient of the streamed columns, maximum and log sum of all, the teacher's log sum, dead, the teacher's maximum,
-                                 // whether a column may be listed twice
+constexpr int DS_STATE = 8;      // per row: reference and coefficient of the streamed columns, maximum of all and 1 / sum, the teacher's factor beside its maximum, dead, the
+                                 // teacher's maximum, whether a column may be listed twice
+constexpr double DS_LEAST = -126.0 / LOG2E;      // exponents below it count as 0, as the columns' own do
 
 // exp((v - m) / tau), v <= m, with c + lo = log2(e) / tau: c alone, rounded to 32 bits, is another temperature for the whole row, and its error of up to
 // 2^-25 does not average out in the loss (1.8e-6 of it where 32-bit divisions made 2e-7).  The difference first: no digits are lost where a row lies
@@ -592,7 +593,7 @@ __device__ __forceinline__ float ds_exp(float v, float m, float c, float lo) {
 // the factor from a sum relative to m to one relative to M >= m (m = -inf: there is no sum yet; M = inf: NaN, by the sum itself)
 __device__ __forceinline__ float ds_rescale(float m, float M, float c, float lo) { return m == -INFINITY ? 0.f : m == M ? 1.f : ds_exp(m, M, c, lo); }
 
-struct DsPlan { int splits, seg; float c, lo, near, inv_tau; double inv_tau64; };      // c + lo = log2(e) / tau; near: the nearest float to it
+struct DsPlan { int splits, seg; float c, lo, near; double inv_tau; };      // c + lo = log2(e) / tau; near: the nearest float to it
 // rows are cut when there are too few of them to fill the chip; a piece's bit map of listed columns has to fit LDS (2^18 columns: 32 KB)
 static DsPlan ds_plan(int64_t rows, int32_t V, double tau) {
   DsPlan p;
@@ -601,8 +602,7 @@ static DsPlan ds_plan(int64_t rows, int32_t V, double tau) {
   p.near = (float)x;
   p.c = (double)p.near > x ? nextafterf(p.near, 0.f) : p.near;
   p.lo = fmaxf((float)(x - p.c), p.c * 1e-12f);
-  p.inv_tau64 = 1.0 / tau;
-  p.inv_tau = (float)p.inv_tau64;
+  p.inv_tau = 1.0 / tau;
   int64_t s = rows > 0 ? (512 + rows - 1) / rows : 1;
   const int64_t most = (V + 8191) / 8192, least = ((int64_t)V + (1 << 18) - 1) >> 18;
   if (s > most) s = most;
@@ -653,14 +653,29 @@ template <int FMT> __device__ __forceinline__ int ds_load_listed(const rumpy_dis
   return mine;
 }
 
+// sum over the L neighbouring lanes of a row (16 or 64), in every one of them: lanes_sum's order in 64 bits
+template <typename Move> __device__ __forceinline__ double moved(double v, Move move) {
+  return __hiloint2double(__float_as_int(move(__int_as_float(__double2hiint(v)))), __float_as_int(move(__int_as_float(__double2loint(v)))));
+}
+template <int L> __device__ __forceinline__ double lanes_sum64(double v, int lane) {
+  v += moved(v, dpp_quad1); v += moved(v, dpp_quad2); v += moved(v, dpp_half_mirror); v += moved(v, dpp_row_mirror);
+  if constexpr (L == 64) {
+    v += moved(v, [&](float x) { return lane_xor16(x, lane >> 4); });
+    v += moved(v, [&](float x) { return lane_xor32(x, lane); });
+  }
+  return v;
+}
+
 // L lanes of one wave: the row's loss and what its gradient needs, from the sum over the streamed columns (all of them, or the unlisted ones when the
-// rest is an outcome): s = sum exp((z - m) / tau).  The logarithms and their sum are made in 64 bits: the loss is a small difference of them.
+// rest is an outcome): s = sum exp((z - m) / tau).  With the rest as an outcome the loss is of second order in the difference of the two distributions,
+// and so is all that s's rounding costs it as long as each distribution sums to 1: what is listed and the joined sums are made in 64 bits.  (In 32 bits they
+// left an error of the first order: 2^-24 tau^2, 5e-4 of the loss of 3 x 168911 columns, 1 listed, tau 4, where it is 2e-7 now; 65536 x 100, 8 listed: 20 us
+// then, 23 now; 16384 x 1000 17 and 18.)
 // idx, v, z: what the teacher lists, in LDS; first(i): no earlier entry names entry i's column; doubled: some column may be named twice.
 template <int L, typename First>
 __device__ __forceinline__ void ds_finish(const rumpy_distill_args& a, const DsPlan& plan, int64_t row, const int* idx, const float* v, const float* z, First first,
                                           bool doubled, float m, float s, int lane) {
-  const float c = plan.c, lo = plan.lo;
-  const double inv_tau = plan.inv_tau64;
+  const double inv_tau = plan.inv_tau;
   const bool rest = a.tail != nullptr;
   const float w = a.row_weight ? a.row_weight[row] : 1.f;
   float vm = -INFINITY, zm = -INFINITY;
@@ -681,40 +696,44 @@ __device__ __forceinline__ void ds_finish(const rumpy_distill_args& a, const DsP
     if (lane % L == 0) { a.row_loss[row] = 0.f; st[0] = st[1] = st[2] = st[3] = st[4] = 0.f; st[5] = 1.f; }
     return;
   }
-  // the teacher's logarithms relative to its largest logit, so that far from zero no digits are lost: lp = (v - vm) / tau - up - ln_p
+  // the teacher's logarithms relative to its largest logit, so that far from zero no digits are lost: log p = (v - vm) / tau - up - log P
   // (up: the tail where it is the larger, or all there is)
   const bool tail_alone = vm == -INFINITY;
   if (tail_alone) vm = 0.f;
   const double tr = tl - vm * inv_tau, up = tr > 0.0 || tail_alone ? tr : 0.0;
   const float M = rest ? fmaxf(m, zm) : m;
-  float p_sum = 0.f, sl = 0.f;
+  double p_listed = 0.0, q_listed = 0.0, loss = 0.0;          // sums of the listed p and q up to the factors 1 / P and 1 / S, and of p times the difference of their exponents
   for (int i = lane % L; i < a.k; i += L) {
     if (idx[i] < 0) continue;
-    p_sum += __builtin_amdgcn_exp2f((float)((((double)v[i] - vm) * inv_tau - up) * LOG2E));
-    if (rest && first(i)) sl += ds_exp(z[i], M, c, lo);
+    const double lp = ((double)v[i] - vm) * inv_tau - up, lq = ((double)z[i] - M) * inv_tau;
+    if (!(lp < DS_LEAST)) {
+      const double e = exp(lp);
+      p_listed += e;
+      loss += e * (lp - lq);
+    }
+    if (rest && first(i)) q_listed += exp(lq);
   }
-  p_sum = lanes_sum<L>(p_sum, lane) + (rest ? __builtin_amdgcn_exp2f((float)((tr - up) * LOG2E)) : 0.f);
-  nan |= p_sum != p_sum;                                   // (infinite logits of the teacher)
-  float S = s;
-  if (rest) S = lanes_sum<L>(sl, lane) + (m == -INFINITY ? 0.f : s * ds_rescale(m, M, c, lo));
-  // (the three logarithms in three lanes at once: one after another they were a third of a short row's time)
-  const double ln = log((double)(lane % 4 == 0 ? p_sum : lane % 4 == 1 ? S : s));
-  const double ln_p = __shfl(ln, 0, L), ln_s = __shfl(ln, 1, L), ln_r = __shfl(ln, 2, L);
-  double loss = 0.0;
-  for (int i = lane % L; i < a.k; i += L) {
-    if (idx[i] < 0) continue;
-    const double lp = ((double)v[i] - vm) * inv_tau - up - ln_p;
-    const float p = __builtin_amdgcn_exp2f((float)(lp * LOG2E));
-    if (p != 0.f) loss += p * (lp - (((double)z[i] - M) * inv_tau - ln_s));
-  }
-#pragma unroll
-  for (int o = 1; o < L; o *= 2) loss += __shfl_xor(loss, o);
-  float coef = 1.f / S;
+  p_listed = lanes_sum64<L>(p_listed, lane);
+  loss = lanes_sum64<L>(loss, lane);
+  // (the row's three exponentials, and its three logarithms, in three lanes at once: one after another the logarithms were a third of a short row's time)
+  const double to_m = m == -INFINITY ? (double)-INFINITY : ((double)m - M) * inv_tau, to_rest = tr - up;
+  double P = p_listed, S = s, p_rest = 0.0, q_rest = 0.0, beside = 1.0;          // beside: of the listed entries' exponents, relative to the teacher's largest logit
   if (rest) {
-    const double lpt = tr - up - ln_p, lqt = m == -INFINITY ? (double)-INFINITY : ((double)m - M) * inv_tau + ln_r - ln_s;
-    const float pt = __builtin_amdgcn_exp2f((float)(lpt * LOG2E)), qt = __builtin_amdgcn_exp2f((float)(lqt * LOG2E));
-    if (pt != 0.f) loss += pt * (lpt - lqt);
-    coef = m == -INFINITY ? 0.f : (qt - pt) / s;
+    const double ex = exp(lane % 4 == 0 ? to_rest : lane % 4 == 1 ? to_m : -up);
+    p_rest = to_rest < DS_LEAST ? 0.0 : __shfl(ex, 0, L);
+    q_rest = m == -INFINITY ? 0.0 : s * __shfl(ex, 1, L);
+    beside = __shfl(ex, 2, L);
+    P += p_rest;
+    S = lanes_sum64<L>(q_listed, lane) + q_rest;
+  }
+  nan |= P != P;                                           // (infinite logits of the teacher)
+  const double ln = log(lane % 4 == 0 ? P : lane % 4 == 1 ? S : (double)s);
+  const double ln_p = __shfl(ln, 0, L), ln_s = __shfl(ln, 1, L), ln_r = __shfl(ln, 2, L), one_p = 1.0 / P, one_s = 1.0 / S;
+  loss = (loss - p_listed * (ln_p - ln_s)) * one_p;
+  float coef = (float)one_s;
+  if (rest) {
+    if (p_rest != 0.0) loss += p_rest * one_p * ((to_rest - ln_p) - (to_m + ln_r - ln_s));
+    coef = m == -INFINITY ? 0.f : (float)(q_rest * one_s - p_rest * one_p) / s;
   }
   if (nan) loss = coef = NOT_A_NUMBER;
   if (lane % L == 0) {
@@ -722,8 +741,8 @@ __device__ __forceinline__ void ds_finish(const rumpy_distill_args& a, const DsP
     st[0] = m == -INFINITY ? 0.f : m;
     st[1] = coef;
     st[2] = M;
-    st[3] = nan ? coef : (float)ln_s;
-    st[4] = (float)(up + ln_p);
+    st[3] = nan ? coef : (float)one_s;
+    st[4] = tail_alone ? 0.f : (float)(beside * one_p);
     st[5] = w == 0.f ? 1.f : 0.f;
     st[6] = vm;
     st[7] = doubled ? 1.f : 0.f;
@@ -868,7 +887,7 @@ template <int FMT> __global__ void __launch_bounds__(DS_WG) distill_join_kernel(
 
 // ---- many short rows: TPR lanes of a wave a row, 8 columns each at a time; several rows a workgroup, none of which waits for another.
 // A row's fixed work (what is listed, three 64-bit logarithms, the state) is as long as its columns': with a workgroup a row, 65536 x 100 fp32 took 468 us
-// forward and 218 backward, with 16 lanes 20 and 11.  Pieces are laid out as in a row of channels: the last one is moved back to end with the row, what it repeats is left out.
+// forward and 218 backward, with 16 lanes 23 and 11.  Pieces are laid out as in a row of channels: the last one is moved back to end with the row, what it repeats is left out.
 template <int FMT, int TPR> struct DsShortRow {
   const typename RowElem<FMT>::type* z;
   int V, l;
@@ -994,14 +1013,14 @@ template <int FMT> __global__ void __launch_bounds__(DS_WG) distill_bwd_kernel(r
     for (int64_t j = j0 + tid * 8; j < j1; j += DS_WG * 8) store8<FMT>(a.dlogits, out + j, (int)min((int64_t)8, j1 - j), zero);
     return;
   }
-  const float c = plan.near;
+  const float c = plan.near;               // (the row's stream)
   float g = (a.loss ? *a.gout * *a.factor : a.gout[row]) * (float)a.tau;
   if (a.row_weight) g *= a.row_weight[row];
   const float m = st[0], coef = g * st[1];
   if (tid < a.k) {
     const int64_t i = ds_index(a, row, tid);
     idx[tid] = i >= j0 && i < j1 ? (int)i : -1;
-    p[tid] = i < 0 ? 0.f : __builtin_amdgcn_exp2f(((ds_value(a, row, tid) - st[6]) * plan.inv_tau - st[4]) * LOG2E_F);
+    p[tid] = i < 0 ? 0.f : ds_exp(ds_value(a, row, tid), st[6], plan.c, plan.lo) * st[4];
   }
   for (int64_t j = j0 + tid * 8; j < j1; j += DS_WG * 8) {
     const int n = (int)min((int64_t)8, j1 - j);
@@ -1023,7 +1042,7 @@ template <int FMT> __global__ void __launch_bounds__(DS_WG) distill_bwd_kernel(r
 #pragma unroll
       for (int i = 0; i < 16; ++i) share += o + i < a.k && other[i] == mine ? po[i] : 0.f;
     }
-    const float q = __builtin_amdgcn_exp2f(((elem_to_f32<FMT>(z[idx[tid]]) - st[2]) * plan.inv_tau - st[3]) * LOG2E_F);
+    const float q = ds_exp(elem_to_f32<FMT>(z[idx[tid]]), st[2], plan.c, plan.lo) * st[3];
     reinterpret_cast<E*>(a.dlogits)[out + idx[tid]] = f32_to_elem<FMT>(g * (q - share));
   }
 }
@@ -1051,8 +1070,8 @@ template <int FMT, int TPR> __global__ void __launch_bounds__(256) distill_short
       const int64_t j = ds_index(a, row, i);
       const bool inside = j >= 0 && j < a.V;
       idx[i] = inside ? (int)j : -1;
-      p[i] = j < 0 ? 0.f : __builtin_amdgcn_exp2f(((ds_value(a, row, i) - st[6]) * plan.inv_tau - st[4]) * LOG2E_F);
-      q[i] = inside ? __builtin_amdgcn_exp2f(((elem_to_f32<FMT>(r.z[j]) - st[2]) * plan.inv_tau - st[3]) * LOG2E_F) : 0.f;
+      p[i] = j < 0 ? 0.f : ds_exp(ds_value(a, row, i), st[6], plan.c, plan.lo) * st[4];
+      q[i] = inside ? ds_exp(elem_to_f32<FMT>(r.z[j]), st[2], plan.c, plan.lo) * st[3] : 0.f;
     }
   }
   if (in) {
@@ -1101,7 +1120,7 @@ extern "C" int64_t rumpy_distill_partial_floats(int64_t rows, int32_t V) {
 }
 
 // Lanes of a short row; 0: a workgroup a row, or more.  us, bf16, forward + gradient, 16 lanes | 64 lanes | a workgroup a row:
-//   65536 x 100, k 8: 20 + 11 | 87 + 29 | 468 + 218     4096 x 256, k 64: 11 + 7 | 9 + 5 | 40 + 13      300 x 1000, k 8: 11 + 6 | 6 + 4 | 8 + 4
+//   65536 x 100, k 8: 23 + 11 | 87 + 29 | 468 + 218     4096 x 256, k 64: 11 + 7 | 10 + 5 | 40 + 13     300 x 1000, k 8: 11 + 6 | 7 + 4 | 8 + 4
 //   16384 x 1000, k 8: 18 + 14 | 30 + 15 | 113 + 45      1200 x 2000, k 8: 9 + 6 (64) | 14 + 6      300 x 4000, k 8: 11 + 7 (64) | 7 + 4
 //   4096 x 4000, k 64: 18 + 14 (64) | 43 + 18            4096 x 8192, k 8: 24 + 24 (64) | 35 + 23     1200 x 8000, k 8: 19 + 13 (64) | 14 + 9
 //   8192 x 12001, k 8: 54 + 83 (64) | 91 + 75            2048 x 16000, k 8: 28 + 25 (64) | 24 + 22

@@ -667,3 +667,48 @@ def test_short_rows_captured_and_on_other_streams(rows, cols):
         side.synchronize()
         want = _pass(z, t, 20, 1.0)
         assert all(torch.equal(a, b) and torch.equal(b, c) for a, b, c in zip(out, want, other))
+
+
+@pytest.mark.parametrize('dtype', [F32, BF16, F16], ids=str)
+@pytest.mark.parametrize('apart', [0.5, 0.02])
+@pytest.mark.parametrize('rows,cols,k,tau,each', [(3, 168911, 1, 4.0, 16), (2, 33007, 2, 2.0, 16), (356, 2950, 213, 4.0, 48), (40, 30000, 64, 2.0, 64), (8200, 100, 4, 4.0, 8),
+                                                  (600, 12001, 8, 8.0, 32)])
+def test_a_student_close_to_its_teacher(rows, cols, k, tau, each, apart, dtype):
+    """the loss is of second order in the difference of the two distributions, with p_l and q_l their listed mass about tau^2 (p_l - q_l)^2 / 2 p_l: no error of the first order may
+    enter it.  The streamed sum s is off by E relative: 3 roundings of an exponent of at most the row's span, twice (the running maximum's factors), 2 of an
+    exponential, `each` columns a thread with half as many roundings for the factors, the joins of lanes, waves and pieces (64 are enough).  It moves
+    q_l by q_l q_t E and, both distributions being of sum 1, the loss by tau^2 (|p_l - q_l| E + q_l E^2).  An unlisted column's gradient (q_t - p_t) r, r = exp / s, is
+    off by r q_l E and E relative for its own quotient, a listed one's q - p by E q, both by their exponentials' roundings and 16 of the factors."""
+    g = torch.Generator().manual_seed(rows + cols)
+    z = torch.randn(rows, cols, generator=g).mul(3).to(dtype)
+    t = z.double() + apart * torch.randn(rows, cols, generator=g).double()
+    v, i = torch.sort(t, dim=1, descending=True)
+    tail = torch.logsumexp(v[:, k:] / tau, 1).float()
+    values, indices = v[:, :k].to(dtype), i[:, :k].contiguous()
+    del t, v, i
+    zd = z.to(DEV).requires_grad_()
+    got = distill_loss(zd, values.to(DEV), indices.to(DEV), tail=tail.to(DEV), temperature=tau, reduction='none')
+    scale = 2.0 ** 12                                               # (fp16 gradients in range)
+    grad, = torch.autograd.grad(got, zd, torch.full((rows,), scale, device=DEV))
+    u, uv = z.double() / tau, values.double() / tau
+    lp = torch.log_softmax(torch.cat([uv, tail.double()[:, None]], 1), 1)
+    lse = torch.logsumexp(u, 1, keepdim=True)
+    rest = u.scatter(1, indices, -INF)
+    lrest = torch.logsumexp(rest, 1, keepdim=True)
+    lq = torch.cat([torch.gather(u, 1, indices) - lse, lrest - lse], 1)
+    p, q = lp.exp(), lq.exp()
+    want = tau ** 2 * (p * (lp - lq)).sum(1)
+    span, pl, ql = u.amax(1) - u.amin(1), p[:, :k].sum(1), q[:, :k].sum(1)
+    E = U24 * (6 * span + 2 * each + 64)
+    tol = tau ** 2 * ((pl - ql).abs() * E + ql * E * E) + 2 * U24 * want.abs()
+    off = (got.detach().double().cpu() - want).abs()
+    assert bool((off <= tol).all()), (float((off / want).max()), float((off / tol).max()))
+    r = (rest - lrest).exp()
+    want = r * (q[:, k:] - p[:, k:])
+    tol = r * (ql * E)[:, None] + want.abs() * (E + U24 * (3 * span + 16))[:, None]
+    vspan = uv.amax(1) - uv.amin(1)
+    want.scatter_(1, indices, q[:, :k] - p[:, :k])
+    tol.scatter_(1, indices, (q + p)[:, :k] * (E + U24 * (3 * (span + vspan) + 16))[:, None])
+    tol = scale * tau * (tol + STEP[dtype] * (want.abs() + tol)) + (2.0 ** -25 if dtype == F16 else 2.0 ** -126) + 2 * scale * tau * 2.0 ** -126
+    off = (grad.double().cpu() - scale * tau * want).abs()
+    assert bool((off <= tol).all()), float((off / tol).max())
