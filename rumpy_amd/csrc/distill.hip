@@ -726,7 +726,8 @@ __device__ __forceinline__ void ds_finish(const rumpy_distill_args& a, const DsP
     P += p_rest;
     S = lanes_sum64<L>(q_listed, lane) + q_rest;
   }
-  nan |= P != P;                                           // (infinite logits of the teacher)
+  // (infinite logits of the teacher; NaN in the streamed columns, which their maximum passes over: m may be -inf beside it)
+  nan |= P != P || s != s;
   const double ln = log(lane % 4 == 0 ? P : lane % 4 == 1 ? S : (double)s);
   const double ln_p = __shfl(ln, 0, L), ln_s = __shfl(ln, 1, L), ln_r = __shfl(ln, 2, L), one_p = 1.0 / P, one_s = 1.0 / S;
   loss = (loss - p_listed * (ln_p - ln_s)) * one_p;

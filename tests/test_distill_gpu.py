@@ -712,3 +712,28 @@ def test_a_student_close_to_its_teacher(rows, cols, k, tau, each, apart, dtype):
     tol = scale * tau * (tol + STEP[dtype] * (want.abs() + tol)) + (2.0 ** -25 if dtype == F16 else 2.0 ** -126) + 2 * scale * tau * 2.0 ** -126
     off = (grad.double().cpu() - scale * tau * want).abs()
     assert bool((off <= tol).all()), float((off / tol).max())
+
+
+@pytest.mark.parametrize('dtype', [F32, BF16, F16], ids=str)
+@pytest.mark.parametrize('rows,cols', [(4, 3), (40, 100), (8200, 3), (40, 700), (40, 9000), (2, 70001)])
+def test_nan_beside_nothing_but_masked_columns(rows, cols, dtype):
+    """one unlisted column is NaN and every other unlisted one -inf, in the whole row or in its piece's part alone: softmax of such a row is NaN"""
+    k = 2
+    g = torch.Generator().manual_seed(cols)
+    for place in (0, cols // 2, cols - 1):
+        for alone in (True, False):
+            z = torch.randn(rows, cols, generator=g)
+            free = [j for j in range(cols) if j != place]
+            listed = torch.tensor([free[0], free[-1]])
+            if alone:
+                keep = z[0, listed].clone()
+                z[0] = -INF
+                z[0, listed] = keep
+            z[0, place] = NAN
+            values, indices = torch.randn(rows, k, generator=g), listed.expand(rows, k)
+            for tail in (0.3, -INF, None):
+                zd = z.to(dtype).to(DEV).requires_grad_()
+                out = distill_loss(zd, values.to(DEV), indices.to(DEV), tail=None if tail is None else torch.full((rows,), tail, device=DEV), reduction='none')
+                grad, = torch.autograd.grad(out.sum(), zd)
+                assert out.isnan().tolist() == [True] + [False] * (rows - 1), (place, alone, tail, float(out[0]))
+                assert grad[0].isnan().all() and grad[1:].isfinite().all(), (place, alone, tail)
