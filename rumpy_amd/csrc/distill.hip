@@ -116,9 +116,11 @@ template <int WG, int LOW> __device__ __forceinline__ uint32_t bound_of(uint32_t
   for (int i = 1; i < WG / 64; ++i) b = min(b, __float_as_uint(sh.red[i]));
   return b;
 }
-// the value that k of the workgroup's `mine` reach: the same search over all waves, a barrier per bit (two buffers in turn)
+// the value that k of the workgroup's `mine` reach: the same search over all waves, a barrier per bit (two buffers in turn, and one barrier in front: with fp16's
+// LOW a search ends in the buffer that the next one begins with, and a row without a finite bound is searched twice)
 template <int WG, int LOW> __device__ __forceinline__ uint32_t bound_of_all(uint32_t mine, int k, TlShared<WG>& sh) {
   uint32_t t = 0;
+  __syncthreads();
   for (int bit = 31; bit >= LOW; --bit) {
     const uint32_t trial = t | (1u << bit);
     uint32_t* n = sh.hist + (bit & 1) * (WG / 64);

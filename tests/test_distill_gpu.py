@@ -737,3 +737,18 @@ def test_nan_beside_nothing_but_masked_columns(rows, cols, dtype):
                 grad, = torch.autograd.grad(out.sum(), zd)
                 assert out.isnan().tolist() == [True] + [False] * (rows - 1), (place, alone, tail, float(out[0]))
                 assert grad[0].isnan().all() and grad[1:].isfinite().all(), (place, alone, tail)
+
+
+@pytest.mark.parametrize('dtype', [F16, BF16, F32], ids=str)
+@pytest.mark.parametrize('rows,cols,k', [(2000, 3000, 64), (600, 9000, 128), (300, 20000, 256)])
+def test_top_logits_of_many_rows_without_a_finite_bound(rows, cols, k, dtype):
+    """rows of which masks leave fewer than k columns, or with more than k infinities: the search for a bound runs twice over all waves"""
+    g = torch.Generator().manual_seed(cols)
+    z = torch.full((rows, cols), -INF)
+    for r in range(rows):
+        at = torch.randint(0, cols, (k - 3,), generator=g)
+        z[r, at] = torch.randn(k - 3, generator=g)
+    z[::3] = torch.randn(len(z[::3]), cols, generator=g)
+    z[::3].masked_fill_(torch.rand(len(z[::3]), cols, generator=g) < 2.0 * k / cols, INF)
+    z = z.to(dtype).to(DEV)
+    _check_top(z, k, 1.0)
