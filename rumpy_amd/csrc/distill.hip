@@ -51,6 +51,15 @@ template <int WAVES> __device__ __forceinline__ float block_max(float v, float* 
   return s;
 }
 
+// A launch has fewer than 2^32 threads along a dimension: calls of more rows than that holds (8.4 million at 512 threads a row) go in parts, each with the
+// arguments of its own rows.  fn(first row, rows)
+template <typename Fn> static void rows_in_parts(int64_t rows, int64_t threads_a_row, Fn fn) {
+  const int64_t most = 0xffffff00ll / threads_a_row / 16 * 16;         // (whole workgroups of rows that share one)
+  for (int64_t r = 0; r < rows; r += most) fn(r, rows - r < most ? rows - r : most);
+}
+static size_t elem_bytes(int fmt) { return fmt == RUMPY_FMT_F32 ? 4 : 2; }
+template <typename T> static void advance(T*& p, int64_t bytes) { if (p) p = (T*)((const char*)p + bytes); }
+
 // ================================================================================================================ selection
 // order of the values as unsigned integers: -inf lowest, NaN highest, -0 = +0
 __device__ __forceinline__ uint32_t order_key(float v) {
@@ -546,6 +555,16 @@ template <int FMT, int WG> static void tl_launch_wg(const rumpy_top_logits_args&
   else if (np <= 8 && MOST > 8) hipLaunchKernelGGL((top_logits_kernel<FMT, WG, (MOST > 8 ? 8 : MOST)>), grid, wg, 0, s, a, plan);
   else hipLaunchKernelGGL((top_logits_kernel<FMT, WG, MOST>), grid, wg, 0, s, a, plan);
 }
+// (rows that are cut are few: never in parts)
+template <int FMT, int WG> static void tl_launch_parts(const rumpy_top_logits_args& a, const TlPlan& plan, hipStream_t s) {
+  rows_in_parts(a.rows, (int64_t)WG * plan.splits, [&](int64_t r, int64_t n) {
+    rumpy_top_logits_args b = a;
+    const int64_t e = elem_bytes(FMT);
+    b.rows = n;
+    advance(b.logits, r * a.ld * e); advance(b.values, r * a.k * e); advance(b.indices, r * a.k * 8); advance(b.tail, r * 4);
+    tl_launch_wg<FMT, WG>(b, plan, s);
+  });
+}
 template <int FMT> static void tl_launch(const rumpy_top_logits_args& a, const TlPlan& plan, hipStream_t s) {
   // Short rows: small workgroups, more rows at once (a row is a chain of latencies: bound, lists, places) and no barriers in one of 64.  At least 2 k threads,
   // so that the bound comes from the better half of the threads' maxima (with k threads the lists run over: 65536 x 1000, k 64: 808 us with 64).
@@ -553,10 +572,10 @@ template <int FMT> static void tl_launch(const rumpy_top_logits_args& a, const T
   // 4096 x 1000, k 64: - | 14 | 18 | 37     4096 x 4000, k 48: - | 17 | 22 | 38     4096 x 8000, k 96: - | - | 33 | 48     4096 x 600, k 192: - | - | 39 | 49
   // 32 x 1000, k 4: 4.8 | 4.7 | 5.2 | 6.8     32 x 4000, k 64: - | 9.7 | 6.5 | 6.6     32 x 16000, k 64: - | - | 10 | 8
   const bool few = a.rows < 256, many = a.rows >= 1024;
-  if (a.k <= 32 && a.V <= (many ? 2048 : 1024)) tl_launch_wg<FMT, 64>(a, plan, s);
-  else if (a.k <= 64 && a.V <= (many ? 4096 : 2048)) tl_launch_wg<FMT, 128>(a, plan, s);
-  else if (few ? a.k <= 96 && a.V <= 4096 : a.k <= 128 ? a.V <= 16384 : many && a.k <= 192 && a.V <= 2048) tl_launch_wg<FMT, 256>(a, plan, s);
-  else tl_launch_wg<FMT, 512>(a, plan, s);
+  if (a.k <= 32 && a.V <= (many ? 2048 : 1024)) tl_launch_parts<FMT, 64>(a, plan, s);
+  else if (a.k <= 64 && a.V <= (many ? 4096 : 2048)) tl_launch_parts<FMT, 128>(a, plan, s);
+  else if (few ? a.k <= 96 && a.V <= 4096 : a.k <= 128 ? a.V <= 16384 : many && a.k <= 192 && a.V <= 2048) tl_launch_parts<FMT, 256>(a, plan, s);
+  else tl_launch_parts<FMT, 512>(a, plan, s);
   if (plan.splits > 1) hipLaunchKernelGGL((top_join_kernel<FMT>), dim3((unsigned)a.rows), dim3(512), 0, s, a, plan);
 }
 extern "C" int rumpy_top_logits(const rumpy_top_logits_args* p, void* stream) {
@@ -568,7 +587,7 @@ extern "C" int rumpy_top_logits(const rumpy_top_logits_args* p, void* stream) {
   if (!bad && p->rows && (!p->logits || !p->values || !p->indices || !p->tail)) bad = "a tensor is missing";
   if (!bad && rumpy_top_logits_work_bytes(p->rows, p->V, p->k) && (!p->work || ((uintptr_t)p->work & 7)))
     bad = "rows of this length and number are cut and need `work` (rumpy_top_logits_work_bytes, at a multiple of 8)";
-  if (!bad && p->rows > 0x7fffffff) bad = "too many rows";
+  if (!bad && p->rows > 0x7fffffff) bad = "at most 2^31 - 1 rows";
   if (bad) { rumpy_set_error("rumpy_top_logits: %s", bad); return RUMPY_E_ARG; }
   if (p->rows == 0) return RUMPY_OK;
   const TlPlan plan = tl_plan(p->rows, p->V, p->tau);
@@ -1111,8 +1130,8 @@ static const char* ds_check(const rumpy_distill_args* p) {
   if (!(p->tau >= 1e-30 && p->tau <= 1e30)) return "a temperature above zero";
   if (p->rows && (!p->logits || !p->top_values || !p->top_indices || !p->row_loss || !p->state)) return "a tensor is missing";
   if (p->loss && !p->factor) return "the reduction's factor is missing";
+  if (p->rows > 0x7fffffff) return "at most 2^31 - 1 rows";
   const DsPlan plan = ds_plan(p->rows, p->V, p->tau);
-  if (p->rows * plan.splits > 0x7fffffff) return "too many rows";
   if (plan.splits > 1 && !p->partial) return "rows of this length and number are cut and need `partial` (rumpy_distill_partial_floats)";
   return nullptr;
 }
@@ -1134,6 +1153,16 @@ static int ds_short(int64_t rows, int32_t V, int32_t k, bool fwd) {
   if (V <= 1024) return 64;
   return rows * 4 >= V && V <= (!fwd ? 4096 : rows >= 4096 ? 16384 : 8192) ? 64 : 0;
 }
+static rumpy_distill_args ds_part(const rumpy_distill_args& a, const DsPlan& plan, int64_t r, int64_t n) {
+  rumpy_distill_args b = a;
+  b.rows = n;
+  advance(b.logits, r * a.ld * elem_bytes(a.fmt)); advance(b.top_values, r * a.k * elem_bytes(a.value_fmt)); advance(b.top_indices, r * a.k * (a.index64 ? 8 : 4));
+  advance(b.tail, r * 4); advance(b.row_weight, r * 4); advance(b.row_loss, r * 4); advance(b.state, r * DS_STATE * 4);
+  advance(b.dlogits, r * a.V * elem_bytes(a.fmt));
+  if (plan.splits > 1) advance(b.partial, r * plan.splits * 8);
+  if (!a.loss) advance(b.gout, r * 4);
+  return b;
+}
 template <int FMT, int TPR> static void ds_launch_short_fwd(const rumpy_distill_args& a, const DsPlan& plan, hipStream_t s) {
   constexpr int SUB = 256 / TPR;
   const dim3 grid((unsigned)((a.rows + SUB - 1) / SUB));
@@ -1141,22 +1170,28 @@ template <int FMT, int TPR> static void ds_launch_short_fwd(const rumpy_distill_
   if (a.tail) hipLaunchKernelGGL((distill_short_fwd_kernel<FMT, true, TPR>), grid, dim3(256), lds, s, a, plan);
   else hipLaunchKernelGGL((distill_short_fwd_kernel<FMT, false, TPR>), grid, dim3(256), lds, s, a, plan);
 }
-template <int FMT> static void ds_launch_bwd(const rumpy_distill_args& a, const DsPlan& plan, hipStream_t s) {
-  const int tpr = ds_short(a.rows, a.V, a.k, false);
-  const size_t lds = tpr ? ds_short_lds(a.V, a.k, 256 / tpr, false) : 0;
-  if (tpr == 16) hipLaunchKernelGGL((distill_short_bwd_kernel<FMT, 16>), dim3((unsigned)((a.rows + 15) / 16)), dim3(256), lds, s, a, plan);
-  else if (tpr == 64) hipLaunchKernelGGL((distill_short_bwd_kernel<FMT, 64>), dim3((unsigned)((a.rows + 3) / 4)), dim3(256), lds, s, a, plan);
-  else hipLaunchKernelGGL((distill_bwd_kernel<FMT>), dim3((unsigned)(a.rows * plan.splits)), dim3(DS_WG), 0, s, a, plan);
+template <int FMT> static void ds_launch_bwd(const rumpy_distill_args& all, const DsPlan& plan, hipStream_t s) {
+  const int tpr = ds_short(all.rows, all.V, all.k, false);
+  const size_t lds = tpr ? ds_short_lds(all.V, all.k, 256 / tpr, false) : 0;
+  rows_in_parts(all.rows, tpr ? tpr : (int64_t)DS_WG * plan.splits, [&](int64_t r, int64_t n) {
+    const rumpy_distill_args a = ds_part(all, plan, r, n);
+    if (tpr == 16) hipLaunchKernelGGL((distill_short_bwd_kernel<FMT, 16>), dim3((unsigned)((n + 15) / 16)), dim3(256), lds, s, a, plan);
+    else if (tpr == 64) hipLaunchKernelGGL((distill_short_bwd_kernel<FMT, 64>), dim3((unsigned)((n + 3) / 4)), dim3(256), lds, s, a, plan);
+    else hipLaunchKernelGGL((distill_bwd_kernel<FMT>), dim3((unsigned)(n * plan.splits)), dim3(DS_WG), 0, s, a, plan);
+  });
 }
-template <int FMT> static void ds_launch_fwd(const rumpy_distill_args& a, const DsPlan& plan, hipStream_t s) {
-  const int tpr = ds_short(a.rows, a.V, a.k, true);
-  if (tpr == 16) return ds_launch_short_fwd<FMT, 16>(a, plan, s);
-  if (tpr == 64) return ds_launch_short_fwd<FMT, 64>(a, plan, s);
-  const dim3 grid((unsigned)(a.rows * plan.splits));
-  const size_t lds = a.tail ? ((size_t)(plan.splits == 1 ? a.V : plan.seg) + 7 + 31) / 32 * 4 : 0;
-  if (a.tail) hipLaunchKernelGGL((distill_fwd_kernel<FMT, true>), grid, dim3(DS_WG), lds, s, a, plan);
-  else hipLaunchKernelGGL((distill_fwd_kernel<FMT, false>), grid, dim3(DS_WG), 0, s, a, plan);
-  if (plan.splits > 1) hipLaunchKernelGGL((distill_join_kernel<FMT>), dim3((unsigned)a.rows), dim3(DS_WG), 0, s, a, plan);
+template <int FMT> static void ds_launch_fwd(const rumpy_distill_args& all, const DsPlan& plan, hipStream_t s) {
+  const int tpr = ds_short(all.rows, all.V, all.k, true);
+  rows_in_parts(all.rows, tpr ? tpr : (int64_t)DS_WG * plan.splits, [&](int64_t r, int64_t n) {
+    const rumpy_distill_args a = ds_part(all, plan, r, n);
+    if (tpr == 16) return ds_launch_short_fwd<FMT, 16>(a, plan, s);
+    if (tpr == 64) return ds_launch_short_fwd<FMT, 64>(a, plan, s);
+    const dim3 grid((unsigned)(n * plan.splits));
+    const size_t lds = a.tail ? ((size_t)(plan.splits == 1 ? a.V : plan.seg) + 7 + 31) / 32 * 4 : 0;
+    if (a.tail) hipLaunchKernelGGL((distill_fwd_kernel<FMT, true>), grid, dim3(DS_WG), lds, s, a, plan);
+    else hipLaunchKernelGGL((distill_fwd_kernel<FMT, false>), grid, dim3(DS_WG), 0, s, a, plan);
+    if (plan.splits > 1) hipLaunchKernelGGL((distill_join_kernel<FMT>), dim3((unsigned)n), dim3(DS_WG), 0, s, a, plan);
+  });
 }
 extern "C" int rumpy_distill_fwd(const rumpy_distill_args* p, void* stream) {
   const char* bad = ds_check(p);

@@ -752,3 +752,53 @@ def test_top_logits_of_many_rows_without_a_finite_bound(rows, cols, k, dtype):
     z[::3].masked_fill_(torch.rand(len(z[::3]), cols, generator=g) < 2.0 * k / cols, INF)
     z = z.to(dtype).to(DEV)
     _check_top(z, k, 1.0)
+
+
+# A launch has fewer than 2^32 threads: calls of more rows go in parts.  Rows overlap in memory (row r begins at element r), so that many of them take little.
+def _overlapping(rows, cols, dtype, seed):
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    return torch.randn(rows + cols, generator=g, device=DEV).mul(2).to(dtype).as_strided((rows, cols), (1, 1))
+
+
+def _about(rows, border):
+    return torch.tensor(sorted({r for b in (0, border, rows) for r in range(b - 4, b + 4) if 0 <= r < rows}), device=DEV)
+
+
+@pytest.mark.parametrize('rows,cols,k,threads', [(2 ** 26 + 9, 8, 1, 64), (2 ** 23 + 9, 300, 256, 512)])
+def test_top_logits_of_more_rows_than_a_launch_holds(rows, cols, k, threads):
+    z = _overlapping(rows, cols, BF16, 41)
+    pick = _about(rows, 0xffffff00 // threads // 16 * 16)
+    values, indices, tail = top_logits(z, k)
+    order, want = _top_reference(z[pick].cpu(), k, 1.0)
+    assert torch.equal(indices[pick].cpu(), order) and torch.equal(values[pick].cpu(), torch.gather(z[pick].cpu(), 1, order))
+    # (logarithms of up to 299 numbers of at most 2 x 6 widths: the tolerance of _check_top at its largest)
+    assert float((tail[pick].double().cpu() - want).abs().max()) <= U24 * (8 * 12 + 64 + 2 + 18)
+
+
+@pytest.mark.parametrize('rows,cols,threads,train', [(2 ** 28 + 9, 8, 16, True), (2 ** 23 + 9, 4100, 512, True), (2 ** 23 + 9, 16400, 512, False)])
+@pytest.mark.parametrize('rest', [False, True])
+def test_loss_of_more_rows_than_a_launch_holds(rows, cols, threads, train, rest):
+    z = _overlapping(rows, cols, BF16, 42).detach().requires_grad_(train)
+    values = _overlapping(rows, 1, BF16, 43)
+    indices = torch.remainder(torch.arange(rows, dtype=torch.int32, device=DEV), cols)[:, None]
+    tail = torch.zeros(rows, device=DEV) if rest else None
+    weight = torch.ones(rows, device=DEV)
+    weight[::3] = 0.5
+    got = distill_loss(z, values, indices, tail=tail, row_weight=weight, reduction='none')
+    pick = _about(rows, 0xffffff00 // threads // 16 * 16)
+    part = lambda t: None if t is None else t.detach()[pick].cpu()
+    one = torch.ones(len(pick), dtype=torch.float64)
+    loss, want, mag, err, tiny = _loss_reference(part(z), part(values), part(indices), part(tail), 1.0, part(weight).double(), one)
+    assert bool(((part(got).double() - loss).abs() <= 3 * err + 16 * U24 * loss.abs()).all())
+    if not train:
+        return
+    up = torch.ones(rows, device=DEV)
+    grad, = torch.autograd.grad(got, z, up)
+    step = STEP[BF16]
+    tol = (step * want.abs() + 3 * err[:, None] * mag) * (1 + step) + 2.0 ** -126 + tiny
+    assert bool(((part(grad).double() - want).abs() <= tol).all())
+    if cols > 8:
+        return
+    total = distill_loss(z, values, indices, tail=tail, row_weight=weight, reduction='sum')
+    whole = got.detach().sum(dtype=torch.float64)
+    assert abs(float(total.detach()) - float(whole)) <= 2 * U24 * float(whole)
