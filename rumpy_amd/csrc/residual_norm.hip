@@ -411,6 +411,7 @@ template <int XF, int TF, int TPR, int MODE> __global__ void __launch_bounds__(T
 // of one: a workgroup for 64 of them took 81 us for 32768 gate rows of 64 channels, 1650 for 700000 of 3; so 9 and 11.
 constexpr int RN_SLICES = 16, RN_REDUCE_WG = 64 * RN_SLICES;
 constexpr int64_t RN_FLAT = 16384;            // elements of gate rows from which on a thread takes one
+constexpr int64_t RN_FLAT_BLOCKS = 8192;      // their workgroups at most (a launch has fewer than 2^32 threads), which walk over the elements
 __device__ __forceinline__ const float* gate_partials(const rumpy_residual_norm_bwd_args& a, const RnPlan& plan, int64_t group, int64_t& count) {
   const int64_t first = group * a.group_rows, last = min(a.rows, first + a.group_rows) - 1;
   const float* src = a.partial + (size_t)4 * plan.wgs * a.C;
@@ -426,14 +427,16 @@ __global__ void __launch_bounds__(RN_REDUCE_WG) residual_norm_reduce_kernel(rump
   float* dst;
   int64_t count;
   if (item >= 4 && flat) {
-    const int64_t e0 = (int64_t)(blockIdx.x - 4 * tiles) * RN_REDUCE_WG, e = e0 + threadIdx.x, g0 = e0 / a.C;
-    if (e >= flat) return;                                     // (no barrier on this way)
-    const uint32_t off = (uint32_t)(e0 - g0 * a.C) + threadIdx.x;
-    src = gate_partials(a, plan, g0 + off / (uint32_t)a.C, count) + off % (uint32_t)a.C;
-    float s = 0.f;
+    const int64_t step = (int64_t)(gridDim.x - 4 * tiles) * RN_REDUCE_WG;
+    for (int64_t e0 = (int64_t)(blockIdx.x - 4 * tiles) * RN_REDUCE_WG; e0 + threadIdx.x < flat; e0 += step) {
+      const int64_t g0 = e0 / a.C;
+      const uint32_t off = (uint32_t)(e0 - g0 * a.C) + threadIdx.x;
+      src = gate_partials(a, plan, g0 + off / (uint32_t)a.C, count) + off % (uint32_t)a.C;
+      float s = 0.f;
 #pragma unroll 4
-    for (int64_t i = 0; i < count; ++i) s += src[(size_t)i * a.C];
-    ((float*)a.dgate)[e] = s;
+      for (int64_t i = 0; i < count; ++i) s += src[(size_t)i * a.C];
+      ((float*)a.dgate)[e0 + threadIdx.x] = s;
+    }
     return;
   }
   const int lane = threadIdx.x & 63, slice = threadIdx.x >> 6, c = (blockIdx.x % tiles) * 64 + lane;
@@ -572,8 +575,8 @@ extern "C" int rumpy_residual_norm_bwd(const rumpy_residual_norm_bwd_args* p, vo
   const bool gate_rows = !bad && p->gate_mode == RN_GATE_GROUP && p->dgate && !(plan.direct && p->group_rows == 1);
   const int tiles = bad ? 0 : (p->C + 63) / 64;
   const int64_t groups = gate_rows ? p->rows / p->group_rows : 0, elements = groups > 1 ? groups * p->C : 0, flat = elements >= RN_FLAT ? elements : 0;
-  const int64_t blocks = (flat ? 4 : 4 + groups) * tiles + (flat + RN_REDUCE_WG - 1) / RN_REDUCE_WG;
-  if (!bad && blocks > 0x7fffffff) bad = "too many gate rows";
+  const int64_t walk = (flat + RN_REDUCE_WG - 1) / RN_REDUCE_WG;
+  const int64_t blocks = (flat ? 4 : 4 + groups) * tiles + (walk < RN_FLAT_BLOCKS ? walk : RN_FLAT_BLOCKS);
   if (bad) { rumpy_set_error("rumpy_residual_norm_bwd: %s", bad); return RUMPY_E_ARG; }
   hipStream_t s = (hipStream_t)stream;
   RN_BY_FORMAT(rn_launch_bwd, *p, plan, s);

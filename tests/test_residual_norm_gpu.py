@@ -565,3 +565,8 @@ def test_few_channels(c):
     for gate, shape in (('none', (1, 1031, c)), ('channel', (3, 700, c)), ('group', (9, 130, c)), ('group', (5, 300, c)), ('full', (1, 517, c))):
         _run_and_check(shape, BF16, BF16, gate, 'layer', 'rms', True, 0.7)
         _run_and_check(shape, F32, F16, gate, 'rms', 'layer', True, 0.7, lay=lambda n, t: torch.nn.functional.pad(t, (1, 2))[..., 1:-2] if t.dim() > 2 else t)
+
+
+def test_more_elements_of_gate_rows_than_threads():
+    """8960000 of them: the threads that sum the gate rows' gradients walk over them"""
+    _run_and_check((140000, 2, 64), BF16, BF16, 'group', 'layer', 'layer', True, 0.7)
