@@ -410,8 +410,14 @@ template <int XF, int TF, int TPR, int MODE> __global__ void __launch_bounds__(T
 // with four a sum of 461 rows took 7 us of dependent loads.  Where there are many gate rows (`flat`), each of a few partial rows, a thread takes an element
 // of one: a workgroup for 64 of them took 81 us for 32768 gate rows of 64 channels, 1650 for 700000 of 3; so 9 and 11.
 constexpr int RN_SLICES = 16, RN_REDUCE_WG = 64 * RN_SLICES;
-constexpr int64_t RN_FLAT = 16384;            // elements of gate rows from which on a thread takes one
 constexpr int64_t RN_FLAT_BLOCKS = 8192;      // their workgroups at most (a launch has fewer than 2^32 threads), which walk over the elements
+// A thread's walk takes about 0.1 us a partial row, the workgroups of 64 columns 2.2 us a thousand: with more than 45 of them a partial row the threads win.  us,
+// threads | workgroups:  65536 gate rows of 64 channels, 2 partial rows each: 18 | 148     4096 x 64, 31: 7.5 | 16.5     64 x 4096, 6: 5 | 17
+// 1024 x 16, 127: 13.7 | 6.7     2048 x 8, 200: 19 | 14     8 x 4096, 33: 6.6 | 5.7     8 x 2048, 33: 8.2 | 4.9     2 x 8192, 130: 14 | 5.4
+static bool rn_flat(const RnPlan& plan, int64_t groups, int64_t group_rows, int tiles) {
+  const int64_t each = plan.direct ? group_rows : group_rows / plan.rpw + 2;
+  return groups * tiles > 45 * each;
+}
 __device__ __forceinline__ const float* gate_partials(const rumpy_residual_norm_bwd_args& a, const RnPlan& plan, int64_t group, int64_t& count) {
   const int64_t first = group * a.group_rows, last = min(a.rows, first + a.group_rows) - 1;
   const float* src = a.partial + (size_t)4 * plan.wgs * a.C;
@@ -574,7 +580,7 @@ extern "C" int rumpy_residual_norm_bwd(const rumpy_residual_norm_bwd_args* p, vo
   const RnPlan plan = bad ? RnPlan{} : rn_plan(p->rows, p->group_rows, p->C, p->gate_mode);
   const bool gate_rows = !bad && p->gate_mode == RN_GATE_GROUP && p->dgate && !(plan.direct && p->group_rows == 1);
   const int tiles = bad ? 0 : (p->C + 63) / 64;
-  const int64_t groups = gate_rows ? p->rows / p->group_rows : 0, elements = groups > 1 ? groups * p->C : 0, flat = elements >= RN_FLAT ? elements : 0;
+  const int64_t groups = gate_rows ? p->rows / p->group_rows : 0, flat = gate_rows && rn_flat(plan, groups, p->group_rows, tiles) ? groups * p->C : 0;
   const int64_t walk = (flat + RN_REDUCE_WG - 1) / RN_REDUCE_WG;
   const int64_t blocks = (flat ? 4 : 4 + groups) * tiles + (walk < RN_FLAT_BLOCKS ? walk : RN_FLAT_BLOCKS);
   if (bad) { rumpy_set_error("rumpy_residual_norm_bwd: %s", bad); return RUMPY_E_ARG; }

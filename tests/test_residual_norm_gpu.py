@@ -570,3 +570,9 @@ def test_few_channels(c):
 def test_more_elements_of_gate_rows_than_threads():
     """8960000 of them: the threads that sum the gate rows' gradients walk over them"""
     _run_and_check((140000, 2, 64), BF16, BF16, 'group', 'layer', 'layer', True, 0.7)
+
+
+@pytest.mark.parametrize('shape', [(2, 300, 8192), (8, 260, 2048), (500, 127, 16), (64, 6, 4096), (45, 9, 64), (46, 2, 64), (1, 700, 300)])
+def test_gate_rows_on_both_sides_of_their_summing_rule(shape):
+    """few long groups of wide rows, many short ones, and numbers beside the border between the two ways of summing a gate row's partial rows"""
+    _run_and_check(shape, BF16, BF16, 'group', 'layer', 'layer', True, 0.7)
