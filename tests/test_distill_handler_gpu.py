@@ -213,3 +213,28 @@ def test_calls_from_several_threads_at_once():
         got = list(pool.map(work, range(4)))
     for a, b in zip(want, got):
         assert all(torch.equal(s, t) for s, t in zip(a, b))
+
+
+def test_under_torch_modes():
+    """saved-tensor hooks, anomaly detection and autocast change nothing; transforms that hold no data of their own are refused"""
+    from rumpy_amd.residual_norm import residual_norm
+    g = torch.Generator().manual_seed(41)
+    x = torch.randn(6, 300, generator=g).to(DEV)
+    values, indices, tail = top_logits(torch.randn(6, 300, generator=g).to(DEV), 5)
+    weight = torch.ones(300, device=DEV)
+
+    def call():
+        leaf = x.clone().requires_grad_()
+        y, h = residual_norm(leaf, leaf * 2, post_norm='rms', post_weight=weight, pre_norm='layer')
+        loss = distill_loss(h + y, values, indices, tail=tail)
+        return [loss.detach(), torch.autograd.grad(loss, leaf)[0]]
+    want = call()
+    for mode in (torch.autograd.graph.save_on_cpu(), torch.autograd.set_detect_anomaly(True), torch.autocast('cuda', dtype=torch.bfloat16)):
+        with mode:
+            got = call()
+        assert all(torch.equal(a, b) for a, b in zip(want, got))
+    for fn in (lambda r: residual_norm(r, pre_norm='rms')[1], lambda r: top_logits(r, 3)[0], lambda r: distill_loss(r, values[0], indices[0])):
+        with pytest.raises(RuntimeError):
+            torch.vmap(fn)(x)
+        with pytest.raises(RuntimeError):
+            torch.func.grad(lambda r: fn(r).sum())(x[0])
