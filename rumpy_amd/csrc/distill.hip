@@ -357,7 +357,7 @@ template <int FMT, int WG> __device__ __forceinline__ float rest_below(const Row
 // value), it is infinite or a type's lowest value (fewer than about k columns that no mask holds), or there is NaN - the elements above T and, as
 // far as they do not suffice, those equal to it in the lowest columns; and where those are too many as well, the k-th pair by radix search.
 // Measured (MI355X): 2048 x 65521 bf16, k 100: 73 us = 3.7 TB/s (k 1: 62); 4096 x 8192 bf16, k 64: 28 us; 16384 x 1000 fp32, k 64: 37 us, k 4: 15; 32 x 8192
-// fp32: 8 us, one row's chain of latencies.  256 x 65521 with 100 valid columns or constant: 34 - 50 us (by radix search: 430 - 560; ascending
+// fp32: 8 us, one row's chain of latencies.  256 x 65521: 18 us; with 100 valid columns, constant, or with its largest in the first 1000: 34 - 50 us (by radix search: 430 - 560; ascending
 // rows still go that way).
 // Six waves a SIMD: three workgroups of 512 a CU, with most of a row each in registers (with two, 2048 rows of 65521 took 80 us instead of 70).
 template <int FMT, int WG, int NP> __global__ void __launch_bounds__(WG, 6) top_logits_kernel(rumpy_top_logits_args a, TlPlan plan) {
@@ -548,7 +548,9 @@ extern "C" int64_t rumpy_top_logits_work_bytes(int64_t rows, int32_t V, int32_t 
 template <int FMT, int WG> static void tl_launch_wg(const rumpy_top_logits_args& a, const TlPlan& plan, hipStream_t s) {
   const dim3 grid((unsigned)(a.rows * plan.splits)), wg(WG);
   const int len = a.V < plan.seg ? a.V : plan.seg, np = (len / 8 + WG - 1) / WG;
-  constexpr int MOST = WG <= 128 ? 4 : WG == 256 ? 8 : FMT == RUMPY_FMT_F32 ? 7 : 15;          // pieces in registers: the callers' limits; 60 registers
+  // pieces in registers: the callers' limits, and 60 registers at 512 threads.  (fp32 at 256 threads: 8 pieces are 64 registers of the 80 that six waves leave, 36 others
+  // lie in scratch: 4096 x 16384, k 64, 56 us = 4.8 TB/s.)
+  constexpr int MOST = WG <= 128 ? 4 : WG == 256 ? 8 : FMT == RUMPY_FMT_F32 ? 7 : 15;
   if (len <= 8 * WG) hipLaunchKernelGGL((top_logits_kernel<FMT, WG, 1>), grid, wg, 0, s, a, plan);
   else if (np <= 2) hipLaunchKernelGGL((top_logits_kernel<FMT, WG, 2>), grid, wg, 0, s, a, plan);
   else if (np <= 4) hipLaunchKernelGGL((top_logits_kernel<FMT, WG, 4>), grid, wg, 0, s, a, plan);
