@@ -32,5 +32,6 @@ def distill_loss(logits, top_values, top_indices, tail=None, temperature=1.0, ro
     row_weight   [...] or None: weights of the rows; a row of weight 0 (padding) is not looked at and gets no gradient.
     reduction    'mean' = sum(weight * l) / sum(weight) (0 when the weights sum to 0), 'sum', or 'none' = weight * l per row.
     The loss is float32, times temperature^2 so that its gradient's size does not depend on the temperature.  A row whose entries are all unused
-    or -inf contributes 0."""
+    or -inf contributes 0.  A probability of the teacher's under 2^-126 of its row's
+    largest counts as 0, also where the student gives the column none at all."""
     return (L.OPS or L.ops()).distill_loss(logits, top_values, top_indices, tail, temperature, row_weight, reduction)

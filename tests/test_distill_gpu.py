@@ -802,3 +802,17 @@ def test_loss_of_more_rows_than_a_launch_holds(rows, cols, threads, train, rest)
     total = distill_loss(z, values, indices, tail=tail, row_weight=weight, reduction='sum')
     whole = got.detach().sum(dtype=torch.float64)
     assert abs(float(total.detach()) - float(whole)) <= 2 * U24 * float(whole)
+
+
+@pytest.mark.parametrize('rest', [False, True])
+@pytest.mark.parametrize('cols', [3, 700, 9000, 70001])
+def test_a_probability_under_the_smallest_float_counts_as_zero(cols, rest):
+    """... relative to the largest of its row, whatever the student gives the column: where p = 2^-125 meets q = 0 the loss is infinite, where p = 2^-128 does it is what -inf leaves"""
+    z = torch.zeros(3, cols)
+    z[:, 1] = -INF
+    values, indices = torch.zeros(3, 2), torch.tensor([0, 1]).expand(3, 2)
+    values[:, 1] = torch.tensor([-125.0, -128.0, -INF]) * math.log(2.0)
+    tail = torch.full((3,), -1.0, device=DEV) if rest else None
+    # (with the rest the other probability is 1 / (1 + e^-1): the exponent of p falls by 0.46)
+    got = distill_loss(z.to(DEV), values.to(DEV), indices.to(DEV), tail=tail, reduction='none').cpu()
+    assert float(got[0]) == INF and math.isfinite(float(got[1])) and torch.equal(got[1], got[2])
